@@ -1,0 +1,379 @@
+"""The KV cache in 8 or 4 bits (ops.kernels *_mx, csrc/kv_mx.hip): its format against a search of the levels, writing and reading back
+against that, attention against float64 over the values the cache holds, and what the entry points refuse."""
+import math
+
+import pytest
+import torch
+
+from xotorch_support_jetson_amd.ops import kernels as K
+from xotorch_support_jetson_amd.ops import reference as ref
+from xotorch_support_jetson_amd.ops.rope import build_cos_sin
+
+FMTS = ("mxfp4", "mxfp8")
+PAGE = 64
+
+
+# ------------------------------------------------------------------ oracles
+def levels(fmt):
+  if fmt == "mxfp4":
+    return torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64)
+  return torch.tensor([(1 + c % 8 / 8) * 2.0 ** (c // 8 - 7) if c >= 8 else c / 8 * 2.0 ** -6 for c in range(127)], dtype=torch.float64)
+
+
+def held(x, fmt):
+  """The values that rows [..., Dh] of any type have in the cache, float64: the exponent by trying them all, elements by search."""
+  lv, top, high = levels(fmt), {"mxfp4": 7.0, "mxfp8": 464.0}[fmt], {"mxfp4": 125, "mxfp8": 119}[fmt]
+  g = x.double().cpu().unflatten(-1, (-1, 32))
+  a = g.abs().amax(-1, keepdim=True)
+  bad = ~torch.isfinite(a)
+  steps = torch.arange(-100, high + 1, dtype=torch.float64)
+  fits = torch.where(bad, 0.0, a) <= top * torch.exp2(steps)
+  e = torch.where(fits.any(-1, keepdim=True), fits.int().argmax(-1, keepdim=True) - 100, high).double()
+  y = (torch.where(bad, 0.0, g.abs()) / torch.exp2(e)).clamp(max=float(lv[-1]))
+  up = torch.searchsorted(lv, y.contiguous()).clamp(max=len(lv) - 1)
+  dn = (up - 1).clamp(min=0)
+  lower = (y - lv[dn] < lv[up] - y) | ((y - lv[dn] == lv[up] - y) & (dn % 2 == 0))
+  v = lv[torch.where(lower, dn, up)] * torch.exp2(e) * torch.sign(torch.where(bad, 1.0, g))
+  return torch.where(bad, float("nan"), v).flatten(-2)
+
+
+def pools(fmt, pages, Hkv, Dh, dev="cpu", fill=0):
+  n = K.mx_page_bytes(fmt, Dh)
+  return tuple(torch.full((pages, Hkv, n), fill, dtype=torch.uint8, device=dev) for _ in range(2))
+
+
+def attend64(q, k, v, scale, past):
+  """Causal attention in float64: q [n, H, Dh] at the end of k, v [past + n, Hkv, Dh]; also sum p |v| (rounding p moves the result by
+  a share of it) and sum |q k|."""
+  q, k, v = q.double().cpu(), k.double().cpu(), v.double().cpu()
+  G = q.shape[1] // k.shape[1]
+  k, v = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
+  s = torch.einsum("qhd,khd->hqk", q, k) * scale
+  mag = torch.einsum("qhd,khd->hqk", q.abs(), k.abs()).amax(-1) * scale
+  see = torch.arange(k.shape[0])[None] <= past + torch.arange(q.shape[0])[:, None]
+  p = torch.softmax(s.masked_fill(~see, float("-inf")), -1)
+  v = torch.where(see.any(0)[:, None, None], v, 0.0)
+  return torch.einsum("hqk,khd->qhd", p, v), torch.einsum("hqk,khd->qhd", p, v.abs()), mag.t()[..., None]
+
+
+def close(got, want, weight, mag):
+  """Per element: the result's rounding to bf16 (2^-8 of it), the probabilities' (2^-8 each, so 2^-8 of sum p |v|), and the scores'
+  error: products of 128 terms added in 32 bits (2^-17 of sum |q k|), the queries' split (2^-21 of the largest times sum |k|, within
+  128 2^-21 <= 2^-14 of sum |q k| only where few dims carry it all: 2^-16 is taken for both), which moves p by twice that share."""
+  got = got.double().cpu()
+  tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -15 * mag) * weight + 1e-30
+  assert torch.isfinite(got).all()
+  worst = ((got - want).abs() / tol).max().item()
+  assert worst <= 1.0, f"{worst} times the bound"
+
+
+class Seqs:
+  """Sequences of unlike length with pages in any order, and their cached values."""
+
+  def __init__(self, fmt, ctx, Hkv, Dh, seed=0, dev="cpu", width=None, spare=2):
+    g = torch.Generator().manual_seed(seed)
+    pages = [-(-c // PAGE) for c in ctx]
+    W = width or max(1, max(pages))
+    pool = sum(pages) + spare
+    self.tables = torch.zeros(len(ctx), W, dtype=torch.int32)
+    order = torch.randperm(pool, generator=g).tolist()
+    for b, n in enumerate(pages):
+      for w in range(n):
+        self.tables[b, w] = order.pop()
+    self.ctx, self.lens, self.fmt, self.Dh = torch.tensor(ctx, dtype=torch.int32), ctx, fmt, Dh
+    self.k, self.v = pools(fmt, pool, Hkv, Dh)
+    chan = torch.exp(0.5 * torch.randn(Hkv, Dh, generator=g))
+    self.kv = []
+    for b, n in enumerate(ctx):
+      k, v = torch.randn(n, Hkv, Dh, generator=g) * chan, torch.randn(n, Hkv, Dh, generator=g)
+      t = torch.arange(n)
+      ref.mx_write(k, v, self.tables[b].long()[t // PAGE] * PAGE + t % PAGE, self.k, self.v)
+      self.kv.append((held(k, fmt), held(v, fmt)))
+    self.to(dev)
+
+  def to(self, dev):
+    self.tables, self.ctx, self.k, self.v = (t.to(dev) for t in (self.tables, self.ctx, self.k, self.v))
+
+  def spoil(self):
+    """Every byte of the pools that holds no cached key becomes 0xff: NaN elements, and scales that read as NaN."""
+    dev = self.k.device
+    keep = ref.mx_read(self.k.cpu(), self.v.cpu(), torch.arange(self.k.shape[0]), self.Dh)
+    self.k, self.v = torch.full_like(self.k, 255).cpu(), torch.full_like(self.v, 255).cpu()
+    for b, n in enumerate(self.lens):
+      t = torch.arange(n)
+      at = self.tables[b].cpu().long()[t // PAGE], t % PAGE
+      ref.mx_write(keep[0][at[0], :, at[1]], keep[1][at[0], :, at[1]], at[0] * PAGE + at[1], self.k, self.v)
+    self.to(dev)
+
+
+def check_decode(s, H, scale, seed=1, **kw):
+  g = torch.Generator().manual_seed(seed)
+  q = (2 * torch.randn(len(s.lens), H, s.Dh, generator=g)).to(torch.bfloat16)
+  out = K.attn_decode_mx(q.to(s.k.device), s.k, s.v, s.tables, s.ctx, scale, **kw)
+  for b, n in enumerate(s.lens):
+    n = min(n, s.tables.shape[1] * PAGE)
+    if n <= 0:
+      assert (out[b] == 0).all()
+      continue
+    close(out[b:b + 1], *attend64(q[b:b + 1], s.kv[b][0][:n], s.kv[b][1][:n], scale, n - 1))
+  return out
+
+
+def check_prompt(s, new, H, scale, seed=1):
+  g = torch.Generator().manual_seed(seed)
+  cu = [0]
+  for n in new:
+    cu.append(cu[-1] + n)
+  q = (2 * torch.randn(cu[-1] + 3, H, s.Dh, generator=g)).to(torch.bfloat16)
+  dev = s.k.device
+  out = torch.full((cu[-1] + 3, H, s.Dh), 7.0, dtype=torch.bfloat16, device=dev)
+  K.attn_prefill_mx(q.to(dev), s.k, s.v, s.tables, torch.tensor(cu, dtype=torch.int32, device=dev), s.ctx, max(new), scale, out=out)
+  for b, n in enumerate(new):
+    if n:
+      close(out[cu[b]:cu[b + 1]], *attend64(q[cu[b]:cu[b + 1]], *s.kv[b], scale, s.lens[b] - n))
+  return out, cu[-1]
+
+
+def qkv_of(T, H, Hkv, Dh, seed=0):
+  g = torch.Generator().manual_seed(seed)
+  return torch.randn(T, (H + 2 * Hkv) * Dh, generator=g).mul(torch.exp(torch.randn(T, 1, generator=g))).to(torch.bfloat16)
+
+
+def rotated(x, pos, cs):
+  """fp32 rotation, each product and sum rounded by itself."""
+  c, s = cs[pos.long()][:, None].chunk(2, -1)
+  a, b = x.float().chunk(2, -1)
+  return torch.cat([a * c - b * s, b * c + a * s], -1)
+
+
+# ------------------------------------------------------------------ format
+@pytest.mark.parametrize("fmt", FMTS)
+def test_format(fmt):
+  g = torch.Generator().manual_seed(0)
+  lv, top = levels(fmt), {"mxfp4": 7.0, "mxfp8": 464.0}[fmt]
+  x = torch.randn(400, 32, generator=g) * torch.exp2(torch.randint(-130, 125, (400, 1), generator=g).float())
+  ties = torch.cat([(lv[:-1] + lv[1:]) / 2, lv]).float()  # with the largest element beside them, so that the exponent is 0
+  rows = [torch.cat([t, lv[-1:].float(), torch.zeros(31 - t.numel())]) * s for t in ties.split(31) for s in (1.0, -1.0, 2.0 ** 40)]
+  rows += [torch.cat([torch.tensor([v]), torch.ones(31)]) for v in (top, math.nextafter(top, 1e9) * (1 + 2e-7), -top, top * 2.0 ** -90)]
+  rows += [torch.zeros(32), torch.full((32,), 3e38), torch.full((32,), 1e-33), torch.full((32,), 2.0 ** -100)]
+  x = torch.cat([x, torch.stack(rows)])
+  code, scale = ref.mx_encode(x, fmt)
+  assert torch.equal(ref.mx_decode(code, scale, fmt).double(), held(x, fmt))
+  v = ref.mx_decode(code, scale, fmt)
+  assert torch.equal(v, v.to(torch.bfloat16).float())  # what the cache holds is exact in bf16
+  assert torch.equal(ref.mx_decode(*ref.mx_encode(v, fmt), fmt), v)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_format_not_finite(fmt):
+  x = torch.ones(4, 64)
+  x[0, 3], x[1, 40], x[2, 63] = float("nan"), float("inf"), float("-inf")
+  v = ref.mx_decode(*ref.mx_encode(x, fmt), fmt)
+  assert torch.isnan(v[0, :32]).all() and torch.isnan(v[1, 32:]).all() and torch.isnan(v[2, 32:]).all()
+  assert (v[0, 32:] == 1).all() and (v[1, :32] == 1).all() and (v[3] == 1).all()
+
+
+@pytest.mark.parametrize("fmt,Dh,Hkv", [("mxfp4", 128, 2), ("mxfp8", 64, 3)])
+def test_write_read(fmt, Dh, Hkv):
+  check_write(fmt, Dh, 4, Hkv, 150, "cpu")
+
+
+def check_write(fmt, Dh, H, Hkv, T, dev, seed=0):
+  """Tokens to pages in any order, some to none: the pools' values against the search, other keys' bytes untouched."""
+  g = torch.Generator().manual_seed(seed)
+  pool = T // PAGE + 3
+  slots = torch.randperm(pool * PAGE, generator=g)[:T]
+  slots[::7] = -1
+  slots[3::11] = pool * PAGE + 5
+  x, pos, cs = qkv_of(T, H, Hkv, Dh, seed), torch.randint(0, 5000, (T,), generator=g, dtype=torch.int32), build_cos_sin(Dh, 5000, 10000.0)
+  if T > 3:
+    pos[1], pos[2] = -4, 9999  # (rows outside the table: its first and last)
+  inside = pos.clamp(0, 4999)
+  rows = x.view(T, H + 2 * Hkv, Dh)
+  k, v = pools(fmt, pool, Hkv, Dh, fill=37)
+  before = ref.mx_read(k, v, torch.arange(pool), Dh)
+  kd, vd = k.to(dev), v.to(dev)
+  on_cpu = dev == "cpu"
+  q = K.rope_kv_write_mx(x.to(dev), (inside if on_cpu else pos).to(dev), cs.to(dev), slots.to(dev), kd, vd, H, Hkv)
+  want_q = rotated(rows[:, :H], inside, cs)
+  assert (q.cpu().float() - want_q).abs().le(2.0 ** -8 * want_q.abs() + 1e-30).all()
+  got = ref.mx_read(kd.cpu(), vd.cpu(), torch.arange(pool), Dh)
+  want_k, want_v = held(rotated(rows[:, H:H + Hkv], inside, cs), fmt), held(rows[:, H + Hkv:], fmt)
+  fresh = torch.zeros(pool * PAGE, dtype=torch.bool)
+  for t, s in enumerate(slots.tolist()):
+    if 0 <= s < pool * PAGE:
+      fresh[s] = True
+      assert torch.equal(got[0][s // PAGE, :, s % PAGE].double(), want_k[t]), t
+      assert torch.equal(got[1][s // PAGE, :, s % PAGE].double(), want_v[t]), t
+  for a, b in zip(got, before):
+    old = ~fresh.view(pool, 1, PAGE, 1).expand_as(a)
+    assert torch.equal(a[old].nan_to_num(-1.0), b[old].nan_to_num(-1.0))
+  # read back through tables: exact, zeros past the contexts, bad entries kept inside the pool
+  tables = torch.tensor([[1, 0], [pool - 1, -3], [pool + 7, 2]], dtype=torch.int32)
+  ctx = torch.tensor([100, 64, 1], dtype=torch.int32)
+  kb, vb = K.kv_read_mx(kd, vd, tables.to(dev), ctx.to(dev), Dh)
+  vb = ref.v_chunks(vb.cpu()).transpose(3, 4).flatten(2, 3)
+  for b in range(3):
+    for w in range(2):
+      n = max(0, min(PAGE, int(ctx[b]) - w * PAGE))
+      for out, src in ((kb.cpu(), got[0]), (vb, got[1])):
+        page = out[2 * b + w].float()
+        assert torch.equal(page[:, :n].nan_to_num(-1.0), src[min(max(int(tables[b, w]), 0), pool - 1)][:, :n].nan_to_num(-1.0))
+        assert (page[:, n:] == 0).all()
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("fmt,Dh", [("mxfp4", 128), ("mxfp8", 64)])
+def test_attention_cpu(fmt, Dh):
+  s = Seqs(fmt, [70, 0, 1, 128], 2, Dh, width=3)
+  check_decode(s, 4, Dh ** -0.5)
+  s = Seqs(fmt, [70, 5, 128], 2, Dh)
+  out, end = check_prompt(s, [10, 5, 1], 4, Dh ** -0.5)
+
+
+def test_formats_refused():
+  with pytest.raises(ValueError, match="mxfp4"):
+    K.mx_page_bytes("int4", 128)
+  k, v = pools("mxfp4", 2, 1, 128)
+  with pytest.raises(ValueError, match="heads of 64"):
+    K.mx_format(k, 64)
+  with pytest.raises(ValueError):
+    K.mx_format(k.to(torch.int8), 128)
+  with pytest.raises(ValueError):
+    ref.mx_format(torch.zeros(2, 1, K.mx_page_bytes("mxfp8", 32), dtype=torch.uint8), 32)
+
+
+# ------------------------------------------------------------------ kernels
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 5, 64, 333, 2100])
+@pytest.mark.parametrize("fmt,Dh,H,Hkv", [("mxfp4", 128, 4, 2), ("mxfp4", 64, 6, 3), ("mxfp8", 128, 7, 1), ("mxfp8", 64, 4, 4)])
+def test_write_read_gpu(gpu, fmt, Dh, H, Hkv, T):
+  check_write(fmt, Dh, H, Hkv, T, gpu, seed=T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_write_format_gpu(gpu, fmt):
+  """Ties, borders of the exponent, values that vanish, overflow and are not finite, written as values (no rotation)."""
+  lv, top = levels(fmt), {"mxfp4": 7.0, "mxfp8": 464.0}[fmt]
+  ties = torch.cat([(lv[:-1] + lv[1:]) / 2, lv, -lv]).float()
+  rows = [torch.cat([t, lv[-1:].float(), torch.zeros(31 - t.numel())]) * s for t in ties.split(31) for s in (1.0, 2.0 ** 40, 2.0 ** -90)]
+  rows += [torch.cat([torch.tensor([v]), torch.ones(31)]) for v in (top, top * (1 + 2.0 ** -7), -top, top * 2.0 ** -90)]
+  rows += [torch.zeros(32), torch.full((32,), 3e38), torch.full((32,), -3e38), torch.full((32,), 1e-33), torch.full((32,), 2.0 ** -100)]
+  for bad in (float("nan"), float("inf"), float("-inf")):
+    rows.append(torch.cat([torch.ones(9), torch.tensor([bad]), torch.ones(22)]))
+  while len(rows) % 4:
+    rows.append(torch.ones(32))
+  x = torch.stack(rows).to(torch.bfloat16).view(-1, 128)  # (what is no bf16 is rounded first)
+  T = x.shape[0]
+  k, v = pools(fmt, T // PAGE + 1, 1, 128, gpu)
+  cs = torch.cat([torch.ones(1, 64), torch.zeros(1, 64)], 1)
+  qkv = torch.cat([torch.zeros_like(x), x, x], 1)
+  K.rope_kv_write_mx(qkv.to(gpu), torch.zeros(T, dtype=torch.int32, device=gpu), cs.to(gpu), torch.arange(T, device=gpu), k, v, 1, 1)
+  got = ref.mx_read(k.cpu(), v.cpu(), torch.arange(k.shape[0]), 128)
+  want = held(x, fmt)
+  assert torch.equal(got[1].reshape(-1, 128)[:T].double().nan_to_num(-1.0), want.nan_to_num(-1.0))
+  fine = torch.isfinite(x.float()).all(-1) & (x.float().abs() < 1e38).all(-1)  # (an infinity times a sine of 0 is NaN in the other half)
+  assert torch.equal(got[0].reshape(-1, 128)[:T][fine].double(), want[fine])
+  kb, vb = K.kv_read_mx(k, v, torch.arange(k.shape[0], dtype=torch.int32, device=gpu)[:, None], torch.full((k.shape[0],), PAGE, dtype=torch.int32, device=gpu), 128)
+  assert torch.equal(kb.cpu().float().nan_to_num(-1.0), got[0].nan_to_num(-1.0))
+  assert torch.equal(ref.v_chunks(vb.cpu()).transpose(3, 4).flatten(2, 3).float().nan_to_num(-1.0), got[1].nan_to_num(-1.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("Dh,H,Hkv", [(128, 8, 1), (128, 32, 2), (64, 14, 2), (64, 3, 3), (128, 5, 1)])
+def test_decode_gpu(gpu, fmt, Dh, H, Hkv):
+  s = Seqs(fmt, [1, 63, 64, 65, 0, 300, 128, 700], Hkv, Dh, dev=gpu, width=12)
+  check_decode(s, H, Dh ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,Dh", [("mxfp4", 128), ("mxfp8", 128), ("mxfp4", 64), ("mxfp8", 64)])
+def test_decode_stale_bytes_gpu(gpu, fmt, Dh):
+  """Bytes past the contexts (of earlier requests, of anything) never reach a result."""
+  s = Seqs(fmt, [1, 63, 65, 7, 0, 130], 2, Dh, dev=gpu, width=4)
+  a = check_decode(s, 4, Dh ** -0.5)
+  s.spoil()
+  assert torch.equal(a, check_decode(s, 4, Dh ** -0.5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_decode_not_finite_gpu(gpu, fmt):
+  """A NaN in a group of keys makes its sequence's heads NaN; one in a group of values those 32 dims; no other sequence."""
+  s = Seqs(fmt, [100, 100, 100], 2, 128, dev=gpu)
+  slot = lambda b, t: int(s.tables[b, t // PAGE]) * PAGE + t % PAGE  # noqa: E731
+  k, v = (t.cpu() for t in (s.k, s.v))
+  x = torch.ones(1, 2, 128)
+  kb, vb = x.clone(), x.clone()
+  kb[0, 0, 5] = float("nan")
+  vb[0, 1, 40] = float("inf")
+  ref.mx_write(kb, x, torch.tensor([slot(0, 70)]), k, v)
+  ref.mx_write(x, vb, torch.tensor([slot(1, 3)]), k, v)
+  q = torch.randn(3, 8, 128, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).to(gpu)
+  out = K.attn_decode_mx(q, k.to(gpu), v.to(gpu), s.tables, s.ctx, 0.1).cpu()
+  bad = torch.zeros(3, 8, 128, dtype=torch.bool)
+  bad[0, :4] = True
+  bad[1, 4:, 32:64] = True
+  assert torch.equal(torch.isnan(out), bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,Dh,H,Hkv", [("mxfp4", 128, 8, 2), ("mxfp8", 64, 6, 3)])
+def test_decode_range_gpu(gpu, fmt, Dh, H, Hkv):
+  """Large and tiny queries: the split keeps their bits (scores of one dominant dim and of tiny ones beside it)."""
+  s = Seqs(fmt, [90, 33], Hkv, Dh, dev=gpu)
+  g = torch.Generator().manual_seed(3)
+  for mul in (2.0 ** -60, 2.0 ** 60):
+    q = torch.randn(2, H, Dh, generator=g)
+    q[:, :, ::5] *= 2.0 ** -7
+    q = (q * mul).to(torch.bfloat16)
+    scale = 1.0 / mul / 8
+    out = K.attn_decode_mx(q.to(gpu), s.k, s.v, s.tables, s.ctx, scale)
+    for b, n in enumerate(s.lens):
+      close(out[b:b + 1], *attend64(q[b:b + 1], *s.kv[b], scale, n - 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,Dh,H,Hkv", [("mxfp4", 128, 8, 2), ("mxfp8", 128, 4, 4), ("mxfp4", 64, 4, 2), ("mxfp8", 64, 8, 1)])
+def test_prompt_gpu(gpu, fmt, Dh, H, Hkv, monkeypatch):
+  ctx, new = [70, 5, 300, 128, 64, 1], [10, 5, 260, 1, 64, 1]
+  s = Seqs(fmt, ctx, Hkv, Dh, dev=gpu, width=6)
+  s.spoil()
+  whole, end = check_prompt(s, new, H, Dh ** -0.5)
+  assert (whole[end:] == 7).all()
+  for limit in (1, 2 * 6 * Hkv * PAGE * Dh * 4):  # a sequence, two sequences at a time
+    monkeypatch.setattr(K, "MX_READ_BYTES", limit)
+    assert torch.equal(check_prompt(s, new, H, Dh ** -0.5)[0], whole)
+
+
+@pytest.mark.gpu
+def test_refusals_gpu(gpu):
+  s = Seqs("mxfp4", [70, 5], 2, 128, dev=gpu)
+  q = torch.zeros(2, 4, 128, dtype=torch.bfloat16, device=gpu)
+  bad = [
+    lambda: K.attn_decode_mx(q.float(), s.k, s.v, s.tables, s.ctx, 1.0),
+    lambda: K.attn_decode_mx(q, s.k.to(torch.int8), s.v, s.tables, s.ctx, 1.0),
+    lambda: K.attn_decode_mx(q, s.k, s.v[..., :-64].contiguous(), s.tables, s.ctx, 1.0),
+    lambda: K.attn_decode_mx(q[..., :64].contiguous(), s.k, s.v, s.tables, s.ctx, 1.0),
+    lambda: K.attn_decode_mx(q, s.k, s.v, s.tables.long(), s.ctx, 1.0),
+    lambda: K.attn_decode_mx(q, s.k, s.v, s.tables[:1], s.ctx, 1.0),
+    lambda: K.attn_decode_mx(q, s.k, s.v, s.tables, s.ctx[:1], 1.0),
+    lambda: K.attn_decode_mx(q, s.k.cpu(), s.v, s.tables, s.ctx, 1.0),
+    lambda: K.attn_decode_mx(q[:, :3].contiguous(), s.k, s.v, s.tables, s.ctx, 1.0),
+    lambda: K.attn_decode_mx(torch.zeros(2, 34, 128, dtype=torch.bfloat16, device=gpu), s.k, s.v, s.tables, s.ctx, 1.0),
+    lambda: K.kv_read_mx(s.k, s.v, s.tables, s.ctx[:1], 128),
+    lambda: K.kv_read_mx(s.k, s.v, s.tables, s.ctx, 64),
+    lambda: K.kv_read_mx(s.k, s.v, s.tables, s.ctx, 128, k_out=torch.zeros(1, 2, 64, 128, dtype=torch.bfloat16, device=gpu)),
+    lambda: K.rope_kv_write_mx(torch.zeros(3, 6 * 128, dtype=torch.bfloat16, device=gpu), torch.zeros(2, dtype=torch.int32, device=gpu),
+                               torch.zeros(9, 128, device=gpu), torch.zeros(3, dtype=torch.int64, device=gpu), s.k, s.v, 2, 2),
+    lambda: K.rope_kv_write_mx(torch.zeros(3, 6 * 128, dtype=torch.bfloat16, device=gpu), torch.zeros(3, dtype=torch.int32, device=gpu),
+                               torch.zeros(9, 128, device=gpu), torch.zeros(3, dtype=torch.int64, device=gpu), s.k, s.v, 4, 1),
+    lambda: K.rope_kv_write_mx(torch.zeros(3, 6 * 128, dtype=torch.bfloat16, device=gpu), torch.zeros(3, dtype=torch.int32, device=gpu),
+                               torch.zeros(9, 64, device=gpu), torch.zeros(3, dtype=torch.int64, device=gpu), s.k, s.v, 2, 2),
+  ]
+  for i, call in enumerate(bad):
+    with pytest.raises((RuntimeError, ValueError)):
+      call()
+      print("not refused:", i)

@@ -19,6 +19,7 @@
 // the causal mask come from context_lens on device: no mask tensor is ever built or shipped
 // (the reference materialises and JSON-ships a [1,T,T] mask per hop, llm_utils.py:473-511).
 #include "common.h"
+#include "handover.h"
 #include "kernels.h"
 #include <cstdlib>
 
@@ -237,23 +238,6 @@ struct DecodeUnit {
   int prow, pstride;        // row of the partial results of the group's first head, rows from head to head
 };
 
-// pairs of floats that workgroups of one launch hand over: relaxed 64-bit accesses at agent scope, past the L2 of an XCD
-__device__ __forceinline__ void agent_store2(float* p, float a, float b) {
-  const uint64_t v = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
-  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void agent_store4(float* p, const f32x4& v) {
-  agent_store2(p, v[0], v[1]);
-  agent_store2(p + 2, v[2], v[3]);
-}
-__device__ __forceinline__ f32x2_t agent_load2(const float* p) {
-  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return {__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
-}
-__device__ __forceinline__ f32x4 agent_load4(const float* p) {
-  const f32x2_t a = agent_load2(p), b = agent_load2(p + 2);
-  return {a[0], a[1], b[0], b[1]};
-}
 // four results o / l in bf16 (a row without keys: zeros)
 __device__ __forceinline__ void st_bf16x4(uint16_t* p, const f32x4& o, float l) {
   s16x4 y;

@@ -1,0 +1,639 @@
+// A paged KV cache in 8 or 4 bits: written as keys are rotated, read back, and read by the attention of single tokens.
+//
+// Format.  A head's row of DH dims in groups of 32.  Each group has one power of two as its scale (a byte: exponent + 127; 255: the
+// group held a NaN or an infinity and reads back as NaN) and elements of e2m1 (0 .5 1 1.5 2 3 4 6) or e4m3.  The exponent is the
+// smallest with absmax <= 7 (464) 2^e, halfway between the largest element and where the next would be, so the largest value of a
+// group is off by half a step of its binade like all others (a scale by the binade alone clips values of 6 to 8 to 6).  Its range, -100
+// to 125 (119), keeps every element a normal bf16 number: what is read back is exact in bf16.  4.25 and 8.25 bits a value.
+//
+// Layout.  A page of one KV head is one run of bytes, 64 keys of elements, then their scales; each wide load of the attention is
+// one operand of a matrix instruction as it stands:
+//   keys     rows of DH elements (4 bits: even dim low): the A operand of v_mfma_scale_f32_16x16x128, which takes these formats and
+//            their scales as they are.  Scales by group, the four score tiles of a page side by side (mx_key_scale)
+//   values   units of 16 bytes with a lane's share of some keys: dims 2r and 2r + 1 of every group (mx_value_off); scales
+//            [64 keys][groups].  A token's write fills whole bytes: no two tokens share one
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+#include "handover.h"
+
+namespace xot {
+namespace {
+
+constexpr int PAGE = 64;
+constexpr float NEG_BIG = -1e30f;
+constexpr float LOG2E = 1.4426950408889634f;
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+template <int DH, bool FP8>
+struct Mx {
+  static constexpr int J = DH / 32;                   // groups of a row
+  static constexpr int ROW = FP8 ? DH : DH / 2;       // bytes of a key's elements
+  static constexpr int ELEMS = PAGE * ROW;            // elements of a page: its scales start here
+  static constexpr int BYTES = ELEMS + PAGE * J;      // a page of one head
+  static constexpr int NB = FP8 ? 2 * J : J;          // bytes of a key in a value unit
+  static constexpr int KC = 16 / NB;                  // keys of a value unit
+  static constexpr int EMAX = FP8 ? 8 : 2;            // exponent of the largest element
+  static constexpr uint32_t TOP = FP8 ? 0x680000u : 0x600000u;  // mantissa of 464 / 256 and of 7 / 4
+  static constexpr int HIGH = FP8 ? 119 : 125;
+};
+constexpr int LOW = -100;
+
+// byte of key i's scale among a group's 64: score tile t, row c of the attention (below) is key 32 (t >> 1) + 4 (t & 1) + 8 (c >> 2) + (c & 3)
+__device__ __forceinline__ int mx_key_scale(int i) { return 4 * (4 * ((i >> 3) & 3) + (i & 3)) + 2 * (i >> 5) + ((i >> 2) & 1); }
+template <int DH, bool FP8>
+__device__ __forceinline__ int mx_value_off(int key, int r) {
+  using M = Mx<DH, FP8>;
+  return ((key / M::KC) * 16 + r) * 16 + (key % M::KC) * M::NB;
+}
+
+// absmax bits of a group -> exponent of its scale
+template <int DH, bool FP8>
+__device__ __forceinline__ int mx_exponent(uint32_t a) {
+  using M = Mx<DH, FP8>;
+  const int e = (int)(a >> 23) - 127 - M::EMAX + ((a & 0x7fffffu) > M::TOP ? 1 : 0);
+  return min(max(e, LOW), M::HIGH);
+}
+__device__ __forceinline__ bool mx_bad(uint32_t a) { return a >= 0x7f800000u; }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// two values -> a byte of e2m1 (a low); the instruction divides by the scale, rounds to the nearest, ties to even, and saturates
+__device__ __forceinline__ uint32_t to_fp4(float a, float b, float scale) {
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a, b, scale, 0) & 0xffu;
+}
+// two values (already divided) -> two bytes of e4m3; past 464 the instruction gives NaN, hence the clamp
+__device__ __forceinline__ uint32_t to_fp8(float a, float b) {
+  a = fminf(fmaxf(a, -448.f), 448.f);
+  b = fminf(fmaxf(b, -448.f), 448.f);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
+}
+// byte b of x, two e2m1 -> two bf16, times the power of two in the scale's exponent field (its other bits do not count; a field of 255
+// gives NaN).  Exact.
+__device__ __forceinline__ uint32_t from_fp4(uint32_t x, float scale, int b) {
+  switch (b) {
+    case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, scale, 0));
+    case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, scale, 1));
+    case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, scale, 2));
+    default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, scale, 3));
+  }
+}
+// half h of x, two e4m3 -> two bf16
+__device__ __forceinline__ uint32_t from_fp8(uint32_t x, float scale, int h) {
+  return h ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, true))
+           : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, false));
+}
+// byte j of x in a float's exponent field (the other bits are whatever stands beside it: from_fp4 and from_fp8 do not look)
+__device__ __forceinline__ float scale_of(uint32_t x, int j) { return __uint_as_float(j == 3 ? x >> 1 : x << (23 - 8 * j)); }
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// largest value of N (8 or 16) neighbouring lanes, in all of them
+template <int N>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  if (N == 16) v = max(v, row_turn<8>(v));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false));  // the eight lanes mirrored
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, false));   // lane ^ 2
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, false));  // lane ^ 1
+}
+
+// ============================================================================ write
+// Sixteen lanes a row of one head (q, k or v) of a token.  k is quantised from its rotation in fp32, v from its bf16; a group's largest
+// value is found among the lanes that hold it (on the bits: a NaN counts as larger than everything).  The rotation's products and sums are
+// rounded one by one, so that a value on the border between two elements falls the same way wherever it is computed.
+// Bound by its launch at a few tokens, by memory at many.
+template <int DH, bool FP8>
+__global__ __launch_bounds__(256) void rope_kv_write_mx_kernel(const uint16_t* __restrict__ qkv, const int32_t* __restrict__ pos,
+                                                               const float* __restrict__ cos_sin, const int64_t* __restrict__ slots,
+                                                               uint16_t* __restrict__ q_out, uint8_t* __restrict__ kc,
+                                                               uint8_t* __restrict__ vc, long rows, int H, int Hkv, int max_pos, long nslots) {
+#pragma clang fp contract(off)
+  using M = Mx<DH, FP8>;
+  constexpr int E = DH / 32, HALF = DH / 2;
+  const long row = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (row >= rows) return;  // (sixteen lanes together)
+  const int r = threadIdx.x & 15, N = H + 2 * Hkv;
+  const long t = row / N;
+  const int h = (int)(row - t * N);
+  const uint16_t* src = qkv + row * DH;
+  long slot = -1;
+  if (h >= H) {
+    slot = slots[t];
+    if (slot < 0 || slot >= nslots) return;
+  }
+  const int off = (int)(slot & (PAGE - 1));
+  if (h < H + Hkv) {
+    int p = pos[t];
+    p = p < 0 ? 0 : (p >= max_pos ? max_pos - 1 : p);
+    const float* cs = cos_sin + (size_t)p * DH;
+    float lo[E], hi[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float a = bf2f(src[E * r + i]), b = bf2f(src[HALF + E * r + i]), c = cs[E * r + i], s = cs[HALF + E * r + i];
+      lo[i] = a * c - b * s;
+      hi[i] = b * c + a * s;
+    }
+    if (h < H) {
+      uint16_t* dst = q_out + ((size_t)t * H + h) * DH + E * r;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        dst[i] = f2bf(lo[i]);
+        dst[HALF + i] = f2bf(hi[i]);
+      }
+      return;
+    }
+    uint8_t* page = kc + ((size_t)(slot / PAGE) * Hkv + (h - H)) * M::BYTES;
+    uint32_t a = 0, b = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      a = max(a, __float_as_uint(lo[i]) & 0x7fffffffu);
+      b = max(b, __float_as_uint(hi[i]) & 0x7fffffffu);
+    }
+    a = lanes_max<32 / E>(a);
+    b = lanes_max<32 / E>(b);
+    const int ea = mx_exponent<DH, FP8>(a), eb = mx_exponent<DH, FP8>(b);
+    const bool na = mx_bad(a), nb = mx_bad(b);
+    uint8_t* dst = page + off * M::ROW;
+    if constexpr (FP8) {
+#pragma unroll
+      for (int i = 0; i < E; i += 2) {
+        const float sa = pow2(-ea), sb = pow2(-eb);
+        const uint32_t x = na ? 0 : to_fp8(lo[i] * sa, lo[i + 1] * sa), y = nb ? 0 : to_fp8(hi[i] * sb, hi[i + 1] * sb);
+        *reinterpret_cast<uint16_t*>(dst + E * r + i) = (uint16_t)x;
+        *reinterpret_cast<uint16_t*>(dst + HALF + E * r + i) = (uint16_t)y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; i += 2) {
+        dst[(E * r + i) / 2] = (uint8_t)(na ? 0 : to_fp4(lo[i], lo[i + 1], pow2(ea)));
+        dst[(HALF + E * r + i) / 2] = (uint8_t)(nb ? 0 : to_fp4(hi[i], hi[i + 1], pow2(eb)));
+      }
+    }
+    if (r % (32 / E) == 0) {
+      const int j = E * r / 32;
+      uint8_t* sc = page + M::ELEMS + mx_key_scale(off);
+      sc[64 * j] = (uint8_t)(na ? 255 : ea + 127);
+      sc[64 * (j + M::J / 2)] = (uint8_t)(nb ? 255 : eb + 127);
+    }
+    return;
+  }
+  uint8_t* page = vc + ((size_t)(slot / PAGE) * Hkv + (h - H - Hkv)) * M::BYTES;
+  uint8_t* dst = page + mx_value_off<DH, FP8>(off, r);
+#pragma unroll
+  for (int j = 0; j < M::J; ++j) {
+    const float x = bf2f(src[32 * j + 2 * r]), y = bf2f(src[32 * j + 2 * r + 1]);
+    const uint32_t a = lanes_max<16>(max(__float_as_uint(x) & 0x7fffffffu, __float_as_uint(y) & 0x7fffffffu));
+    const int e = mx_exponent<DH, FP8>(a);
+    const bool bad = mx_bad(a);
+    if constexpr (FP8) {
+      const float s = pow2(-e);
+      *reinterpret_cast<uint16_t*>(dst + 2 * j) = (uint16_t)(bad ? 0 : to_fp8(x * s, y * s));
+    } else {
+      dst[j] = (uint8_t)(bad ? 0 : to_fp4(x, y, pow2(e)));
+    }
+    if (r == 0) page[M::ELEMS + off * M::J + j] = (uint8_t)(bad ? 255 : e + 127);
+  }
+}
+
+// ============================================================================ read
+// One workgroup a page of one head: bf16 keys [64][DH] and values chunk-major (v_page_off), what the prompt attention reads.  Keys past
+// the context are zeros, in pages that hold some and (skip unset) in those that lie wholly past it.
+template <int DH, bool FP8>
+__global__ __launch_bounds__(256) void kv_read_mx_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+                                                         const int32_t* __restrict__ tables, int width, const int32_t* __restrict__ ctx_lens,
+                                                         uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out, int Hkv,
+                                                         int num_pages, bool skip) {
+  using M = Mx<DH, FP8>;
+  const long unit = blockIdx.x;
+  const int kvh = (int)(unit % Hkv);
+  const long entry = unit / Hkv;
+  const int b = (int)(entry / width), w = (int)(entry % width);
+  const int live = min(max(ctx_lens[b] - w * PAGE, 0), PAGE);
+  if (live == 0 && skip) return;
+  const long page = min(max(tables[entry], 0), num_pages - 1);
+  const uint8_t* kp = kc + ((size_t)page * Hkv + kvh) * M::BYTES;
+  const uint8_t* vp = vc + ((size_t)page * Hkv + kvh) * M::BYTES;
+  uint16_t* ko = k_out + ((size_t)entry * Hkv + kvh) * PAGE * DH;
+  uint16_t* vo = v_out + ((size_t)entry * Hkv + kvh) * PAGE * DH;
+  constexpr int CPR = DH / 8;
+  for (int i = threadIdx.x; i < PAGE * CPR; i += 256) {  // eight dims of a key
+    const int key = i / CPR, d = (i % CPR) * 8;
+    u32x4 y = {0, 0, 0, 0};
+    if (key < live) {
+      const float s = scale_of(kp[M::ELEMS + 64 * (d >> 5) + mx_key_scale(key)], 0);
+      const uint32_t* x = reinterpret_cast<const uint32_t*>(kp + key * M::ROW + (FP8 ? d : d / 2));
+#pragma unroll
+      for (int n = 0; n < 4; ++n) y[n] = FP8 ? from_fp8(x[n >> 1], s, n & 1) : from_fp4(x[0], s, n);
+    }
+    *reinterpret_cast<u32x4*>(ko + key * DH + d) = y;
+  }
+  for (int i = threadIdx.x; i < 128 * M::J; i += 256) {  // eight keys of two dims
+    const int r = i & 15, j = (i >> 4) % M::J, k0 = 8 * (i / (16 * M::J));
+    u32x4 lo, hi;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      uint32_t y[2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const int key = k0 + 2 * n + m;
+        y[m] = 0;
+        if (key < live) {
+          const uint8_t* x = vp + mx_value_off<DH, FP8>(key, r);
+          const float s = scale_of(vp[M::ELEMS + key * M::J + j], 0);
+          y[m] = FP8 ? from_fp8(reinterpret_cast<const uint16_t*>(x)[j], s, 0) : from_fp4(x[j], s, 0);
+        }
+      }
+      lo[n] = low_halves(y[0], y[1]);
+      hi[n] = high_halves(y[0], y[1]);
+    }
+    uint16_t* o = vo + v_page_off(k0, 32 * j + 2 * r, DH);
+    *reinterpret_cast<u32x4*>(o) = lo;
+    *reinterpret_cast<u32x4*>(o + 8) = hi;
+  }
+}
+
+// ============================================================================ attention of single tokens
+// Scores S^T = K . Q^T: sixteen keys (A) by the query heads of a KV head (B columns) on v_mfma_scale_f32_16x16x128_f8f6f4, which reads the
+// cache's elements and scales as they stand.  A query is the sum of two e4m3 numbers, one 1/16 of the other's scale: bf16 has 8
+// significant bits, each of the two takes 4, so the split is exact down to 2^-21 of the query's largest value (below e4m3's normal
+// range).  Heads of 128 take one instruction for each, heads of 64 both in the two halves of one.
+// Operand maps (lane (g, c) = (l >> 4, l & 15)): e2m1 A: dims 32 g .. of row c, 16 bytes; e4m3: 16 g .. in the first 16 bytes, 64 + 16 g
+// .. in the second; a scale byte counts for dims 32 g .. of its lane's row.  Score tile t's row c = 4 q + r is key 32 (t >> 1) + 8 q + 4 (t
+// & 1) + r, so that a lane's scores of tiles 2 kk and 2 kk + 1 are the eight keys 32 kk + 8 g .. that it holds in the B operand of
+// O^T = V^T . P^T: probabilities stay in their registers.
+// Values: two e2m1 / e4m3 of a key become two bf16 (exact, scaled on the way), and two keys' pairs change halves: tile (j, e) of O^T
+// has dims 32 j + 2 row + e.  P is rounded to bf16, the values' own type; sums, maxima and the output are fp32.
+template <int DH, bool FP8>
+struct PageRegs {
+  using M = Mx<DH, FP8>;
+  static constexpr int KV = FP8 && DH == 128 ? 2 : 1;  // 16-byte loads of a key row's share
+  static constexpr int VU = 8 / M::KC;                 // value units of eight keys
+  static constexpr int VS = M::J / 2;                  // 16-byte loads of eight keys' scales
+  u32x4 k[4][KV], v[2][VU], vs[2][VS];
+  uint32_t ks;
+};
+
+template <int DH, bool FP8>
+__device__ __forceinline__ f32x4 score_mfma(const u32x4 (&k)[PageRegs<DH, FP8>::KV], const i32x8& q, f32x4 acc, uint32_t ks, int qs, int t) {
+  constexpr int F = FP8 ? 0 : 4;
+  i32x8 a;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    a[i] = (int)k[0][i];
+    a[4 + i] = !FP8 ? 0 : (int)k[PageRegs<DH, FP8>::KV - 1][i];
+  }
+  switch (t) {
+    case 0: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, acc, F, 0, 0, (int)ks, 0, qs);
+    case 1: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, acc, F, 0, 1, (int)ks, 0, qs);
+    case 2: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, acc, F, 0, 2, (int)ks, 0, qs);
+    default: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, acc, F, 0, 3, (int)ks, 0, qs);
+  }
+}
+
+struct DecodeArgs {
+  const uint16_t* q;
+  const uint8_t *kc, *vc;
+  const int32_t *tables, *ctx_lens;
+  uint16_t* out;
+  float *ws_o, *ws_ml;
+  int* tickets;
+  int width, H, Hkv, ppp, nparts, num_pages;
+  float scale_log2;
+};
+
+template <int DH, bool FP8, int NW>
+__global__ __launch_bounds__(64 * NW) void attn_decode_mx_kernel(const DecodeArgs A) {
+  using M = Mx<DH, FP8>;
+  using R = PageRegs<DH, FP8>;
+  constexpr int J = M::J, LD = DH + 4;
+  extern __shared__ __attribute__((aligned(16))) float sm[];
+  const int kvh = blockIdx.x % A.Hkv, b = blockIdx.x / A.Hkv;
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, G = A.H / A.Hkv;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ctx = min(max(A.ctx_lens[b], 0), A.width * PAGE);
+  const int first = 0, last = (ctx + PAGE - 1) / PAGE;
+
+  // the query in two parts
+  i32x8 qhi = {0, 0, 0, 0, 0, 0, 0, 0}, qlo = qhi;
+  int shi, slo;
+  {
+    const uint16_t* qp = A.q + ((size_t)b * A.H + kvh * G + min(c, G - 1)) * DH + 16 * g;
+    s16x8 x[DH / 32];
+    uint32_t a = 0;
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i) {
+      x[i] = ld16(qp + (i >> 1) * 64 + (i & 1) * 8);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) a = max(a, ((uint32_t)(uint16_t)x[i][n] << 16) & 0x7fffffffu);
+    }
+    auto most = [](uint32_t u, uint32_t v) { return max(u, v); };
+    a = lane_xor<16>(lane_xor<32>(a, most), most);
+    const int e = min(max((int)(a >> 23) - 127 - 7, -120), 120);
+    const float inv = pow2(-e);
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i)
+#pragma unroll
+      for (int n = 0; n < 8; n += 4) {
+        int hi = 0, lo = 0;
+        const float f0 = bf2f(x[i][n]) * inv, f1 = bf2f(x[i][n + 1]) * inv, f2 = bf2f(x[i][n + 2]) * inv, f3 = bf2f(x[i][n + 3]) * inv;
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(f0, f1, hi, false);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(f2, f3, hi, true);
+        const f32x2_t h0 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), h1 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32((f0 - h0[0]) * 16.f, (f1 - h0[1]) * 16.f, lo, false);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32((f2 - h1[0]) * 16.f, (f3 - h1[1]) * 16.f, lo, true);
+        const int at = 2 * i + n / 4;  // dword of the operand
+        if (c >= G) hi = lo = 0;
+        qhi[at] = hi;
+        if (DH == 128) qlo[at] = lo;
+        else qhi[4 + at] = lo;
+      }
+    const bool bad = mx_bad(a) && c < G;
+    shi = bad ? 255 : e + 127;
+    slo = bad ? 255 : e + 127 - 4;
+    if (DH == 64 && g >= 2) shi = slo;
+  }
+
+  float m = NEG_BIG, l = 0.f;
+  f32x4 o[J][2];
+#pragma unroll
+  for (int j = 0; j < J; ++j) o[j][0] = o[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int32_t* bt = A.tables + (size_t)b * A.width;
+  const int krow = 8 * (c >> 2) + (c & 3);
+
+  auto load = [&](int p, R& x) {
+    const long page = min(max(bt[p], 0), A.num_pages - 1);
+    const uint8_t* kp = A.kc + ((size_t)page * A.Hkv + kvh) * M::BYTES;
+    const uint8_t* vp = A.vc + ((size_t)page * A.Hkv + kvh) * M::BYTES;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < R::KV; ++i)
+        x.k[t][i] = *reinterpret_cast<const u32x4*>(kp + (32 * (t >> 1) + 4 * (t & 1) + krow) * M::ROW + 64 * i +
+                                                    16 * (DH == 64 && !FP8 ? g & 1 : g));
+    x.ks = *reinterpret_cast<const uint32_t*>(kp + M::ELEMS + 64 * (g & (J - 1)) + 4 * c);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+#pragma unroll
+      for (int u = 0; u < R::VU; ++u)
+        x.v[kk][u] = *reinterpret_cast<const u32x4*>(vp + (((32 * kk + 8 * g) / M::KC + u) * 16 + c) * 16);
+#pragma unroll
+      for (int u = 0; u < R::VS; ++u) x.vs[kk][u] = *reinterpret_cast<const u32x4*>(vp + M::ELEMS + (32 * kk + 8 * g) * J + 16 * u);
+    }
+  };
+
+  for (int p = first + wave; p < last; p += NW) {
+    R x;
+    load(p, x);
+    f32x4 st[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      st[t] = score_mfma<DH, FP8>(x.k[t], qhi, f32x4{0.f, 0.f, 0.f, 0.f}, x.ks, shi, t);
+      if (DH == 128) st[t] = score_mfma<DH, FP8>(x.k[t], qlo, st[t], x.ks, slo, t);
+    }
+    const int left = ctx - p * PAGE - 8 * g;  // keys of this lane group inside the context
+    float mx = NEG_BIG;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v = 32 * (t >> 1) + 4 * (t & 1) + r < left ? st[t][r] * A.scale_log2 : -INFINITY;
+        st[t][r] = v;
+        mx = fmaxf(mx, v);
+      }
+    mx = xor_max<16>(mx);
+    mx = xor_max<32>(mx);
+    const float mn = fmaxf(m, mx), alpha = exp2f(m - mn);
+    m = mn;
+    l *= alpha;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      o[j][0] *= alpha;
+      o[j][1] *= alpha;
+    }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      s16x8 pf;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float pv = exp2f(st[2 * kk + h][r] - mn);
+          l += pv;
+          pf[4 * h + r] = (short)f2bf(pv);
+        }
+      // what lies past the context may be anything, NaN too: it becomes zeros (their probabilities are 0, but 0 NaN is NaN)
+      constexpr int ND = 2 * M::NB;  // dwords of eight keys' elements
+      uint32_t vd[ND], sd[2 * J];
+#pragma unroll
+      for (int i = 0; i < ND; ++i) vd[i] = x.v[kk][i >> 2][i & 3];
+#pragma unroll
+      for (int i = 0; i < 2 * J; ++i) sd[i] = x.vs[kk][i >> 2][i & 3];
+      if (ctx - p * PAGE < PAGE) {
+#pragma unroll
+        for (int key = 0; key < 8; ++key) {
+          const bool dead = 32 * kk + key >= left;
+          if constexpr (M::NB >= 4) {
+#pragma unroll
+            for (int i = 0; i < M::NB / 4; ++i) vd[key * (M::NB / 4) + i] = dead ? 0 : vd[key * (M::NB / 4) + i];
+          } else {
+            vd[key >> 1] = dead ? vd[key >> 1] & (key & 1 ? 0xffffu : 0xffff0000u) : vd[key >> 1];
+          }
+          if constexpr (J == 4) sd[key] = dead ? 0x7f7f7f7fu : sd[key];
+          else sd[key >> 1] = dead ? (key & 1 ? (sd[key >> 1] & 0xffffu) | 0x7f7f0000u : (sd[key >> 1] & 0xffff0000u) | 0x7f7fu) : sd[key >> 1];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        u32x4 ae, ao;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          uint32_t y[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int key = 2 * n + i, at = key * M::NB + (FP8 ? 2 * j : j);  // byte among the eight keys'
+            const float s = scale_of(sd[key * J / 4], (key * J + j) & 3);
+            y[i] = FP8 ? from_fp8(vd[at >> 2], s, (at >> 1) & 1) : from_fp4(vd[at >> 2], s, at & 3);
+          }
+          ae[n] = low_halves(y[0], y[1]);
+          ao[n] = high_halves(y[0], y[1]);
+        }
+        o[j][0] = mfma16(__builtin_bit_cast(s16x8, ae), pf, o[j][0]);
+        o[j][1] = mfma16(__builtin_bit_cast(s16x8, ao), pf, o[j][1]);
+      }
+    }
+  }
+
+  // the waves meet in LDS: [NW][G][LD] sums, [NW][G][2] maxima and sums of weights
+  l = xor_sum<16>(l);
+  l = xor_sum<32>(l);
+  float* ml = sm + NW * G * LD;
+  if (c < G) {
+    float* so = sm + (wave * G + c) * LD + 8 * g;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      *reinterpret_cast<f32x4*>(so + 32 * j) = f32x4{o[j][0][0], o[j][1][0], o[j][0][1], o[j][1][1]};
+      *reinterpret_cast<f32x4*>(so + 32 * j + 4) = f32x4{o[j][0][2], o[j][1][2], o[j][0][3], o[j][1][3]};
+    }
+    if (g == 0) {
+      ml[(wave * G + c) * 2] = m;
+      ml[(wave * G + c) * 2 + 1] = l;
+    }
+  }
+  __syncthreads();
+  for (int e = 4 * threadIdx.x; e < G * DH; e += 4 * NW * 64) {
+    const int hq = e / DH, d = e - hq * DH;
+    float mm = NEG_BIG;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) mm = fmaxf(mm, ml[(w * G + hq) * 2]);
+    float L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = exp2f(ml[(w * G + hq) * 2] - mm);
+      L += ml[(w * G + hq) * 2 + 1] * f;
+      O += *reinterpret_cast<const f32x4*>(sm + (w * G + hq) * LD + d) * f;
+    }
+    s16x4 y;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = (short)f2bf(ctx > 0 ? O[r] / L : 0.f);
+    *reinterpret_cast<s16x4*>(A.out + ((size_t)b * A.H + kvh * G + hq) * DH + d) = y;
+  }
+}
+
+// ============================================================================ bindings
+#define XCHECK(cond, ...) TORCH_CHECK(cond, "xot kernel: ", __VA_ARGS__)
+inline hipStream_t stream() { return at::hip::getCurrentHIPStream().stream(); }
+inline uint16_t* bf(const at::Tensor& t) { return reinterpret_cast<uint16_t*>(t.data_ptr()); }
+
+void on_gpu(const char* op, const at::Tensor& t, at::ScalarType dt, const char* name, const at::Device& dev) {
+  XCHECK(t.is_cuda() && t.device() == dev, op, ": ", name, " must be on the queries' GPU");
+  XCHECK(t.scalar_type() == dt, op, ": ", name, " must be ", dt);
+  XCHECK(t.is_contiguous(), op, ": ", name, " must be contiguous");
+}
+
+int64_t page_bytes(int64_t Dh, bool fp8) { return PAGE * (fp8 ? Dh : Dh / 2) + PAGE * (Dh / 32); }
+
+// both pools [pages, Hkv, bytes] of one format; true: e4m3
+bool caches_ok(const char* op, const at::Tensor& k, const at::Tensor& v, int64_t Dh, const at::Device& dev) {
+  XCHECK(Dh == 64 || Dh == 128, op, ": heads of 64 or 128 dims");
+  on_gpu(op, k, at::kByte, "k_cache", dev);
+  on_gpu(op, v, at::kByte, "v_cache", dev);
+  XCHECK(k.dim() == 3 && v.sizes() == k.sizes(), op, ": caches must be two [pages, Hkv, page bytes] of the same size");
+  XCHECK(k.size(0) >= 1 && k.size(0) < (int64_t(1) << 31) && k.size(1) >= 1, op, ": caches without pages or heads");
+  const bool fp8 = k.size(2) == page_bytes(Dh, true);
+  XCHECK(fp8 || k.size(2) == page_bytes(Dh, false), op, ": a page of ", k.size(2), " bytes is neither mxfp4 nor mxfp8 of heads of ", Dh);
+  XCHECK((reinterpret_cast<uintptr_t>(k.data_ptr()) | reinterpret_cast<uintptr_t>(v.data_ptr())) % 16 == 0, op, ": caches must be aligned to 16 bytes");
+  return fp8;
+}
+
+#define MX_GO(fp8, Dh, GO)                  \
+  do {                                      \
+    if ((Dh) == 128) {                      \
+      if (fp8) GO(128, true);               \
+      else GO(128, false);                  \
+    } else {                                \
+      if (fp8) GO(64, true);                \
+      else GO(64, false);                   \
+    }                                       \
+  } while (0)
+
+void rope_kv_write_mx(const at::Tensor& qkv, const at::Tensor& pos, const at::Tensor& cos_sin, const at::Tensor& slots, at::Tensor& q_out,
+                      at::Tensor& k_cache, at::Tensor& v_cache, int64_t H, int64_t Hkv) {
+  const char* op = "rope_kv_write_mx";
+  XCHECK(qkv.is_cuda() && qkv.dim() == 2, op, ": qkv must be [T, (H + 2 Hkv) Dh] on a GPU");
+  const at::Device dev = qkv.device();
+  const c10::DeviceGuard guard(dev);
+  const int64_t T = qkv.size(0);
+  XCHECK(H >= 1 && Hkv >= 1 && qkv.size(1) % (H + 2 * Hkv) == 0, op, ": qkv columns are not H + 2 Hkv heads");
+  const int64_t Dh = qkv.size(1) / (H + 2 * Hkv);
+  on_gpu(op, qkv, at::kBFloat16, "qkv", dev);
+  on_gpu(op, pos, at::kInt, "pos", dev);
+  on_gpu(op, cos_sin, at::kFloat, "cos_sin", dev);
+  on_gpu(op, slots, at::kLong, "slots", dev);
+  on_gpu(op, q_out, at::kBFloat16, "q_out", dev);
+  const bool fp8 = caches_ok(op, k_cache, v_cache, Dh, dev);
+  XCHECK(k_cache.size(1) == Hkv, op, ": the caches have ", k_cache.size(1), " heads");
+  XCHECK(pos.numel() == T && slots.numel() == T && q_out.numel() == T * H * Dh, op, ": pos, slots or q_out of another length");
+  XCHECK(cos_sin.dim() == 2 && cos_sin.size(1) == Dh && cos_sin.size(0) >= 1, op, ": cos_sin must be [positions, Dh]");
+  if (T == 0) return;
+  const int64_t rows = T * (H + 2 * Hkv), blocks = (rows + 15) / 16;
+  XCHECK(blocks < (int64_t(1) << 24), op, ": too many tokens for one launch");
+#define GO(DHV, F)                                                                                                                      \
+  rope_kv_write_mx_kernel<DHV, F><<<(unsigned)blocks, 256, 0, stream()>>>(                                                              \
+      bf(qkv), pos.data_ptr<int32_t>(), cos_sin.data_ptr<float>(), slots.data_ptr<int64_t>(), bf(q_out), k_cache.data_ptr<uint8_t>(),   \
+      v_cache.data_ptr<uint8_t>(), (long)rows, (int)H, (int)Hkv, (int)cos_sin.size(0), (long)k_cache.size(0) * PAGE)
+  MX_GO(fp8, Dh, GO);
+#undef GO
+}
+
+void kv_read_mx(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables, const at::Tensor& ctx_lens, at::Tensor& k_out,
+                at::Tensor& v_out, bool skip) {
+  const char* op = "kv_read_mx";
+  XCHECK(k_cache.is_cuda(), op, ": k_cache must be on a GPU");
+  const at::Device dev = k_cache.device();
+  const c10::DeviceGuard guard(dev);
+  on_gpu(op, tables, at::kInt, "block_tables", dev);
+  on_gpu(op, ctx_lens, at::kInt, "ctx_lens", dev);
+  on_gpu(op, k_out, at::kBFloat16, "k_out", dev);
+  on_gpu(op, v_out, at::kBFloat16, "v_out", dev);
+  XCHECK(tables.dim() == 2 && ctx_lens.numel() == tables.size(0), op, ": a row of block_tables for each of ctx_lens");
+  XCHECK(k_out.dim() == 4 && v_out.dim() == 4, op, ": k_out and v_out must be 4-D");
+  const int64_t Dh = k_out.size(3), n = tables.numel(), Hkv = k_cache.dim() == 3 ? k_cache.size(1) : 0;
+  const bool fp8 = caches_ok(op, k_cache, v_cache, Dh, dev);
+  XCHECK(k_out.size(0) == n && k_out.size(1) == Hkv && k_out.size(2) == PAGE && v_out.size(0) == n && v_out.size(1) == Hkv &&
+             v_out.size(2) == Dh && v_out.size(3) == PAGE,
+         op, ": k_out must be [entries, Hkv, 64, Dh], v_out [entries, Hkv, Dh, 64]");
+  XCHECK((reinterpret_cast<uintptr_t>(k_out.data_ptr()) | reinterpret_cast<uintptr_t>(v_out.data_ptr())) % 16 == 0, op,
+         ": k_out and v_out must be aligned to 16 bytes");
+  if (n == 0) return;
+  XCHECK(n * Hkv < (int64_t(1) << 24), op, ": too many pages for one launch");
+#define GO(DHV, F)                                                                                                                         \
+  kv_read_mx_kernel<DHV, F><<<(unsigned)(n * Hkv), 256, 0, stream()>>>(                                                                    \
+      k_cache.data_ptr<uint8_t>(), v_cache.data_ptr<uint8_t>(), tables.data_ptr<int32_t>(), (int)tables.size(1), ctx_lens.data_ptr<int32_t>(), \
+      bf(k_out), bf(v_out), (int)Hkv, (int)k_cache.size(0), skip)
+  MX_GO(fp8, Dh, GO);
+#undef GO
+}
+
+void attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables,
+                    const at::Tensor& ctx_lens, at::Tensor& out, at::Tensor& ws_o, at::Tensor& ws_ml, at::Tensor& tickets,
+                    int64_t pages_per_part, int64_t nparts, double scale) {
+  const char* op = "attn_decode_mx";
+  XCHECK(q.is_cuda() && q.dim() == 3, op, ": q must be [B, H, Dh] on a GPU");
+  const at::Device dev = q.device();
+  const c10::DeviceGuard guard(dev);
+  on_gpu(op, q, at::kBFloat16, "q", dev);
+  on_gpu(op, out, at::kBFloat16, "out", dev);
+  on_gpu(op, tables, at::kInt, "block_tables", dev);
+  on_gpu(op, ctx_lens, at::kInt, "ctx_lens", dev);
+  on_gpu(op, ws_o, at::kFloat, "ws_o", dev);
+  on_gpu(op, ws_ml, at::kFloat, "ws_ml", dev);
+  on_gpu(op, tickets, at::kInt, "tickets", dev);
+  const int64_t B = q.size(0), H = q.size(1), Dh = q.size(2), Hkv = k_cache.dim() == 3 ? k_cache.size(1) : 0;
+  const bool fp8 = caches_ok(op, k_cache, v_cache, Dh, dev);
+  XCHECK(H % Hkv == 0 && H / Hkv <= 16 && H >= 1, op, ": ", H, " query heads on ", Hkv, " (at most 16 each)");
+  XCHECK(tables.dim() == 2 && tables.size(0) == B && ctx_lens.numel() == B, op, ": a row of block_tables and a length for each query");
+  XCHECK(tables.size(1) >= 1 && tables.size(1) < (1 << 24), op, ": block_tables of no or too many columns");
+  XCHECK(out.numel() == q.numel(), op, ": out must have q's shape");
+  XCHECK((reinterpret_cast<uintptr_t>(q.data_ptr()) | reinterpret_cast<uintptr_t>(out.data_ptr())) % 16 == 0, op, ": q and out must be aligned to 16 bytes");
+  XCHECK(pages_per_part >= 1 && nparts >= 1, op, ": bad partitioning");
+  if (B == 0) return;
+  XCHECK(B * Hkv * nparts < (int64_t(1) << 24), op, ": too many parts for one launch");
+  const DecodeArgs a = {bf(q), k_cache.data_ptr<uint8_t>(), v_cache.data_ptr<uint8_t>(), tables.data_ptr<int32_t>(), ctx_lens.data_ptr<int32_t>(),
+                        bf(out), ws_o.data_ptr<float>(), ws_ml.data_ptr<float>(), tickets.data_ptr<int32_t>(), (int)tables.size(1), (int)H,
+                        (int)Hkv, (int)pages_per_part, (int)nparts, (int)k_cache.size(0), (float)scale * LOG2E};
+  const size_t lds = (size_t)4 * (H / Hkv) * (Dh + 6) * sizeof(float);
+#define GO(DHV, F) attn_decode_mx_kernel<DHV, F, 4><<<(unsigned)(B * Hkv), 256, lds, stream()>>>(a)
+  MX_GO(fp8, Dh, GO);
+#undef GO
+}
+
+}  // namespace
+
+void bind_kv_mx(pybind11::module& m) {
+  m.def("rope_kv_write_mx", &rope_kv_write_mx);
+  m.def("kv_read_mx", &kv_read_mx);
+  m.def("attn_decode_mx", &attn_decode_mx);
+}
+
+}  // namespace xot

@@ -349,6 +349,101 @@ def attn_prefill(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, max_qlen: in
   return out
 
 
+# ------------------------------------------------------------------ KV cache in 8 or 4 bits
+# Pools of mxfp8 / mxfp4 pages (csrc/kv_mx.hip): uint8 [pages, Hkv, mx_page_bytes(format, Dh)] for keys and the same for values, heads of
+# 64 or 128.  The format is told from the bytes of a page.
+MX_FORMATS = ref.MX_FORMATS
+mx_page_bytes = ref.mx_page_bytes
+mx_format = ref.mx_format
+
+
+def rope_kv_write_mx(qkv: torch.Tensor, pos: torch.Tensor, cos_sin: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
+                     v_cache: torch.Tensor, H: int, Hkv: int, q_out: torch.Tensor | None = None) -> torch.Tensor:
+  """qkv [T, (H+2Hkv)*Dh] -> rotated q [T, H, Dh]; rotated k (quantised from fp32) and v into the pools at `slots` (distinct; one
+  outside the pools is not written)."""
+  T = qkv.shape[0]
+  Dh = qkv.shape[1] // (H + 2 * Hkv)
+  if not _gpu(qkv):
+    x = qkv.view(T, H + 2 * Hkv, Dh)
+    q = ref.rope(x[:, :H], pos, cos_sin)
+    ref.mx_write(ref.rope(x[:, H:H + Hkv].float(), pos, cos_sin), x[:, H + Hkv:], slots, k_cache, v_cache)
+    if q_out is not None:
+      q_out.copy_(q.view(q_out.shape))
+      return q_out
+    return q
+  q_out = torch.empty(T, H, Dh, dtype=qkv.dtype, device=qkv.device) if q_out is None else q_out
+  require().rope_kv_write_mx(qkv, pos, cos_sin, slots, q_out, k_cache, v_cache, int(H), int(Hkv))
+  return q_out
+
+
+def kv_read_mx(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor, Dh: int,
+               k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None, skip: bool = False):
+  """The pages that block_tables [B, W] names, exactly as bf16: (K [B*W, Hkv, 64, Dh], V [B*W, Hkv, Dh, 64] in the bf16 pool's layout).
+  Keys past a sequence's context are zeros; skip: pages wholly past it are left as they are."""
+  n, Hkv = block_tables.numel(), k_cache.shape[1]
+  if k_out is None:
+    k_out = torch.empty(n, Hkv, PAGE, Dh, dtype=torch.bfloat16, device=k_cache.device)
+  if v_out is None:
+    v_out = torch.empty(n, Hkv, Dh, PAGE, dtype=torch.bfloat16, device=k_cache.device)
+  if not _gpu(k_cache):
+    ref.kv_read_mx(k_cache, v_cache, block_tables, ctx_lens, k_out, v_out)
+  else:
+    require().kv_read_mx(k_cache, v_cache, block_tables, ctx_lens, k_out, v_out, bool(skip))
+  return k_out, v_out
+
+
+class MXDecodeWorkspace:
+  """Scratch of attn_decode_mx for every batch up to max_batch at this context bound."""
+
+  def __init__(self, max_batch: int, H: int, Hkv: int, Dh: int, max_ctx: int, device):
+    self.max_batch = max_batch
+    self.o = torch.empty(1, dtype=torch.float32, device=device)
+    self.ml = torch.empty(1, dtype=torch.float32, device=device)
+    self.tickets = torch.zeros(max_batch * Hkv, dtype=torch.int32, device=device)
+
+
+def attn_decode_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
+                   scale: float, ws: MXDecodeWorkspace | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+  """attn_decode over pools in 8 or 4 bits: q [B, H, Dh], one token a sequence, attends to its first ctx_lens keys; a sequence without
+  any gives zeros."""
+  if not _gpu(q):
+    y = ref.attn_decode_mx(q, k_cache, v_cache, block_tables, ctx_lens, scale)
+    if out is not None:
+      out.copy_(y.view(out.shape))
+      return out
+    return y
+  B, H, Dh = q.shape
+  if ws is None:
+    ws = MXDecodeWorkspace(B, H, k_cache.shape[1], Dh, block_tables.shape[1] * PAGE, q.device)
+  out = torch.empty_like(q) if out is None else out
+  require().attn_decode_mx(q, k_cache, v_cache, block_tables, ctx_lens, out, ws.o, ws.ml, ws.tickets, block_tables.shape[1], 1, float(scale))
+  return out
+
+
+# scratch of attn_prefill_mx's bf16 pages: at most this much, or one sequence's
+MX_READ_BYTES = 1 << 30
+
+
+def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, cu_q: torch.Tensor,
+                    ctx_lens: torch.Tensor, max_qlen: int, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
+  """attn_prefill over pools in 8 or 4 bits: the sequences' pages are read back into bf16 scratch (a group of sequences at a time), which
+  the prompt attention reads.  The products of a prompt outweigh that pass: 2 Dh bytes written a key and head against 4 Dh G flops for
+  each of its tokens."""
+  T, H, Dh = q.shape
+  B, W = block_tables.shape
+  Hkv = k_cache.shape[1]
+  out = torch.empty_like(q) if out is None else out
+  per = max(1, min(B, MX_READ_BYTES // max(1, W * Hkv * PAGE * Dh * 4))) if q.is_cuda else max(1, B)
+  k = torch.empty(per * W, Hkv, PAGE, Dh, dtype=torch.bfloat16, device=q.device)
+  v = torch.empty(per * W, Hkv, Dh, PAGE, dtype=torch.bfloat16, device=q.device)
+  own = torch.arange(per * W, dtype=torch.int32, device=q.device).view(per, W)
+  for b in range(0, B, per):
+    n = min(per, B - b)
+    kv_read_mx(k_cache, v_cache, block_tables[b:b + n], ctx_lens[b:b + n], Dh, k[:n * W], v[:n * W], skip=True)
+    attn_prefill(q, k, v, own[:n], cu_q[b:b + n + 1], ctx_lens[b:b + n], max_qlen, scale, out=out)
+  return out
+
+
 # ------------------------------------------------------------------ sampling
 def attention_bidir(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, B: int, L: int, H: int, Dh: int,
                     scale: float) -> torch.Tensor:

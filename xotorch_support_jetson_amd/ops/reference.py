@@ -151,6 +151,130 @@ def attn_prefill(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, scale):
   return out
 
 
+# ------------------------------------------------------------------ KV cache in 8 or 4 bits (csrc/kv_mx.hip)
+MX_FORMATS = ("mxfp4", "mxfp8")
+_MX_TOP = {"mxfp4": (2, 7.0, 6.0, 125), "mxfp8": (8, 464.0, 448.0, 119)}  # exponent, rounding bound and value of the largest element, highest scale
+_MX_LOW = -100
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def mx_page_bytes(fmt: str, Dh: int) -> int:
+  """Bytes of a 64-key page of one KV head: the elements, then a scale byte for every 32 of them."""
+  if fmt not in MX_FORMATS:
+    raise ValueError(f"cache format {fmt!r}: one of {', '.join(MX_FORMATS)}")
+  return 64 * (Dh if fmt == "mxfp8" else Dh // 2) + 64 * (Dh // 32)
+
+
+def mx_format(cache: torch.Tensor, Dh: int) -> str:
+  """The format of a pool [pages, Hkv, page bytes] of heads of Dh."""
+  for fmt in MX_FORMATS:
+    if Dh in (64, 128) and cache.dtype == torch.uint8 and cache.dim() == 3 and cache.shape[2] == mx_page_bytes(fmt, Dh):
+      return fmt
+  raise ValueError(f"no cache of mxfp4 or mxfp8 pages of heads of {Dh} (64 or 128): {cache.dtype} {tuple(cache.shape)}")
+
+
+def mx_encode(x: torch.Tensor, fmt: str):
+  """fp32 rows [..., Dh] -> element codes [..., Dh] and scale bytes [..., Dh / 32] (csrc/kv_mx.hip says how the exponent is chosen)."""
+  emax, top, most, high = _MX_TOP[fmt]
+  x = x.float().unflatten(-1, (-1, 32))
+  a = x.abs().amax(-1, keepdim=True)
+  bad = ~torch.isfinite(a)
+  x, a = torch.where(bad, 0.0, x), torch.where(bad, 0.0, a)
+  e = torch.frexp(a)[1] - 1 - emax
+  e = torch.where(torch.ldexp(a.double(), -e) > top, e + 1, e)
+  e = torch.where(a == 0, _MX_LOW, e).clamp(_MX_LOW, high)
+  y = torch.ldexp(x.double(), -e).clamp(-most, most)
+  if fmt == "mxfp8":
+    code = y.float().to(torch.float8_e4m3fn).view(torch.uint8)
+  else:
+    ulp = torch.ldexp(torch.ones_like(y), torch.frexp(y)[1].clamp(min=1) - 2)
+    level = torch.round(y / ulp) * ulp  # (torch.round: ties to even, so to the even mantissa)
+    code = torch.bucketize(level.abs(), torch.tensor(_E2M1, dtype=y.dtype, device=y.device)).to(torch.uint8) | (level < 0).to(torch.uint8) << 3
+  return code.flatten(-2), torch.where(bad, 255, e + 127).to(torch.uint8).squeeze(-1)
+
+
+def mx_decode(code: torch.Tensor, scale: torch.Tensor, fmt: str) -> torch.Tensor:
+  """The values (fp32, exact in bf16) of element codes [..., Dh] under scale bytes [..., Dh / 32]."""
+  if fmt == "mxfp8":
+    v = code.contiguous().view(torch.float8_e4m3fn).float()
+  else:
+    v = torch.tensor(_E2M1 + tuple(-t for t in _E2M1), device=code.device)[code.long()]
+  s = torch.ldexp(torch.ones(scale.shape, device=scale.device), scale.int() - 127)
+  return (v.unflatten(-1, (-1, 32)) * torch.where(scale == 255, float("nan"), s)[..., None]).flatten(-2)
+
+
+def _mx_key_scale(key: torch.Tensor) -> torch.Tensor:
+  return 4 * (4 * (key // 8 % 4) + key % 4) + 2 * (key // 32) + key // 4 % 2
+
+
+def _mx_views(k_cache, v_cache, Dh: int):
+  """(format, key elements [pages, Hkv, 64, row], key scales [pages, Hkv, J, 64], value elements [pages, Hkv, units, 16, keys, bytes],
+  value scales [pages, Hkv, 64, J]) as views of the pools."""
+  fmt = mx_format(k_cache, Dh)
+  mx_format(v_cache, Dh)
+  n, G, J = k_cache.shape[0], k_cache.shape[1], Dh // 32
+  w = 2 if fmt == "mxfp8" else 1
+  e = 64 * Dh * w // 2
+  nb = J * w
+  return (fmt, k_cache[..., :e].view(n, G, 64, Dh * w // 2), k_cache[..., e:].view(n, G, J, 64),
+          v_cache[..., :e].view(n, G, 4 * nb, 16, 16 // nb, nb), v_cache[..., e:].view(n, G, 64, J))
+
+
+def mx_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
+  """fp32 k, v [T, Hkv, Dh] quantised into the pools at global slots (outside them: skipped)."""
+  Dh = k.shape[-1]
+  fmt, ke, ks, ve, vs = _mx_views(k_cache, v_cache, Dh)
+  ok = (slots >= 0) & (slots < k_cache.shape[0] * 64)
+  page, off = slots[ok].long() // 64, slots[ok].long() % 64
+  code, scale = mx_encode(k[ok], fmt)
+  ke[page, :, off] = code if fmt == "mxfp8" else code[..., ::2] | code[..., 1::2] << 4
+  ks[page, :, :, _mx_key_scale(off)] = scale
+  code, scale = mx_encode(v[ok], fmt)
+  code = code.unflatten(-1, (Dh // 32, 16, 2)).transpose(2, 3)  # [T, Hkv, r, group, even / odd dim]
+  code = code if fmt == "mxfp8" else code[..., :1] | code[..., 1:] << 4
+  per = ve.shape[4]
+  ve[page, :, off // per, :, off % per] = code.flatten(3)
+  vs[page, :, off] = scale
+
+
+def mx_read(k_cache: torch.Tensor, v_cache: torch.Tensor, pages: torch.Tensor, Dh: int):
+  """Pages [n] of the pools as fp32 keys and values [n, Hkv, 64, Dh]."""
+  fmt, ke, ks, ve, vs = _mx_views(k_cache, v_cache, Dh)
+  pages = pages.long().clamp(0, k_cache.shape[0] - 1)
+  ke, ve = ke[pages], ve[pages]
+  code = ke if fmt == "mxfp8" else torch.stack([ke & 15, ke >> 4], -1).flatten(-2)
+  k = mx_decode(code, ks[pages][..., _mx_key_scale(torch.arange(64, device=ks.device))].transpose(2, 3), fmt)
+  ve = ve.permute(0, 1, 2, 4, 3, 5).flatten(2, 3)  # [n, Hkv, 64, r, group (even / odd)]
+  code = ve.unflatten(-1, (-1, 2)) if fmt == "mxfp8" else torch.stack([ve & 15, ve >> 4], -1)
+  return k, mx_decode(code.transpose(3, 4).flatten(3), vs[pages], fmt)
+
+
+def mx_gather(k_cache, v_cache, table, n: int, Dh: int):
+  """Dense [n, Hkv, Dh] K and V (fp32) of one sequence from its block table."""
+  k, v = mx_read(k_cache, v_cache, table[:-(-n // 64)], Dh)
+  return tuple(t.transpose(1, 2).flatten(0, 1)[:n] for t in (k, v))
+
+
+def kv_read_mx(k_cache, v_cache, block_tables, ctx_lens, k_out, v_out) -> None:
+  """The tables' pages as bf16 pages [entries, Hkv, 64, Dh] and (storage chunk-major) [entries, Hkv, Dh, 64]; zeros past the contexts."""
+  B, W = block_tables.shape
+  k, v = mx_read(k_cache, v_cache, block_tables.flatten(), k_out.shape[-1])
+  live = (torch.arange(W * 64, device=k.device)[None] < ctx_lens[:, None]).view(B * W, 1, 64, 1)
+  k_out.copy_(torch.where(live, k, 0.0))
+  v_chunks(v_out).copy_(torch.where(live, v, 0.0).unflatten(2, (8, 8)).transpose(3, 4))
+
+
+def attn_decode_mx(q, k_cache, v_cache, block_tables, ctx_lens, scale):
+  """q [B, H, Dh] -> [B, H, Dh] over pools in 8 or 4 bits"""
+  out = torch.zeros_like(q)
+  width = 64 * block_tables.shape[1]
+  for b in range(q.shape[0]):
+    n = min(int(ctx_lens[b]), width)
+    if n > 0:
+      out[b] = _attend(q[b:b + 1], *mx_gather(k_cache, v_cache, block_tables[b], n, q.shape[-1]), scale, None)[0].to(q.dtype)
+  return out
+
+
 def sample_greedy(logits: torch.Tensor) -> torch.Tensor:
   return logits.float().argmax(dim=-1).to(torch.int32)
 
