@@ -299,6 +299,46 @@ def test_decode_stale_bytes_gpu(gpu, fmt, Dh):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("waves", [1, 2, 4])
+@pytest.mark.parametrize("fmt,Dh,H,Hkv", [("mxfp4", 128, 8, 1), ("mxfp8", 128, 32, 2), ("mxfp4", 64, 3, 3), ("mxfp8", 64, 14, 2)])
+def test_decode_parts_gpu(gpu, fmt, Dh, H, Hkv, waves, monkeypatch):
+  """Contexts in parts, shorter ones than others and some without any: merged in the launch, the same whoever comes last, tickets left at
+  zero; one sequence's parts more than one round of the merge."""
+  s = Seqs(fmt, [1, 63, 64, 65, 0, 300, 640, 1350], Hkv, Dh, dev=gpu, width=22)
+  s.spoil()
+  monkeypatch.setattr(K, "mx_decode_waves", lambda *a: waves)
+  for least in (1, 2, 5):
+    monkeypatch.setattr(K.MXDecodeWorkspace, "parts", staticmethod(lambda b, h, pages: (least, -(-pages // least))))
+    ws = K.MXDecodeWorkspace(8, H, Hkv, Dh, 22 * PAGE, gpu)
+    a = check_decode(s, H, Dh ** -0.5, ws=ws)
+    for _ in range(3):
+      assert torch.equal(a, check_decode(s, H, Dh ** -0.5, ws=ws))
+    assert (ws.tickets == 0).all()
+
+
+@pytest.mark.gpu
+def test_decode_workspace_gpu(gpu):
+  """Wider tables than the workspace was made for, fewer sequences, and the rule's own choice at many sizes."""
+  s = Seqs("mxfp4", [70, 1200, 0], 2, 64, dev=gpu, width=40)
+  for max_ctx in (64, 700, 40 * PAGE):
+    check_decode(s, 4, 0.125, ws=K.MXDecodeWorkspace(5, 4, 2, 64, max_ctx, gpu))
+  with pytest.raises(RuntimeError, match="workspace"):
+    check_decode(s, 4, 0.125, ws=K.MXDecodeWorkspace(2, 4, 2, 64, 4096, gpu))
+
+
+def test_decode_parts_rule():
+  for batch in (1, 3, 16, 64, 200, 512):
+    for Hkv in (1, 2, 8, 32):
+      for pages in (1, 4, 11, 16, 17, 64, 129, 513, 4096):
+        least, most = K.MXDecodeWorkspace.parts(batch, Hkv, pages)
+        assert 1 <= most <= pages and least * most >= pages and least <= 128
+        ws = K.MXDecodeWorkspace(batch, 16, Hkv, 64, min(pages, 64) * PAGE, "meta")
+        for b in (1, batch):
+          least, most = ws.partition(b, pages)
+          assert least * most >= pages and (most == 1 or b * most <= ws.rows) and most <= pages
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FMTS)
 def test_decode_not_finite_gpu(gpu, fmt):
   """A NaN in a group of keys makes its sequence's heads NaN; one in a group of values those 32 dims; no other sequence."""

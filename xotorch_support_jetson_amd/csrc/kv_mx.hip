@@ -15,6 +15,7 @@
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <cmath>
 #include "handover.h"
 
 namespace xot {
@@ -301,17 +302,35 @@ struct DecodeArgs {
   float scale_log2;
 };
 
+// Four results O / L in bf16.
+__device__ __forceinline__ void st_results(uint16_t* p, const f32x4& O, float L) {
+  s16x4 y;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) y[r] = (short)f2bf(O[r] / L);
+  *reinterpret_cast<s16x4*>(p) = y;
+}
+
+// NW waves share a part of a (sequence, KV head)'s pages, wave w takes pages w, w + NW, ... with the next one's loads in flight under
+// this one's math, and meet in LDS.  A context of several parts (at most nparts, of ppp pages and more) is merged by the workgroup that
+// arrives last (tickets [B][Hkv], zero between launches), in the parts' order whoever it is.
+// Bound by memory where the pairs fill the chip: 512 sequences of 1500 tokens, 32 heads of 128 on 8, mxfp8 1.66 GB in 257 us (6.5 TB/s),
+// mxfp4 856 MB in 138 us (6.2 TB/s); of 525 tokens, 64 heads, mxfp4 58 us (5.0 TB/s of what counts).  A page of mxfp4 is about 330 vector
+// operations a wave, 190 of them making bf16 values; K needs none.  Without loads ahead and parts: 87 us, and 8 sequences of 32000
+// tokens 239 us, now 49.
 template <int DH, bool FP8, int NW>
-__global__ __launch_bounds__(64 * NW) void attn_decode_mx_kernel(const DecodeArgs A) {
+__global__ __launch_bounds__(64 * NW, 2) void attn_decode_mx_kernel(const DecodeArgs A) {
   using M = Mx<DH, FP8>;
   using R = PageRegs<DH, FP8>;
   constexpr int J = M::J, LD = DH + 4;
   extern __shared__ __attribute__((aligned(16))) float sm[];
-  const int kvh = blockIdx.x % A.Hkv, b = blockIdx.x / A.Hkv;
+  const int kvh = blockIdx.x % A.Hkv, bp = blockIdx.x / A.Hkv, part = bp % A.nparts, b = bp / A.nparts;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, G = A.H / A.Hkv;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int ctx = min(max(A.ctx_lens[b], 0), A.width * PAGE);
-  const int first = 0, last = (ctx + PAGE - 1) / PAGE;
+  const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ctx = min(max(A.ctx_lens[b], 0), A.width * PAGE), pages = (ctx + PAGE - 1) / PAGE;
+  const int parts = max(1, min(A.nparts, (pages + A.ppp - 1) / A.ppp));
+  if (part >= parts) return;  // the whole workgroup
+  const int share = pages / parts, rest = pages - share * parts;
+  const int first = part * share + min(part, rest), last = first + share + (part < rest ? 1 : 0);
 
   // the query in two parts
   i32x8 qhi = {0, 0, 0, 0, 0, 0, 0, 0}, qlo = qhi;
@@ -360,88 +379,101 @@ __global__ __launch_bounds__(64 * NW) void attn_decode_mx_kernel(const DecodeArg
   const int32_t* bt = A.tables + (size_t)b * A.width;
   const int krow = 8 * (c >> 2) + (c & 3);
 
-  auto load = [&](int p, R& x) {
-    const long page = min(max(bt[p], 0), A.num_pages - 1);
+  auto page_of = [&](int p) -> long { return min(max(bt[min(p, last - 1)], 0), A.num_pages - 1); };
+  // (read once a launch: non-temporal, as fast as plain loads for small caches and up to 11 % faster for large ones)
+  auto ld = [](const uint8_t* p) -> u32x4 { return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)); };
+  // page p of the sequence, which lies at `page`.  Rows past the context read its last row again: no bytes that do not count
+  // (512 contexts of 525 tokens end 13 tokens into a page)
+  auto load = [&](int p, long page, R& x) {
     const uint8_t* kp = A.kc + ((size_t)page * A.Hkv + kvh) * M::BYTES;
     const uint8_t* vp = A.vc + ((size_t)page * A.Hkv + kvh) * M::BYTES;
+    const int end = ctx - 1 - p * PAGE;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int i = 0; i < R::KV; ++i)
-        x.k[t][i] = *reinterpret_cast<const u32x4*>(kp + (32 * (t >> 1) + 4 * (t & 1) + krow) * M::ROW + 64 * i +
-                                                    16 * (DH == 64 && !FP8 ? g & 1 : g));
+        x.k[t][i] = ld(kp + (uint32_t)(min(32 * (t >> 1) + 4 * (t & 1) + krow, end) * M::ROW + 16 * (DH == 64 && !FP8 ? g & 1 : g)) + 64 * i);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int u = 0; u < R::VU; ++u)
+        x.v[kk][u] = ld(vp + (uint32_t)((min(32 * kk + 8 * g + u * M::KC, end) / M::KC) * 256 + 16 * c));
     x.ks = *reinterpret_cast<const uint32_t*>(kp + M::ELEMS + 64 * (g & (J - 1)) + 4 * c);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
-      for (int u = 0; u < R::VU; ++u)
-        x.v[kk][u] = *reinterpret_cast<const u32x4*>(vp + (((32 * kk + 8 * g) / M::KC + u) * 16 + c) * 16);
-#pragma unroll
-      for (int u = 0; u < R::VS; ++u) x.vs[kk][u] = *reinterpret_cast<const u32x4*>(vp + M::ELEMS + (32 * kk + 8 * g) * J + 16 * u);
+      for (int u = 0; u < R::VS; ++u) x.vs[kk][u] = ld(vp + M::ELEMS + (32 * kk + 8 * g) * J + 16 * u);
     }
   };
-
-  for (int p = first + wave; p < last; p += NW) {
-    R x;
-    load(p, x);
+  // What lies past the context may be anything, NaN too: it becomes zeros (their probabilities are 0, but 0 NaN is NaN).
+  // left: keys of this lane group inside the context
+  auto cut = [&](R& x, int left) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int key = 0; key < 8; ++key) {
+        const bool dead = 32 * kk + key >= left;
+        auto put = [&](u32x4 (&w)[R::VU], int i, uint32_t keep, uint32_t or_) {
+          w[i >> 2][i & 3] = dead ? (w[i >> 2][i & 3] & keep) | or_ : w[i >> 2][i & 3];
+        };
+        auto puts = [&](int i, uint32_t keep, uint32_t or_) {
+          x.vs[kk][i >> 2][i & 3] = dead ? (x.vs[kk][i >> 2][i & 3] & keep) | or_ : x.vs[kk][i >> 2][i & 3];
+        };
+        const uint32_t other = key & 1 ? 0xffffu : 0xffff0000u;
+        if constexpr (M::NB >= 4) {
+#pragma unroll
+          for (int i = 0; i < M::NB / 4; ++i) put(x.v[kk], key * (M::NB / 4) + i, 0u, 0u);
+        } else {
+          put(x.v[kk], key >> 1, other, 0u);
+        }
+        if constexpr (J == 4) puts(key, 0u, 0x7f7f7f7fu);
+        else puts(key >> 1, other, 0x7f7f7f7fu & ~other);
+      }
+  };
+  auto compute = [&](int p, R& x) {
     f32x4 st[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       st[t] = score_mfma<DH, FP8>(x.k[t], qhi, f32x4{0.f, 0.f, 0.f, 0.f}, x.ks, shi, t);
       if (DH == 128) st[t] = score_mfma<DH, FP8>(x.k[t], qlo, st[t], x.ks, slo, t);
     }
-    const int left = ctx - p * PAGE - 8 * g;  // keys of this lane group inside the context
-    float mx = NEG_BIG;
+    if (ctx - p * PAGE < PAGE) {  // (the last page)
+      const int left = ctx - p * PAGE - 8 * g;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[t][r] = 32 * (t >> 1) + 4 * (t & 1) + r < left ? st[t][r] : -INFINITY;
+      cut(x, left);
+    }
+    float mx = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float v = 32 * (t >> 1) + 4 * (t & 1) + r < left ? st[t][r] * A.scale_log2 : -INFINITY;
-        st[t][r] = v;
-        mx = fmaxf(mx, v);
-      }
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[t][r]);
     mx = xor_max<16>(mx);
     mx = xor_max<32>(mx);
-    const float mn = fmaxf(m, mx), alpha = exp2f(m - mn);
+    const float mn = fmaxf(m, mx * A.scale_log2);  // (the scale is positive)
+    const float alpha = __builtin_amdgcn_exp2f(m - mn);
     m = mn;
-    l *= alpha;
+    if (__ballot(alpha != 1.f)) {  // a head's maximum moved
+      l *= alpha;
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      o[j][0] *= alpha;
-      o[j][1] *= alpha;
+      for (int j = 0; j < J; ++j) {
+        o[j][0] *= alpha;
+        o[j][1] *= alpha;
+      }
     }
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
-      s16x8 pf;
+      u32x4 pw;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float pv = exp2f(st[2 * kk + h][r] - mn);
-          l += pv;
-          pf[4 * h + r] = (short)f2bf(pv);
-        }
-      // what lies past the context may be anything, NaN too: it becomes zeros (their probabilities are 0, but 0 NaN is NaN)
-      constexpr int ND = 2 * M::NB;  // dwords of eight keys' elements
-      uint32_t vd[ND], sd[2 * J];
-#pragma unroll
-      for (int i = 0; i < ND; ++i) vd[i] = x.v[kk][i >> 2][i & 3];
-#pragma unroll
-      for (int i = 0; i < 2 * J; ++i) sd[i] = x.vs[kk][i >> 2][i & 3];
-      if (ctx - p * PAGE < PAGE) {
-#pragma unroll
-        for (int key = 0; key < 8; ++key) {
-          const bool dead = 32 * kk + key >= left;
-          if constexpr (M::NB >= 4) {
-#pragma unroll
-            for (int i = 0; i < M::NB / 4; ++i) vd[key * (M::NB / 4) + i] = dead ? 0 : vd[key * (M::NB / 4) + i];
-          } else {
-            vd[key >> 1] = dead ? vd[key >> 1] & (key & 1 ? 0xffffu : 0xffff0000u) : vd[key >> 1];
-          }
-          if constexpr (J == 4) sd[key] = dead ? 0x7f7f7f7fu : sd[key];
-          else sd[key >> 1] = dead ? (key & 1 ? (sd[key >> 1] & 0xffffu) | 0x7f7f0000u : (sd[key >> 1] & 0xffff0000u) | 0x7f7fu) : sd[key >> 1];
-        }
+      for (int e = 0; e < 8; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(st[2 * kk + (e >> 2)][e & 3], A.scale_log2, -mn));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(st[2 * kk + (e >> 2)][(e & 3) + 1], A.scale_log2, -mn));
+        l += p0 + p1;
+        pw[e >> 1] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p0, p1}), bf16x2_t));
       }
+      const s16x8 pf = __builtin_bit_cast(s16x8, pw);
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         u32x4 ae, ao;
@@ -450,9 +482,10 @@ __global__ __launch_bounds__(64 * NW) void attn_decode_mx_kernel(const DecodeArg
           uint32_t y[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int key = 2 * n + i, at = key * M::NB + (FP8 ? 2 * j : j);  // byte among the eight keys'
-            const float s = scale_of(sd[key * J / 4], (key * J + j) & 3);
-            y[i] = FP8 ? from_fp8(vd[at >> 2], s, (at >> 1) & 1) : from_fp4(vd[at >> 2], s, at & 3);
+            const int key = 2 * n + i, at = key * M::NB + (FP8 ? 2 * j : j), sa = key * J + j;  // bytes among the eight keys'
+            const uint32_t w = x.v[kk][at >> 4][(at >> 2) & 3];
+            const float s = scale_of(x.vs[kk][sa >> 4][(sa >> 2) & 3], sa & 3);
+            y[i] = FP8 ? from_fp8(w, s, (at >> 1) & 1) : from_fp4(w, s, at & 3);
           }
           ae[n] = low_halves(y[0], y[1]);
           ao[n] = high_halves(y[0], y[1]);
@@ -461,42 +494,119 @@ __global__ __launch_bounds__(64 * NW) void attn_decode_mx_kernel(const DecodeArg
         o[j][1] = mfma16(__builtin_bit_cast(s16x8, ao), pf, o[j][1]);
       }
     }
+  };
+
+  {
+    R xa, xb;
+    int p = first + wave;
+    if (p < last) load(p, page_of(p), xa);
+    long nxt = last > first ? page_of(p + NW) : 0;  // (scalar reads of the table, ahead of the loads that need them)
+    while (p < last) {
+      if (p + NW < last) {
+        load(p + NW, nxt, xb);
+        nxt = page_of(p + 2 * NW);
+      }
+      compute(p, xa);
+      p += NW;
+      if (p >= last) break;
+      if (p + NW < last) {
+        load(p + NW, nxt, xa);
+        nxt = page_of(p + 2 * NW);
+      }
+      compute(p, xb);
+      p += NW;
+    }
   }
 
-  // the waves meet in LDS: [NW][G][LD] sums, [NW][G][2] maxima and sums of weights
   l = xor_sum<16>(l);
   l = xor_sum<32>(l);
-  float* ml = sm + NW * G * LD;
-  if (c < G) {
-    float* so = sm + (wave * G + c) * LD + 8 * g;
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      *reinterpret_cast<f32x4*>(so + 32 * j) = f32x4{o[j][0][0], o[j][1][0], o[j][0][1], o[j][1][1]};
-      *reinterpret_cast<f32x4*>(so + 32 * j + 4) = f32x4{o[j][0][2], o[j][1][2], o[j][0][3], o[j][1][3]};
+  const size_t row0 = ((size_t)b * A.nparts * A.Hkv + kvh) * G, step = (size_t)A.Hkv * G;  // partial results: part 0's first head, from part to part
+  auto leave = [&](int hq, int d, const f32x4& O, float mm, float L) {
+    if (parts == 1) {
+      if (ctx > 0) st_results(A.out + ((size_t)b * A.H + kvh * G + hq) * DH + d, O, L);
+      else *reinterpret_cast<s16x4*>(A.out + ((size_t)b * A.H + kvh * G + hq) * DH + d) = s16x4{0, 0, 0, 0};
+      return;
     }
-    if (g == 0) {
-      ml[(wave * G + c) * 2] = m;
-      ml[(wave * G + c) * 2 + 1] = l;
+    const size_t row = row0 + part * step + hq;
+    agent_store4(A.ws_o + row * DH + d, O);
+    if (d == 0) agent_store2(A.ws_ml + row * 2, mm, L);
+  };
+  if constexpr (NW == 1) {
+    if (c < G)
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        leave(c, 32 * j + 8 * g, f32x4{o[j][0][0], o[j][1][0], o[j][0][1], o[j][1][1]}, m, l);
+        leave(c, 32 * j + 8 * g + 4, f32x4{o[j][0][2], o[j][1][2], o[j][0][3], o[j][1][3]}, m, l);
+      }
+  } else {  // the waves meet in LDS: [NW][G][LD] sums, [NW][G][2] maxima and sums of weights
+    float* ml = sm + NW * G * LD;
+    if (c < G) {
+      float* so = sm + (wave * G + c) * LD + 8 * g;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        *reinterpret_cast<f32x4*>(so + 32 * j) = f32x4{o[j][0][0], o[j][1][0], o[j][0][1], o[j][1][1]};
+        *reinterpret_cast<f32x4*>(so + 32 * j + 4) = f32x4{o[j][0][2], o[j][1][2], o[j][0][3], o[j][1][3]};
+      }
+      if (g == 0) {
+        ml[(wave * G + c) * 2] = m;
+        ml[(wave * G + c) * 2 + 1] = l;
+      }
+    }
+    __syncthreads();
+    for (int e = 4 * threadIdx.x; e < G * DH; e += 4 * NW * 64) {
+      const int hq = e / DH, d = e - hq * DH;
+      float mm = NEG_BIG;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) mm = fmaxf(mm, ml[(w * G + hq) * 2]);
+      float L = 0.f;
+      f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {  // (a wave without pages: m = NEG_BIG, l = 0, o = 0)
+        const float f = __builtin_amdgcn_exp2f(ml[(w * G + hq) * 2] - mm);
+        L += ml[(w * G + hq) * 2 + 1] * f;
+        O += *reinterpret_cast<const f32x4*>(sm + (w * G + hq) * LD + d) * f;
+      }
+      leave(hq, d, O, mm, L);
     }
   }
+  if (parts == 1) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the partial results have left
   __syncthreads();
+  __shared__ int last_sm;
+  int* t = A.tickets + b * A.Hkv + kvh;
+  if (threadIdx.x == 0) last_sm = __hip_atomic_fetch_add(t, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+  __syncthreads();
+  if (!last_sm) return;
+  if (threadIdx.x == 0) __hip_atomic_store(t, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   for (int e = 4 * threadIdx.x; e < G * DH; e += 4 * NW * 64) {
     const int hq = e / DH, d = e - hq * DH;
-    float mm = NEG_BIG;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) mm = fmaxf(mm, ml[(w * G + hq) * 2]);
-    float L = 0.f;
+    float mm = NEG_BIG, L = 0.f;
     f32x4 O = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < parts; s0 += 8) {
+      f32x2_t ml[8];
+      f32x4 po[8];
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float f = exp2f(ml[(w * G + hq) * 2] - mm);
-      L += ml[(w * G + hq) * 2 + 1] * f;
-      O += *reinterpret_cast<const f32x4*>(sm + (w * G + hq) * LD + d) * f;
+      for (int i = 0; i < 8; ++i) {
+        const size_t row = row0 + min(s0 + i, parts - 1) * step + hq;
+        ml[i] = agent_load2(A.ws_ml + row * 2);
+        po[i] = agent_load4(A.ws_o + row * DH + d);
+      }
+      float mx = mm;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, ml[i][0]);
+      const float f0 = __builtin_amdgcn_exp2f(mm - mx);
+      L *= f0;
+      O *= f0;
+      mm = mx;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (s0 + i < parts) {
+          const float f = __builtin_amdgcn_exp2f(ml[i][0] - mm);
+          L += ml[i][1] * f;
+          O += po[i] * f;
+        }
     }
-    s16x4 y;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) y[r] = (short)f2bf(ctx > 0 ? O[r] / L : 0.f);
-    *reinterpret_cast<s16x4*>(A.out + ((size_t)b * A.H + kvh * G + hq) * DH + d) = y;
+    st_results(A.out + ((size_t)b * A.H + kvh * G + hq) * DH + d, O, L);
   }
 }
 
@@ -597,7 +707,7 @@ void kv_read_mx(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::
 
 void attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables,
                     const at::Tensor& ctx_lens, at::Tensor& out, at::Tensor& ws_o, at::Tensor& ws_ml, at::Tensor& tickets,
-                    int64_t pages_per_part, int64_t nparts, double scale) {
+                    int64_t pages_per_part, int64_t nparts, int64_t waves, double scale) {
   const char* op = "attn_decode_mx";
   XCHECK(q.is_cuda() && q.dim() == 3, op, ": q must be [B, H, Dh] on a GPU");
   const at::Device dev = q.device();
@@ -616,14 +726,26 @@ void attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Te
   XCHECK(tables.size(1) >= 1 && tables.size(1) < (1 << 24), op, ": block_tables of no or too many columns");
   XCHECK(out.numel() == q.numel(), op, ": out must have q's shape");
   XCHECK((reinterpret_cast<uintptr_t>(q.data_ptr()) | reinterpret_cast<uintptr_t>(out.data_ptr())) % 16 == 0, op, ": q and out must be aligned to 16 bytes");
-  XCHECK(pages_per_part >= 1 && nparts >= 1, op, ": bad partitioning");
+  XCHECK(pages_per_part >= 1 && pages_per_part <= (1 << 24) && nparts >= 1 && nparts <= tables.size(1), op, ": bad partitioning");
+  XCHECK(waves == 1 || waves == 2 || waves == 4, op, ": 1, 2 or 4 waves");
+  XCHECK(scale > 0 && std::isfinite(scale), op, ": the scale must be positive");
   if (B == 0) return;
   XCHECK(B * Hkv * nparts < (int64_t(1) << 24), op, ": too many parts for one launch");
+  if (nparts > 1)
+    XCHECK(tickets.numel() >= B * Hkv && ws_o.numel() >= B * nparts * H * Dh && ws_ml.numel() >= B * nparts * H * 2 &&
+               (reinterpret_cast<uintptr_t>(ws_o.data_ptr()) | reinterpret_cast<uintptr_t>(ws_ml.data_ptr())) % 16 == 0,
+           op, ": workspace small");
   const DecodeArgs a = {bf(q), k_cache.data_ptr<uint8_t>(), v_cache.data_ptr<uint8_t>(), tables.data_ptr<int32_t>(), ctx_lens.data_ptr<int32_t>(),
                         bf(out), ws_o.data_ptr<float>(), ws_ml.data_ptr<float>(), tickets.data_ptr<int32_t>(), (int)tables.size(1), (int)H,
                         (int)Hkv, (int)pages_per_part, (int)nparts, (int)k_cache.size(0), (float)scale * LOG2E};
-  const size_t lds = (size_t)4 * (H / Hkv) * (Dh + 6) * sizeof(float);
-#define GO(DHV, F) attn_decode_mx_kernel<DHV, F, 4><<<(unsigned)(B * Hkv), 256, lds, stream()>>>(a)
+  const size_t lds = waves == 1 ? 0 : (size_t)waves * (H / Hkv) * (Dh + 6) * sizeof(float);  // at most 34 KB
+  const unsigned units = (unsigned)(B * nparts * Hkv);
+#define GO(DHV, F)                                                                                   \
+  do {                                                                                               \
+    if (waves == 1) attn_decode_mx_kernel<DHV, F, 1><<<units, 64, lds, stream()>>>(a);               \
+    else if (waves == 2) attn_decode_mx_kernel<DHV, F, 2><<<units, 128, lds, stream()>>>(a);         \
+    else attn_decode_mx_kernel<DHV, F, 4><<<units, 256, lds, stream()>>>(a);                         \
+  } while (0)
   MX_GO(fp8, Dh, GO);
 #undef GO
 }

@@ -393,13 +393,50 @@ def kv_read_mx(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch
 
 
 class MXDecodeWorkspace:
-  """Scratch of attn_decode_mx for every batch up to max_batch at this context bound."""
+  """Scratch of attn_decode_mx for every batch up to max_batch at this context bound (wider tables: parts as long as the scratch allows).
+  Calls that share one run one after the other: on one stream, or ordered by events."""
 
   def __init__(self, max_batch: int, H: int, Hkv: int, Dh: int, max_ctx: int, device):
-    self.max_batch = max_batch
-    self.o = torch.empty(1, dtype=torch.float32, device=device)
-    self.ml = torch.empty(1, dtype=torch.float32, device=device)
+    self.max_batch, self.Hkv = max_batch, Hkv
+    pages = max(1, -(-max_ctx // PAGE))
+    rows = max((b * p for b, p in ((b, self.parts(b, Hkv, pages)[1]) for b in range(1, max_batch + 1)) if p > 1), default=0)
+    self.rows = rows  # parts of all sequences
+    self.o = torch.empty(max(1, rows * H * Dh), dtype=torch.float32, device=device)
+    self.ml = torch.empty(max(1, rows * H * 2), dtype=torch.float32, device=device)
     self.tickets = torch.zeros(max_batch * Hkv, dtype=torch.int32, device=device)
+
+  @staticmethod
+  def parts(batch: int, Hkv: int, pages: int):
+    """(least pages of a part, most parts of a context) at tables of this width.  Cut while the units (of four waves, two a CU at
+    once) stay within two a CU, and no part is shorter than a page a wave, or two in longer contexts, whose parts are more to merge: us in
+    parts of 4 / 8 / 16 / 64 pages, mxfp4, 32 heads of 128 on 8: 700 tokens 6.4 / 6.9 uncut, 8000 11.4 / 9.5 / 10.2, 16 sequences of 500 to
+    2000 - / 11.2 / 10.8 (12.9 uncut), 8 of 32000 - / - / 60 / 49 (239 uncut).  From 256 pairs on contexts below 64 pages stay whole: 8
+    sequences of up to 700 tokens on 32 KV heads 7.5 uncut, 8.4 in 2, 64 of 30 to 2000 on 8 20.8, 26 in 2.  Past 128 pages every context is
+    cut: its longest part ends the launch."""
+    pairs = max(1, batch * Hkv)
+    most = min(512 // pairs, pages // (4 if pages <= 16 else 8)) if pairs < 256 or pages >= 64 else 1
+    most = max(1, most, -(-pages // 128))
+    return -(-pages // most), most
+
+  def partition(self, batch: int, pages: int):
+    if batch > self.max_batch:
+      raise RuntimeError(f"decode workspace for batches of {self.max_batch}, not {batch}")
+    ppp, most = self.parts(batch, self.Hkv, pages)
+    if most > 1 and batch * most > self.rows:
+      most = max(1, self.rows // batch)
+      ppp = -(-pages // most)
+    return ppp, most
+
+
+def mx_decode_waves(pairs: int, pages: int, fp8: bool) -> int:
+  """Waves of an attn_decode_mx workgroup.  Four share the pages of a (sequence, KV head) where there are few of those, or many pages; many
+  with few pages each leave some of four waves idle.  us with 1 / 2 / 4, heads of 128, even contexts | ragged: mxfp4 1024 pairs of 520
+  tokens 18.3 / 17.9 / 19.6 | 16.7 / 14.1 / 16.6, 2048 of 200 16.9 / 18.5 / 20.9 | 14.1 / 14.8 / 19.0, 4096 of 520 57 / 58 / 67 | 40 / 40 /
+  50, of 1000 96 / 97 / 99 | 66 / 63 / 72, 512 of 520 16.5 / 13.2 / 11.5; mxfp8 4096 of 520 103 / 98 / 104 | 66 / 60 / 70, of 1500 265 / 257
+  / 253 | 175 / 156 / 162; 1024 of 30 to 8000 129 in 2, 106 in 4; 2048 of 100 to 1500, heads of 64, 33 / 29 / 28."""
+  if pairs < 1024 or pages > 16:
+    return 4
+  return 1 if pairs >= 2048 and pages <= 12 and not fp8 else 2
 
 
 def attn_decode_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
@@ -413,10 +450,13 @@ def attn_decode_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
       return out
     return y
   B, H, Dh = q.shape
+  Hkv, width = k_cache.shape[1], block_tables.shape[1]
   if ws is None:
-    ws = MXDecodeWorkspace(B, H, k_cache.shape[1], Dh, block_tables.shape[1] * PAGE, q.device)
+    ws = MXDecodeWorkspace(B, H, Hkv, Dh, width * PAGE, q.device)
   out = torch.empty_like(q) if out is None else out
-  require().attn_decode_mx(q, k_cache, v_cache, block_tables, ctx_lens, out, ws.o, ws.ml, ws.tickets, block_tables.shape[1], 1, float(scale))
+  ppp, nparts = ws.partition(B, width)
+  waves = mx_decode_waves(B * Hkv, width, k_cache.shape[2] > PAGE * Dh)
+  require().attn_decode_mx(q, k_cache, v_cache, block_tables, ctx_lens, out, ws.o, ws.ml, ws.tickets, ppp, nparts, waves, float(scale))
   return out
 
 
