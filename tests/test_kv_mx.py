@@ -381,11 +381,33 @@ def test_prompt_gpu(gpu, fmt, Dh, H, Hkv, monkeypatch):
   ctx, new = [70, 5, 300, 128, 64, 1], [10, 5, 260, 1, 64, 1]
   s = Seqs(fmt, ctx, Hkv, Dh, dev=gpu, width=6)
   s.spoil()
-  whole, end = check_prompt(s, new, H, Dh ** -0.5)
-  assert (whole[end:] == 7).all()
+  for direct in (True, False):  # from the pools, and through bf16 pages
+    monkeypatch.setattr(K, "mx_turn", lambda *a: direct)
+    whole, end = check_prompt(s, new, H, Dh ** -0.5)
+    assert (whole[end:] == 7).all()
   for limit in (1, 2 * 6 * Hkv * PAGE * Dh * 4):  # a sequence, two sequences at a time
     monkeypatch.setattr(K, "MX_READ_BYTES", limit)
     assert torch.equal(check_prompt(s, new, H, Dh ** -0.5)[0], whole)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,Dh,H,Hkv", [("mxfp4", 128, 4, 1), ("mxfp8", 128, 16, 1), ("mxfp4", 64, 7, 1), ("mxfp8", 64, 2, 2), ("mxfp4", 128, 3, 3)])
+def test_turns_gpu(gpu, fmt, Dh, H, Hkv, monkeypatch):
+  """A few new tokens behind long contexts (in parts), none, a token alone, more tokens than keys would allow."""
+  s = Seqs(fmt, [1500, 2200, 33, 64, 1, 700], Hkv, Dh, dev=gpu, width=36)
+  s.spoil()
+  new = [3, 17, 0, 5, 1, 16]
+  a, end = check_prompt(s, new, H, Dh ** -0.5)
+  assert (a[end:] == 7).all()
+  for _ in range(3):
+    assert torch.equal(a, check_prompt(s, new, H, Dh ** -0.5)[0])
+  s = Seqs(fmt, [3, 0], Hkv, Dh, dev=gpu)  # (rows before the first key: zeros, as in attn_prefill)
+  for direct in (True, False):
+    monkeypatch.setattr(K, "mx_turn", lambda *a: direct)
+    q = torch.randn(7, H, Dh, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    out = K.attn_prefill_mx(q.to(gpu), s.k, s.v, s.tables, torch.tensor([0, 5, 7], dtype=torch.int32, device=gpu), s.ctx, 5, Dh ** -0.5)
+    close(out[2:5], *attend64(q[2:5], *s.kv[0], Dh ** -0.5, 0))
+    assert (out[:2] == 0).all() and (out[5:] == 0).all()
 
 
 @pytest.mark.gpu
@@ -403,6 +425,11 @@ def test_refusals_gpu(gpu):
     lambda: K.attn_decode_mx(q, s.k.cpu(), s.v, s.tables, s.ctx, 1.0),
     lambda: K.attn_decode_mx(q[:, :3].contiguous(), s.k, s.v, s.tables, s.ctx, 1.0),
     lambda: K.attn_decode_mx(torch.zeros(2, 34, 128, dtype=torch.bfloat16, device=gpu), s.k, s.v, s.tables, s.ctx, 1.0),
+    lambda: K.attn_decode_mx(q, s.k, s.v, s.tables, s.ctx, 0.0),
+    lambda: K.attn_decode_mx(q, s.k, s.v, s.tables, s.ctx, float("nan")),
+    lambda: K.attn_decode_mx(q, s.k, s.v, s.tables, s.ctx, 1.0, out=q.float()),
+    lambda: K.attn_prefill_mx(q, s.k, s.v, s.tables, torch.tensor([0, 2], dtype=torch.int32, device=gpu), s.ctx, 1, 1.0),
+    lambda: K.attn_prefill_mx(q, s.k, s.v, s.tables, torch.tensor([0, 1, 2], device=gpu), s.ctx, 1, 1.0),
     lambda: K.kv_read_mx(s.k, s.v, s.tables, s.ctx[:1], 128),
     lambda: K.kv_read_mx(s.k, s.v, s.tables, s.ctx, 64),
     lambda: K.kv_read_mx(s.k, s.v, s.tables, s.ctx, 128, k_out=torch.zeros(1, 2, 64, 128, dtype=torch.bfloat16, device=gpu)),

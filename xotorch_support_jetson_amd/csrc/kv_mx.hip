@@ -15,6 +15,7 @@
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <algorithm>
 #include <cmath>
 #include "handover.h"
 
@@ -99,24 +100,53 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 }
 
 // ============================================================================ write
-// Sixteen lanes a row of one head (q, k or v) of a token.  k is quantised from its rotation in fp32, v from its bf16; a group's largest
+// Sixteen lanes a row of one head (q, k or v) of a token; a wave takes a head's rows of four neighbouring tokens, whose elements lie side
+// by side in a page (keys 256 bytes, value units whole).  k is quantised from its rotation in fp32, v from its bf16; a group's largest
 // value is found among the lanes that hold it (on the bits: a NaN counts as larger than everything).  The rotation's products and sums are
 // rounded one by one, so that a value on the border between two elements falls the same way wherever it is computed.
 // Bound by its launch at a few tokens, by memory at many.
+template <int N>
+__device__ __forceinline__ void ld_bf16(const uint16_t* p, float (&x)[N]) {
+  static_assert(N == 2 || N == 4, "a dword or two");
+  if constexpr (N == 4) {
+    const uint64_t u = *reinterpret_cast<const uint64_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = bf2f((uint16_t)(u >> (16 * i)));
+  } else {
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+    x[0] = bf2f((uint16_t)u);
+    x[1] = bf2f((uint16_t)(u >> 16));
+  }
+}
+// N values under one scale -> N bytes of e4m3 or N / 2 of e2m1
+template <bool FP8, int N>
+__device__ __forceinline__ uint32_t mx_elements(const float (&x)[N], int e, bool bad) {
+  uint32_t y = 0;
+  const float s = pow2(FP8 ? -e : e);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) y |= FP8 ? to_fp8(x[i] * s, x[i + 1] * s) << (8 * i) : to_fp4(x[i], x[i + 1], s) << (4 * i);
+  return bad ? 0u : y;
+}
+template <int BYTES>
+__device__ __forceinline__ void st_bytes(uint8_t* p, uint64_t v) {
+  if constexpr (BYTES == 8) *reinterpret_cast<uint64_t*>(p) = v;
+  else if constexpr (BYTES == 4) *reinterpret_cast<uint32_t*>(p) = (uint32_t)v;
+  else if constexpr (BYTES == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)v;
+  else *p = (uint8_t)v;
+}
+
 template <int DH, bool FP8>
 __global__ __launch_bounds__(256) void rope_kv_write_mx_kernel(const uint16_t* __restrict__ qkv, const int32_t* __restrict__ pos,
                                                                const float* __restrict__ cos_sin, const int64_t* __restrict__ slots,
                                                                uint16_t* __restrict__ q_out, uint8_t* __restrict__ kc,
-                                                               uint8_t* __restrict__ vc, long rows, int H, int Hkv, int max_pos, long nslots) {
+                                                               uint8_t* __restrict__ vc, int T, int H, int Hkv, int max_pos, long nslots) {
 #pragma clang fp contract(off)
   using M = Mx<DH, FP8>;
-  constexpr int E = DH / 32, HALF = DH / 2;
-  const long row = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (row >= rows) return;  // (sixteen lanes together)
-  const int r = threadIdx.x & 15, N = H + 2 * Hkv;
-  const long t = row / N;
-  const int h = (int)(row - t * N);
-  const uint16_t* src = qkv + row * DH;
+  constexpr int E = DH / 32, HALF = DH / 2, KB = FP8 ? E : E / 2;  // dims a lane takes of each half; their bytes
+  const int N = H + 2 * Hkv, w = blockIdx.x * 4 + (threadIdx.x >> 6), quad = w / N, h = w - quad * N;
+  const int t = 4 * quad + ((threadIdx.x >> 4) & 3), r = threadIdx.x & 15;
+  if (t >= T) return;  // (sixteen lanes together, here and below)
+  const uint16_t* src = qkv + ((size_t)t * N + h) * DH;
   long slot = -1;
   if (h >= H) {
     slot = slots[t];
@@ -126,21 +156,26 @@ __global__ __launch_bounds__(256) void rope_kv_write_mx_kernel(const uint16_t* _
   if (h < H + Hkv) {
     int p = pos[t];
     p = p < 0 ? 0 : (p >= max_pos ? max_pos - 1 : p);
-    const float* cs = cos_sin + (size_t)p * DH;
-    float lo[E], hi[E];
+    const float* cs = cos_sin + (size_t)p * DH + E * r;
+    float x[E], y[E], lo[E], hi[E];
+    ld_bf16(src + E * r, x);
+    ld_bf16(src + HALF + E * r, y);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const float a = bf2f(src[E * r + i]), b = bf2f(src[HALF + E * r + i]), c = cs[E * r + i], s = cs[HALF + E * r + i];
-      lo[i] = a * c - b * s;
-      hi[i] = b * c + a * s;
+      const float c = cs[i], s = cs[HALF + i];
+      lo[i] = x[i] * c - y[i] * s;
+      hi[i] = y[i] * c + x[i] * s;
     }
     if (h < H) {
-      uint16_t* dst = q_out + ((size_t)t * H + h) * DH + E * r;
+      uint8_t* dst = reinterpret_cast<uint8_t*>(q_out + ((size_t)t * H + h) * DH + E * r);
+      uint64_t a = 0, b = 0;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        dst[i] = f2bf(lo[i]);
-        dst[HALF + i] = f2bf(hi[i]);
+        a |= (uint64_t)f2bf(lo[i]) << (16 * i);
+        b |= (uint64_t)f2bf(hi[i]) << (16 * i);
       }
+      st_bytes<2 * E>(dst, a);
+      st_bytes<2 * E>(dst + 2 * HALF, b);
       return;
     }
     uint8_t* page = kc + ((size_t)(slot / PAGE) * Hkv + (h - H)) * M::BYTES;
@@ -154,22 +189,9 @@ __global__ __launch_bounds__(256) void rope_kv_write_mx_kernel(const uint16_t* _
     b = lanes_max<32 / E>(b);
     const int ea = mx_exponent<DH, FP8>(a), eb = mx_exponent<DH, FP8>(b);
     const bool na = mx_bad(a), nb = mx_bad(b);
-    uint8_t* dst = page + off * M::ROW;
-    if constexpr (FP8) {
-#pragma unroll
-      for (int i = 0; i < E; i += 2) {
-        const float sa = pow2(-ea), sb = pow2(-eb);
-        const uint32_t x = na ? 0 : to_fp8(lo[i] * sa, lo[i + 1] * sa), y = nb ? 0 : to_fp8(hi[i] * sb, hi[i + 1] * sb);
-        *reinterpret_cast<uint16_t*>(dst + E * r + i) = (uint16_t)x;
-        *reinterpret_cast<uint16_t*>(dst + HALF + E * r + i) = (uint16_t)y;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; i += 2) {
-        dst[(E * r + i) / 2] = (uint8_t)(na ? 0 : to_fp4(lo[i], lo[i + 1], pow2(ea)));
-        dst[(HALF + E * r + i) / 2] = (uint8_t)(nb ? 0 : to_fp4(hi[i], hi[i + 1], pow2(eb)));
-      }
-    }
+    uint8_t* dst = page + off * M::ROW + KB * r;
+    st_bytes<KB>(dst, mx_elements<FP8>(lo, ea, na));
+    st_bytes<KB>(dst + M::ROW / 2, mx_elements<FP8>(hi, eb, nb));
     if (r % (32 / E) == 0) {
       const int j = E * r / 32;
       uint8_t* sc = page + M::ELEMS + mx_key_scale(off);
@@ -179,75 +201,100 @@ __global__ __launch_bounds__(256) void rope_kv_write_mx_kernel(const uint16_t* _
     return;
   }
   uint8_t* page = vc + ((size_t)(slot / PAGE) * Hkv + (h - H - Hkv)) * M::BYTES;
-  uint8_t* dst = page + mx_value_off<DH, FP8>(off, r);
+  float x[M::J][2];
+#pragma unroll
+  for (int j = 0; j < M::J; ++j) ld_bf16(src + 32 * j + 2 * r, x[j]);
+  uint64_t y = 0;
+  uint32_t sc = 0;
 #pragma unroll
   for (int j = 0; j < M::J; ++j) {
-    const float x = bf2f(src[32 * j + 2 * r]), y = bf2f(src[32 * j + 2 * r + 1]);
-    const uint32_t a = lanes_max<16>(max(__float_as_uint(x) & 0x7fffffffu, __float_as_uint(y) & 0x7fffffffu));
+    const uint32_t a = lanes_max<16>(max(__float_as_uint(x[j][0]) & 0x7fffffffu, __float_as_uint(x[j][1]) & 0x7fffffffu));
     const int e = mx_exponent<DH, FP8>(a);
-    const bool bad = mx_bad(a);
-    if constexpr (FP8) {
-      const float s = pow2(-e);
-      *reinterpret_cast<uint16_t*>(dst + 2 * j) = (uint16_t)(bad ? 0 : to_fp8(x * s, y * s));
-    } else {
-      dst[j] = (uint8_t)(bad ? 0 : to_fp4(x, y, pow2(e)));
-    }
-    if (r == 0) page[M::ELEMS + off * M::J + j] = (uint8_t)(bad ? 255 : e + 127);
+    y |= (uint64_t)mx_elements<FP8>(x[j], e, mx_bad(a)) << (FP8 ? 16 * j : 8 * j);
+    sc |= (uint32_t)(mx_bad(a) ? 255 : e + 127) << (8 * j);
   }
+  st_bytes<M::NB>(page + mx_value_off<DH, FP8>(off, r), y);
+  if (r == 0) st_bytes<M::J>(page + M::ELEMS + off * M::J, sc);
 }
 
 // ============================================================================ read
 // One workgroup a page of one head: bf16 keys [64][DH] and values chunk-major (v_page_off), what the prompt attention reads.  Keys past
-// the context are zeros, in pages that hold some and (skip unset) in those that lie wholly past it.
+// the context are zeros, in pages that hold some and (skip unset) in those that lie wholly past it.  own: the table of what is written,
+// entry i page i.  Bound by memory (mostly its writes).
 template <int DH, bool FP8>
 __global__ __launch_bounds__(256) void kv_read_mx_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
                                                          const int32_t* __restrict__ tables, int width, const int32_t* __restrict__ ctx_lens,
                                                          uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out, int Hkv,
-                                                         int num_pages, bool skip) {
+                                                         int num_pages, bool skip, int32_t* __restrict__ own) {
   using M = Mx<DH, FP8>;
-  const long unit = blockIdx.x;
-  const int kvh = (int)(unit % Hkv);
-  const long entry = unit / Hkv;
-  const int b = (int)(entry / width), w = (int)(entry % width);
-  const int live = min(max(ctx_lens[b] - w * PAGE, 0), PAGE);
+  const int kvh = (int)(blockIdx.x % Hkv), entry = (int)(blockIdx.x / Hkv), b = entry / width, w = entry - b * width;
+  if (own != nullptr && kvh == 0 && threadIdx.x == 0) own[entry] = entry;
+  const int live = min(max(ctx_lens[b] - w * PAGE, 0), PAGE);  // (a context past the table's width: whole pages)
   if (live == 0 && skip) return;
   const long page = min(max(tables[entry], 0), num_pages - 1);
   const uint8_t* kp = kc + ((size_t)page * Hkv + kvh) * M::BYTES;
   const uint8_t* vp = vc + ((size_t)page * Hkv + kvh) * M::BYTES;
   uint16_t* ko = k_out + ((size_t)entry * Hkv + kvh) * PAGE * DH;
   uint16_t* vo = v_out + ((size_t)entry * Hkv + kvh) * PAGE * DH;
-  constexpr int CPR = DH / 8;
-  for (int i = threadIdx.x; i < PAGE * CPR; i += 256) {  // eight dims of a key
-    const int key = i / CPR, d = (i % CPR) * 8;
-    u32x4 y = {0, 0, 0, 0};
-    if (key < live) {
-      const float s = scale_of(kp[M::ELEMS + 64 * (d >> 5) + mx_key_scale(key)], 0);
-      const uint32_t* x = reinterpret_cast<const uint32_t*>(kp + key * M::ROW + (FP8 ? d : d / 2));
+  constexpr int CPR = DH / 8, KI = PAGE * CPR / 256;
+  // eight dims of a key a thread and turn, all loads first
+  uint32_t kx[KI][2], ks[KI];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) y[n] = FP8 ? from_fp8(x[n >> 1], s, n & 1) : from_fp4(x[0], s, n);
+  for (int n = 0; n < KI; ++n) {
+    const int i = threadIdx.x + 256 * n, key = i / CPR, d = (i % CPR) * 8;
+    if constexpr (FP8) {
+      const uint64_t u = *reinterpret_cast<const uint64_t*>(kp + key * M::ROW + d);
+      kx[n][0] = (uint32_t)u;
+      kx[n][1] = (uint32_t)(u >> 32);
+    } else {
+      kx[n][0] = kx[n][1] = *reinterpret_cast<const uint32_t*>(kp + key * M::ROW + d / 2);
+    }
+    ks[n] = kp[M::ELEMS + 64 * (d >> 5) + mx_key_scale(key)];
+  }
+  // eight keys of the dims 2 r, 2 r + 1 of a group: two threads share a lane's units, and J / 2 groups each
+  constexpr int VU = 8 / M::KC, JT = M::J / 2;
+  const int r = threadIdx.x & 15, half = (threadIdx.x >> 4) & 1, k0 = 8 * (threadIdx.x >> 5);
+  u32x4 v[VU];
+  uint32_t vs[2 * M::J];
+#pragma unroll
+  for (int u = 0; u < VU; ++u) v[u] = *reinterpret_cast<const u32x4*>(vp + ((k0 / M::KC + u) * 16 + r) * 16);
+#pragma unroll
+  for (int u = 0; u < 2 * M::J; ++u) vs[u] = *reinterpret_cast<const uint32_t*>(vp + M::ELEMS + k0 * M::J + 4 * u);
+#pragma unroll
+  for (int n = 0; n < KI; ++n) {
+    const int i = threadIdx.x + 256 * n, key = i / CPR, d = (i % CPR) * 8;
+    const float s = scale_of(ks[n], 0);
+    u32x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      y[e] = FP8 ? from_fp8(kx[n][e >> 1], s, e & 1) : from_fp4(kx[n][0], s, e);
+      y[e] = key < live ? y[e] : 0u;
     }
     *reinterpret_cast<u32x4*>(ko + key * DH + d) = y;
   }
-  for (int i = threadIdx.x; i < 128 * M::J; i += 256) {  // eight keys of two dims
-    const int r = i & 15, j = (i >> 4) % M::J, k0 = 8 * (i / (16 * M::J));
+#pragma unroll
+  for (int jj = 0; jj < JT; ++jj) {
     u32x4 lo, hi;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       uint32_t y[2];
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const int key = k0 + 2 * n + m;
-        y[m] = 0;
-        if (key < live) {
-          const uint8_t* x = vp + mx_value_off<DH, FP8>(key, r);
-          const float s = scale_of(vp[M::ELEMS + key * M::J + j], 0);
-          y[m] = FP8 ? from_fp8(reinterpret_cast<const uint16_t*>(x)[j], s, 0) : from_fp4(x[j], s, 0);
-        }
+        const int key = 2 * n + m;
+        // (both halves' groups are compile-time places: a thread converts one of the two)
+        auto conv = [&](int j) {
+          const int at = key * M::NB + (FP8 ? 2 * j : j), sa = key * M::J + j;
+          const uint32_t x = v[at >> 4][(at >> 2) & 3];
+          const float s = scale_of(vs[sa >> 2], sa & 3);
+          return FP8 ? from_fp8(x, s, (at >> 1) & 1) : from_fp4(x, s, at & 3);
+        };
+        y[m] = half ? conv(JT + jj) : conv(jj);
+        y[m] = k0 + key < live ? y[m] : 0u;
       }
       lo[n] = low_halves(y[0], y[1]);
       hi[n] = high_halves(y[0], y[1]);
     }
-    uint16_t* o = vo + v_page_off(k0, 32 * j + 2 * r, DH);
+    uint16_t* o = vo + v_page_off(k0, 32 * (half ? JT + jj : jj) + 2 * r, DH);
     *reinterpret_cast<u32x4*>(o) = lo;
     *reinterpret_cast<u32x4*>(o + 8) = hi;
   }
@@ -291,14 +338,14 @@ __device__ __forceinline__ f32x4 score_mfma(const u32x4 (&k)[PageRegs<DH, FP8>::
   }
 }
 
-struct DecodeArgs {
+struct AttnArgs {
   const uint16_t* q;
   const uint8_t *kc, *vc;
-  const int32_t *tables, *ctx_lens;
+  const int32_t *tables, *ctx_lens, *cu_q;
   uint16_t* out;
   float *ws_o, *ws_ml;
   int* tickets;
-  int width, H, Hkv, ppp, nparts, num_pages;
+  int T, width, H, Hkv, ppp, nparts, num_pages, blocks;
   float scale_log2;
 };
 
@@ -310,33 +357,46 @@ __device__ __forceinline__ void st_results(uint16_t* p, const f32x4& O, float L)
   *reinterpret_cast<s16x4*>(p) = y;
 }
 
-// NW waves share a part of a (sequence, KV head)'s pages, wave w takes pages w, w + NW, ... with the next one's loads in flight under
-// this one's math, and meet in LDS.  A context of several parts (at most nparts, of ppp pages and more) is merged by the workgroup that
-// arrives last (tickets [B][Hkv], zero between launches), in the parts' order whoever it is.
-// Bound by memory where the pairs fill the chip: 512 sequences of 1500 tokens, 32 heads of 128 on 8, mxfp8 1.66 GB in 257 us (6.5 TB/s),
-// mxfp4 856 MB in 138 us (6.2 TB/s); of 525 tokens, 64 heads, mxfp4 58 us (5.0 TB/s of what counts).  A page of mxfp4 is about 330 vector
-// operations a wave, 190 of them making bf16 values; K needs none.  Without loads ahead and parts: 87 us, and 8 sequences of 32000
-// tokens 239 us, now 49.
-template <int DH, bool FP8, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attn_decode_mx_kernel(const DecodeArgs A) {
+// One unit: 16 NB rows (tokens of a sequence x query heads of a KV head; single tokens: its G heads) against a part of the pages.
+// NW waves share the part, wave w takes pages w, w + NW, ... with the next one's loads in flight under this one's math, and meet in
+// LDS.  A context of several parts (at most nparts, of ppp pages and more) is merged by the workgroup that arrives last (a ticket a (rows,
+// KV head), zero between launches), in the parts' order whoever it is.
+// Bound by memory where the pairs of single tokens fill the chip: 512 sequences of 1500 tokens, 32 heads of 128 on 8, mxfp8 1.66 GB in 257
+// us (6.5 TB/s), mxfp4 856 MB in 138 us (6.2 TB/s); of 525 tokens, 64 heads, mxfp4 58 us (5.0 TB/s of what counts).  A page of mxfp4 is
+// about 330 vector operations a wave, 190 of them making bf16 values; K needs none.  Without loads ahead and parts: 87 us, and 8
+// sequences of 32000 tokens 239 us, now 49.
+template <int DH, bool FP8, int NW, int NB, bool PROMPT>
+__global__ __launch_bounds__(64 * NW, 2) void attn_mx_kernel(const AttnArgs A) {
+  static_assert(PROMPT || NB == 1, "a single token's heads are one column block");
   using M = Mx<DH, FP8>;
   using R = PageRegs<DH, FP8>;
   constexpr int J = M::J, LD = DH + 4;
   extern __shared__ __attribute__((aligned(16))) float sm[];
-  const int kvh = blockIdx.x % A.Hkv, bp = blockIdx.x / A.Hkv, part = bp % A.nparts, b = bp / A.nparts;
+  const int kvh = blockIdx.x % A.Hkv, bp = blockIdx.x / A.Hkv, part = bp % A.nparts, bu = bp / A.nparts;
+  const int b = PROMPT ? bu / A.blocks : bu, row0 = PROMPT ? (bu - b * A.blocks) * 16 * NB : 0;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, G = A.H / A.Hkv;
   const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int ctx = min(max(A.ctx_lens[b], 0), A.width * PAGE), pages = (ctx + PAGE - 1) / PAGE;
+  const int q0 = PROMPT ? min(max(A.cu_q[b], 0), A.T) : b, qlen = PROMPT ? min(max(A.cu_q[b + 1], q0), A.T) - q0 : 1, nrows = qlen * G;
+  if (PROMPT && row0 >= nrows) return;  // the whole workgroup, here and below
+  const int RN = PROMPT ? min(16 * NB, nrows - row0) : G, RS = PROMPT ? 16 * NB : G;  // rows, and from unit to unit
+  const int ctx = min(max(A.ctx_lens[b], 0), A.width * PAGE), pos0 = ctx - qlen;       // pos0: keys before the new tokens
+  const int seen = PROMPT ? max(0, pos0 + (row0 + RN - 1) / G + 1) : ctx;              // keys that the unit's last row sees
+  const int pages = (seen + PAGE - 1) / PAGE;
   const int parts = max(1, min(A.nparts, (pages + A.ppp - 1) / A.ppp));
-  if (part >= parts) return;  // the whole workgroup
+  if (part >= parts) return;
   const int share = pages / parts, rest = pages - share * parts;
   const int first = part * share + min(part, rest), last = first + share + (part < rest ? 1 : 0);
 
-  // the query in two parts
-  i32x8 qhi = {0, 0, 0, 0, 0, 0, 0, 0}, qlo = qhi;
-  int shi, slo;
-  {
-    const uint16_t* qp = A.q + ((size_t)b * A.H + kvh * G + min(c, G - 1)) * DH + 16 * g;
+  // the queries in two parts
+  i32x8 qhi[NB], qlo[NB];
+  int shi[NB], slo[NB], sees[NB];  // sees: the last key of the lane's row
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int row = row0 + 16 * nb + c, ti = PROMPT ? min(row, nrows - 1) / G : 0, hi_ = PROMPT ? min(row, nrows - 1) - ti * G : min(c, G - 1);
+    const bool ok = row < nrows;
+    sees[nb] = pos0 + ti;
+    qhi[nb] = qlo[nb] = i32x8{0, 0, 0, 0, 0, 0, 0, 0};
+    const uint16_t* qp = A.q + ((size_t)(q0 + ti) * A.H + kvh * G + hi_) * DH + 16 * g;
     s16x8 x[DH / 32];
     uint32_t a = 0;
 #pragma unroll
@@ -361,25 +421,30 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_decode_mx_kernel(const Decode
         lo = __builtin_amdgcn_cvt_pk_fp8_f32((f0 - h0[0]) * 16.f, (f1 - h0[1]) * 16.f, lo, false);
         lo = __builtin_amdgcn_cvt_pk_fp8_f32((f2 - h1[0]) * 16.f, (f3 - h1[1]) * 16.f, lo, true);
         const int at = 2 * i + n / 4;  // dword of the operand
-        if (c >= G) hi = lo = 0;
-        qhi[at] = hi;
-        if (DH == 128) qlo[at] = lo;
-        else qhi[4 + at] = lo;
+        if (!ok) hi = lo = 0;
+        qhi[nb][at] = hi;
+        if (DH == 128) qlo[nb][at] = lo;
+        else qhi[nb][4 + at] = lo;
       }
-    const bool bad = mx_bad(a) && c < G;
-    shi = bad ? 255 : e + 127;
-    slo = bad ? 255 : e + 127 - 4;
-    if (DH == 64 && g >= 2) shi = slo;
+    const bool bad = mx_bad(a) && ok;
+    shi[nb] = bad ? 255 : e + 127;
+    slo[nb] = bad ? 255 : e + 127 - 4;
+    if (DH == 64 && g >= 2) shi[nb] = slo[nb];
   }
 
-  float m = NEG_BIG, l = 0.f;
-  f32x4 o[J][2];
+  float m[NB], l[NB];
+  f32x4 o[NB][J][2];
 #pragma unroll
-  for (int j = 0; j < J; ++j) o[j][0] = o[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int nb = 0; nb < NB; ++nb) {
+    m[nb] = NEG_BIG;
+    l[nb] = 0.f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) o[nb][j][0] = o[nb][j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   const int32_t* bt = A.tables + (size_t)b * A.width;
   const int krow = 8 * (c >> 2) + (c & 3);
 
-  auto page_of = [&](int p) -> long { return min(max(bt[min(p, last - 1)], 0), A.num_pages - 1); };
+  auto page_of = [&](int p) -> long { return min(max(bt[min(p, last - 1)], 0), A.num_pages - 1); };  // (last > first)
   // (read once a launch: non-temporal, as fast as plain loads for small caches and up to 11 % faster for large ones)
   auto ld = [](const uint8_t* p) -> u32x4 { return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)); };
   // page p of the sequence, which lies at `page`.  Rows past the context read its last row again: no bytes that do not count
@@ -387,7 +452,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_decode_mx_kernel(const Decode
   auto load = [&](int p, long page, R& x) {
     const uint8_t* kp = A.kc + ((size_t)page * A.Hkv + kvh) * M::BYTES;
     const uint8_t* vp = A.vc + ((size_t)page * A.Hkv + kvh) * M::BYTES;
-    const int end = ctx - 1 - p * PAGE;
+    const int end = min(ctx - 1 - p * PAGE, PAGE - 1);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -431,49 +496,62 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_decode_mx_kernel(const Decode
       }
   };
   auto compute = [&](int p, R& x) {
-    f32x4 st[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      st[t] = score_mfma<DH, FP8>(x.k[t], qhi, f32x4{0.f, 0.f, 0.f, 0.f}, x.ks, shi, t);
-      if (DH == 128) st[t] = score_mfma<DH, FP8>(x.k[t], qlo, st[t], x.ks, slo, t);
-    }
-    if (ctx - p * PAGE < PAGE) {  // (the last page)
-      const int left = ctx - p * PAGE - 8 * g;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) st[t][r] = 32 * (t >> 1) + 4 * (t & 1) + r < left ? st[t][r] : -INFINITY;
-      cut(x, left);
-    }
-    float mx = -INFINITY;
+    f32x4 st[NB][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[t][r]);
-    mx = xor_max<16>(mx);
-    mx = xor_max<32>(mx);
-    const float mn = fmaxf(m, mx * A.scale_log2);  // (the scale is positive)
-    const float alpha = __builtin_amdgcn_exp2f(m - mn);
-    m = mn;
-    if (__ballot(alpha != 1.f)) {  // a head's maximum moved
-      l *= alpha;
+      for (int nb = 0; nb < NB; ++nb) {
+        st[nb][t] = score_mfma<DH, FP8>(x.k[t], qhi[nb], f32x4{0.f, 0.f, 0.f, 0.f}, x.ks, shi[nb], t);
+        if (DH == 128) st[nb][t] = score_mfma<DH, FP8>(x.k[t], qlo[nb], st[nb][t], x.ks, slo[nb], t);
+      }
+    // keys that some row does not see: past the context (the last page), or past a new token
+    if ((PROMPT ? pos0 + row0 / G + 1 : ctx) - p * PAGE < PAGE) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        o[j][0] *= alpha;
-        o[j][1] *= alpha;
+      for (int nb = 0; nb < NB; ++nb) {
+        const int left = (PROMPT ? sees[nb] + 1 : ctx) - p * PAGE - 8 * g;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) st[nb][t][r] = 32 * (t >> 1) + 4 * (t & 1) + r < left ? st[nb][t][r] : -INFINITY;
+      }
+      cut(x, ctx - p * PAGE - 8 * g);
+    }
+    s16x8 pf[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[nb][t][r]);
+      mx = xor_max<16>(mx);
+      mx = xor_max<32>(mx);
+      const float mn = fmaxf(m[nb], mx * A.scale_log2);  // (the scale is positive)
+      const float alpha = __builtin_amdgcn_exp2f(m[nb] - mn);
+      m[nb] = mn;
+      if (__ballot(alpha != 1.f)) {  // a row's maximum moved
+        l[nb] *= alpha;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          o[nb][j][0] *= alpha;
+          o[nb][j][1] *= alpha;
+        }
+      }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        u32x4 pw;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(st[nb][2 * kk + (e >> 2)][e & 3], A.scale_log2, -mn));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(st[nb][2 * kk + (e >> 2)][(e & 3) + 1], A.scale_log2, -mn));
+          l[nb] += p0 + p1;
+          pw[e >> 1] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p0, p1}), bf16x2_t));
+        }
+        pf[nb][kk] = __builtin_bit_cast(s16x8, pw);
       }
     }
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      u32x4 pw;
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(st[2 * kk + (e >> 2)][e & 3], A.scale_log2, -mn));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(st[2 * kk + (e >> 2)][(e & 3) + 1], A.scale_log2, -mn));
-        l += p0 + p1;
-        pw[e >> 1] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p0, p1}), bf16x2_t));
-      }
-      const s16x8 pf = __builtin_bit_cast(s16x8, pw);
+    for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         u32x4 ae, ao;
@@ -490,13 +568,17 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_decode_mx_kernel(const Decode
           ae[n] = low_halves(y[0], y[1]);
           ao[n] = high_halves(y[0], y[1]);
         }
-        o[j][0] = mfma16(__builtin_bit_cast(s16x8, ae), pf, o[j][0]);
-        o[j][1] = mfma16(__builtin_bit_cast(s16x8, ao), pf, o[j][1]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          o[nb][j][0] = mfma16(__builtin_bit_cast(s16x8, ae), pf[nb][kk], o[nb][j][0]);
+          o[nb][j][1] = mfma16(__builtin_bit_cast(s16x8, ao), pf[nb][kk], o[nb][j][1]);
+        }
       }
-    }
   };
 
-  {
+  // (two blocks of rows and mxfp8 pages of 128 dims: two register sets of a page would spill)
+  constexpr bool AHEAD = !(FP8 && DH == 128 && NB > 1);
+  if constexpr (AHEAD) {
     R xa, xb;
     int p = first + wave;
     if (p < last) load(p, page_of(p), xa);
@@ -516,70 +598,90 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_decode_mx_kernel(const Decode
       compute(p, xb);
       p += NW;
     }
+  } else {
+    R x;
+    long nxt = last > first ? page_of(first + wave) : 0;
+    for (int p = first + wave; p < last; p += NW) {
+      load(p, nxt, x);
+      nxt = page_of(p + NW);
+      compute(p, x);
+    }
   }
 
-  l = xor_sum<16>(l);
-  l = xor_sum<32>(l);
-  const size_t row0 = ((size_t)b * A.nparts * A.Hkv + kvh) * G, step = (size_t)A.Hkv * G;  // partial results: part 0's first head, from part to part
-  auto leave = [&](int hq, int d, const f32x4& O, float mm, float L) {
-    if (parts == 1) {
-      if (ctx > 0) st_results(A.out + ((size_t)b * A.H + kvh * G + hq) * DH + d, O, L);
-      else *reinterpret_cast<s16x4*>(A.out + ((size_t)b * A.H + kvh * G + hq) * DH + d) = s16x4{0, 0, 0, 0};
-      return;
-    }
-    const size_t row = row0 + part * step + hq;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    l[nb] = xor_sum<16>(l[nb]);
+    l[nb] = xor_sum<32>(l[nb]);
+  }
+  const size_t row_ws = ((size_t)bu * A.nparts * A.Hkv + kvh) * RS, step = (size_t)A.Hkv * RS;  // partial results: part 0's first row, from part to part
+  auto result = [&](int rw, int d, const f32x4& O, float L) {
+    const int row = row0 + rw, ti = PROMPT ? row / G : 0, hq = row - ti * G;
+    uint16_t* p = A.out + ((size_t)(q0 + ti) * A.H + kvh * G + hq) * DH + d;
+    if (pos0 + ti >= 0) st_results(p, O, L);
+    else *reinterpret_cast<s16x4*>(p) = s16x4{0, 0, 0, 0};  // a row without keys
+  };
+  auto leave = [&](int rw, int d, const f32x4& O, float mm, float L) {
+    if (parts == 1) return result(rw, d, O, L);
+    const size_t row = row_ws + part * step + rw;
     agent_store4(A.ws_o + row * DH + d, O);
     if (d == 0) agent_store2(A.ws_ml + row * 2, mm, L);
   };
   if constexpr (NW == 1) {
-    if (c < G)
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        leave(c, 32 * j + 8 * g, f32x4{o[j][0][0], o[j][1][0], o[j][0][1], o[j][1][1]}, m, l);
-        leave(c, 32 * j + 8 * g + 4, f32x4{o[j][0][2], o[j][1][2], o[j][0][3], o[j][1][3]}, m, l);
-      }
-  } else {  // the waves meet in LDS: [NW][G][LD] sums, [NW][G][2] maxima and sums of weights
-    float* ml = sm + NW * G * LD;
-    if (c < G) {
-      float* so = sm + (wave * G + c) * LD + 8 * g;
+    for (int nb = 0; nb < NB; ++nb)
+      if (16 * nb + c < RN)
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        *reinterpret_cast<f32x4*>(so + 32 * j) = f32x4{o[j][0][0], o[j][1][0], o[j][0][1], o[j][1][1]};
-        *reinterpret_cast<f32x4*>(so + 32 * j + 4) = f32x4{o[j][0][2], o[j][1][2], o[j][0][3], o[j][1][3]};
+        for (int j = 0; j < J; ++j) {
+          const f32x4 &e = o[nb][j][0], &d = o[nb][j][1];
+          leave(16 * nb + c, 32 * j + 8 * g, f32x4{e[0], d[0], e[1], d[1]}, m[nb], l[nb]);
+          leave(16 * nb + c, 32 * j + 8 * g + 4, f32x4{e[2], d[2], e[3], d[3]}, m[nb], l[nb]);
+        }
+  } else {  // the waves meet in LDS: [NW][RS][LD] sums, [NW][RS][2] maxima and sums of weights
+    float* ml = sm + NW * RS * LD;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+      if (16 * nb + c < RN) {
+        const int at = wave * RS + 16 * nb + c;
+        float* so = sm + at * LD + 8 * g;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const f32x4 &e = o[nb][j][0], &d = o[nb][j][1];
+          *reinterpret_cast<f32x4*>(so + 32 * j) = f32x4{e[0], d[0], e[1], d[1]};
+          *reinterpret_cast<f32x4*>(so + 32 * j + 4) = f32x4{e[2], d[2], e[3], d[3]};
+        }
+        if (g == 0) {
+          ml[at * 2] = m[nb];
+          ml[at * 2 + 1] = l[nb];
+        }
       }
-      if (g == 0) {
-        ml[(wave * G + c) * 2] = m;
-        ml[(wave * G + c) * 2 + 1] = l;
-      }
-    }
     __syncthreads();
-    for (int e = 4 * threadIdx.x; e < G * DH; e += 4 * NW * 64) {
-      const int hq = e / DH, d = e - hq * DH;
+    for (int e = 4 * threadIdx.x; e < RN * DH; e += 4 * NW * 64) {
+      const int rw = e / DH, d = e - rw * DH;
       float mm = NEG_BIG;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) mm = fmaxf(mm, ml[(w * G + hq) * 2]);
+      for (int w = 0; w < NW; ++w) mm = fmaxf(mm, ml[(w * RS + rw) * 2]);
       float L = 0.f;
       f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < NW; ++w) {  // (a wave without pages: m = NEG_BIG, l = 0, o = 0)
-        const float f = __builtin_amdgcn_exp2f(ml[(w * G + hq) * 2] - mm);
-        L += ml[(w * G + hq) * 2 + 1] * f;
-        O += *reinterpret_cast<const f32x4*>(sm + (w * G + hq) * LD + d) * f;
+        const float f = __builtin_amdgcn_exp2f(ml[(w * RS + rw) * 2] - mm);
+        L += ml[(w * RS + rw) * 2 + 1] * f;
+        O += *reinterpret_cast<const f32x4*>(sm + (w * RS + rw) * LD + d) * f;
       }
-      leave(hq, d, O, mm, L);
+      leave(rw, d, O, mm, L);
     }
   }
   if (parts == 1) return;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the partial results have left
   __syncthreads();
   __shared__ int last_sm;
-  int* t = A.tickets + b * A.Hkv + kvh;
+  int* t = A.tickets + bu * A.Hkv + kvh;
   if (threadIdx.x == 0) last_sm = __hip_atomic_fetch_add(t, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
   __syncthreads();
   if (!last_sm) return;
   if (threadIdx.x == 0) __hip_atomic_store(t, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  for (int e = 4 * threadIdx.x; e < G * DH; e += 4 * NW * 64) {
-    const int hq = e / DH, d = e - hq * DH;
+  for (int e = 4 * threadIdx.x; e < RN * DH; e += 4 * NW * 64) {
+    const int rw = e / DH, d = e - rw * DH;
     float mm = NEG_BIG, L = 0.f;
     f32x4 O = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < parts; s0 += 8) {
@@ -587,7 +689,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_decode_mx_kernel(const Decode
       f32x4 po[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const size_t row = row0 + min(s0 + i, parts - 1) * step + hq;
+        const size_t row = row_ws + min(s0 + i, parts - 1) * step + rw;
         ml[i] = agent_load2(A.ws_ml + row * 2);
         po[i] = agent_load4(A.ws_o + row * DH + d);
       }
@@ -606,7 +708,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_decode_mx_kernel(const Decode
           O += po[i] * f;
         }
     }
-    st_results(A.out + ((size_t)b * A.H + kvh * G + hq) * DH + d, O, L);
+    result(rw, d, O, L);
   }
 }
 
@@ -666,18 +768,21 @@ void rope_kv_write_mx(const at::Tensor& qkv, const at::Tensor& pos, const at::Te
   XCHECK(pos.numel() == T && slots.numel() == T && q_out.numel() == T * H * Dh, op, ": pos, slots or q_out of another length");
   XCHECK(cos_sin.dim() == 2 && cos_sin.size(1) == Dh && cos_sin.size(0) >= 1, op, ": cos_sin must be [positions, Dh]");
   if (T == 0) return;
-  const int64_t rows = T * (H + 2 * Hkv), blocks = (rows + 15) / 16;
-  XCHECK(blocks < (int64_t(1) << 24), op, ": too many tokens for one launch");
+  XCHECK((reinterpret_cast<uintptr_t>(qkv.data_ptr()) | reinterpret_cast<uintptr_t>(q_out.data_ptr()) | reinterpret_cast<uintptr_t>(cos_sin.data_ptr())) % 16 == 0,
+         op, ": qkv, q_out and cos_sin must be aligned to 16 bytes");
+  XCHECK(T < (1 << 26) && H + 2 * Hkv < (1 << 20) && (T + 3) / 4 * (H + 2 * Hkv) < (int64_t(1) << 26), op, ": too many tokens for one launch");
+  const unsigned blocks = (unsigned)(((T + 3) / 4 * (H + 2 * Hkv) + 3) / 4);
 #define GO(DHV, F)                                                                                                                      \
-  rope_kv_write_mx_kernel<DHV, F><<<(unsigned)blocks, 256, 0, stream()>>>(                                                              \
-      bf(qkv), pos.data_ptr<int32_t>(), cos_sin.data_ptr<float>(), slots.data_ptr<int64_t>(), bf(q_out), k_cache.data_ptr<uint8_t>(),   \
-      v_cache.data_ptr<uint8_t>(), (long)rows, (int)H, (int)Hkv, (int)cos_sin.size(0), (long)k_cache.size(0) * PAGE)
+  rope_kv_write_mx_kernel<DHV, F><<<blocks, 256, 0, stream()>>>(bf(qkv), pos.data_ptr<int32_t>(), cos_sin.data_ptr<float>(),            \
+                                                                slots.data_ptr<int64_t>(), bf(q_out), k_cache.data_ptr<uint8_t>(),      \
+                                                                v_cache.data_ptr<uint8_t>(), (int)T, (int)H, (int)Hkv,                  \
+                                                                (int)cos_sin.size(0), (long)k_cache.size(0) * PAGE)
   MX_GO(fp8, Dh, GO);
 #undef GO
 }
 
 void kv_read_mx(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables, const at::Tensor& ctx_lens, at::Tensor& k_out,
-                at::Tensor& v_out, bool skip) {
+                at::Tensor& v_out, bool skip, const c10::optional<at::Tensor>& own) {
   const char* op = "kv_read_mx";
   XCHECK(k_cache.is_cuda(), op, ": k_cache must be on a GPU");
   const at::Device dev = k_cache.device();
@@ -695,56 +800,118 @@ void kv_read_mx(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::
          op, ": k_out must be [entries, Hkv, 64, Dh], v_out [entries, Hkv, Dh, 64]");
   XCHECK((reinterpret_cast<uintptr_t>(k_out.data_ptr()) | reinterpret_cast<uintptr_t>(v_out.data_ptr())) % 16 == 0, op,
          ": k_out and v_out must be aligned to 16 bytes");
+  if (own.has_value()) {
+    on_gpu(op, *own, at::kInt, "own", dev);
+    XCHECK(own->numel() == n, op, ": own must be of the entries' length");
+  }
   if (n == 0) return;
-  XCHECK(n * Hkv < (int64_t(1) << 24), op, ": too many pages for one launch");
+  XCHECK(n < (int64_t(1) << 24) && n * Hkv < (int64_t(1) << 24), op, ": too many pages for one launch");
 #define GO(DHV, F)                                                                                                                         \
   kv_read_mx_kernel<DHV, F><<<(unsigned)(n * Hkv), 256, 0, stream()>>>(                                                                    \
       k_cache.data_ptr<uint8_t>(), v_cache.data_ptr<uint8_t>(), tables.data_ptr<int32_t>(), (int)tables.size(1), ctx_lens.data_ptr<int32_t>(), \
-      bf(k_out), bf(v_out), (int)Hkv, (int)k_cache.size(0), skip)
+      bf(k_out), bf(v_out), (int)Hkv, (int)k_cache.size(0), skip, own.has_value() ? own->data_ptr<int32_t>() : nullptr)
   MX_GO(fp8, Dh, GO);
 #undef GO
 }
 
-void attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables,
-                    const at::Tensor& ctx_lens, at::Tensor& out, at::Tensor& ws_o, at::Tensor& ws_ml, at::Tensor& tickets,
-                    int64_t pages_per_part, int64_t nparts, int64_t waves, double scale) {
-  const char* op = "attn_decode_mx";
-  XCHECK(q.is_cuda() && q.dim() == 3, op, ": q must be [B, H, Dh] on a GPU");
+// what both forms of the attention check; cu_q: several tokens a sequence
+AttnArgs attn_args(const char* op, bool& fp8, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables,
+                   const at::Tensor& ctx_lens, const at::Tensor* cu_q, at::Tensor& out, const c10::optional<at::Tensor>& ws_o,
+                   const c10::optional<at::Tensor>& ws_ml, const c10::optional<at::Tensor>& tickets, int64_t blocks, int64_t block_rows,
+                   int64_t pages_per_part, int64_t nparts, double scale) {
   const at::Device dev = q.device();
-  const c10::DeviceGuard guard(dev);
   on_gpu(op, q, at::kBFloat16, "q", dev);
   on_gpu(op, out, at::kBFloat16, "out", dev);
   on_gpu(op, tables, at::kInt, "block_tables", dev);
   on_gpu(op, ctx_lens, at::kInt, "ctx_lens", dev);
-  on_gpu(op, ws_o, at::kFloat, "ws_o", dev);
-  on_gpu(op, ws_ml, at::kFloat, "ws_ml", dev);
-  on_gpu(op, tickets, at::kInt, "tickets", dev);
-  const int64_t B = q.size(0), H = q.size(1), Dh = q.size(2), Hkv = k_cache.dim() == 3 ? k_cache.size(1) : 0;
-  const bool fp8 = caches_ok(op, k_cache, v_cache, Dh, dev);
-  XCHECK(H % Hkv == 0 && H / Hkv <= 16 && H >= 1, op, ": ", H, " query heads on ", Hkv, " (at most 16 each)");
-  XCHECK(tables.dim() == 2 && tables.size(0) == B && ctx_lens.numel() == B, op, ": a row of block_tables and a length for each query");
-  XCHECK(tables.size(1) >= 1 && tables.size(1) < (1 << 24), op, ": block_tables of no or too many columns");
-  XCHECK(out.numel() == q.numel(), op, ": out must have q's shape");
+  const int64_t T = q.size(0), H = q.size(1), Dh = q.size(2), Hkv = k_cache.dim() == 3 ? k_cache.size(1) : 0;
+  const int64_t B = ctx_lens.numel();
+  fp8 = caches_ok(op, k_cache, v_cache, Dh, dev);
+  XCHECK(H >= 1 && H % Hkv == 0 && H / Hkv <= 16, op, ": ", H, " query heads on ", Hkv, " (at most 16 each)");
+  XCHECK(tables.dim() == 2 && tables.size(0) == B, op, ": a row of block_tables for each of ctx_lens");
+  XCHECK(B == 0 || (tables.size(1) >= 1 && tables.size(1) < (1 << 24)), op, ": block_tables of no or too many columns");
+  if (cu_q != nullptr) {
+    on_gpu(op, *cu_q, at::kInt, "cu_q", dev);
+    XCHECK(cu_q->numel() == B + 1, op, ": cu_q must have one entry more than ctx_lens");
+  } else {
+    XCHECK(T == B, op, ": a length for each query");
+  }
+  XCHECK(T < (int64_t(1) << 31) / std::max<int64_t>(H, 1), op, ": too many tokens");
+  XCHECK(out.sizes() == q.sizes(), op, ": out must have q's shape");
   XCHECK((reinterpret_cast<uintptr_t>(q.data_ptr()) | reinterpret_cast<uintptr_t>(out.data_ptr())) % 16 == 0, op, ": q and out must be aligned to 16 bytes");
-  XCHECK(pages_per_part >= 1 && pages_per_part <= (1 << 24) && nparts >= 1 && nparts <= tables.size(1), op, ": bad partitioning");
-  XCHECK(waves == 1 || waves == 2 || waves == 4, op, ": 1, 2 or 4 waves");
+  XCHECK(pages_per_part >= 1 && pages_per_part <= (1 << 24) && nparts >= 1 && blocks >= 1, op, ": bad partitioning");
   XCHECK(scale > 0 && std::isfinite(scale), op, ": the scale must be positive");
-  if (B == 0) return;
-  XCHECK(B * Hkv * nparts < (int64_t(1) << 24), op, ": too many parts for one launch");
-  if (nparts > 1)
-    XCHECK(tickets.numel() >= B * Hkv && ws_o.numel() >= B * nparts * H * Dh && ws_ml.numel() >= B * nparts * H * 2 &&
-               (reinterpret_cast<uintptr_t>(ws_o.data_ptr()) | reinterpret_cast<uintptr_t>(ws_ml.data_ptr())) % 16 == 0,
+  XCHECK(blocks < (1 << 24) && nparts < (1 << 24) && B * blocks < (int64_t(1) << 24) && B * blocks * nparts < (int64_t(1) << 24) &&
+             B * blocks * nparts * Hkv < (int64_t(1) << 24),
+         op, ": too many parts for one launch");
+  float *o = nullptr, *ml = nullptr;
+  int* tk = nullptr;
+  if (nparts > 1) {
+    XCHECK(ws_o.has_value() && ws_ml.has_value() && tickets.has_value(), op, ": parts need a workspace");
+    on_gpu(op, *ws_o, at::kFloat, "ws_o", dev);
+    on_gpu(op, *ws_ml, at::kFloat, "ws_ml", dev);
+    on_gpu(op, *tickets, at::kInt, "tickets", dev);
+    const int64_t rows = B * blocks * nparts * Hkv * block_rows;
+    XCHECK(tickets->numel() >= B * blocks * Hkv && ws_o->numel() >= rows * Dh && ws_ml->numel() >= rows * 2 &&
+               (reinterpret_cast<uintptr_t>(ws_o->data_ptr()) | reinterpret_cast<uintptr_t>(ws_ml->data_ptr())) % 16 == 0,
            op, ": workspace small");
-  const DecodeArgs a = {bf(q), k_cache.data_ptr<uint8_t>(), v_cache.data_ptr<uint8_t>(), tables.data_ptr<int32_t>(), ctx_lens.data_ptr<int32_t>(),
-                        bf(out), ws_o.data_ptr<float>(), ws_ml.data_ptr<float>(), tickets.data_ptr<int32_t>(), (int)tables.size(1), (int)H,
-                        (int)Hkv, (int)pages_per_part, (int)nparts, (int)k_cache.size(0), (float)scale * LOG2E};
+    o = ws_o->data_ptr<float>();
+    ml = ws_ml->data_ptr<float>();
+    tk = tickets->data_ptr<int32_t>();
+  }
+  return {bf(q), k_cache.data_ptr<uint8_t>(), v_cache.data_ptr<uint8_t>(), tables.data_ptr<int32_t>(), ctx_lens.data_ptr<int32_t>(),
+          cu_q == nullptr ? nullptr : cu_q->data_ptr<int32_t>(), bf(out), o, ml, tk, (int)T, (int)tables.size(1), (int)H, (int)Hkv, (int)pages_per_part,
+          (int)nparts, (int)k_cache.size(0), (int)blocks, (float)scale * LOG2E};
+}
+
+void attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables,
+                    const at::Tensor& ctx_lens, at::Tensor& out, const c10::optional<at::Tensor>& ws_o, const c10::optional<at::Tensor>& ws_ml,
+                    const c10::optional<at::Tensor>& tickets, int64_t pages_per_part, int64_t nparts, int64_t waves, double scale) {
+  const char* op = "attn_decode_mx";
+  XCHECK(q.is_cuda() && q.dim() == 3, op, ": q must be [B, H, Dh] on a GPU");
+  const c10::DeviceGuard guard(q.device());
+  bool fp8 = false;
+  const int64_t H = q.size(1), Dh = q.size(2), Hkv = k_cache.dim() == 3 ? k_cache.size(1) : 1;
+  const AttnArgs a = attn_args(op, fp8, q, k_cache, v_cache, tables, ctx_lens, nullptr, out, ws_o, ws_ml, tickets, 1, H / std::max<int64_t>(Hkv, 1),
+                               pages_per_part, nparts, scale);
+  XCHECK(waves == 1 || waves == 2 || waves == 4, op, ": 1, 2 or 4 waves");
+  if (q.size(0) == 0) return;
   const size_t lds = waves == 1 ? 0 : (size_t)waves * (H / Hkv) * (Dh + 6) * sizeof(float);  // at most 34 KB
-  const unsigned units = (unsigned)(B * nparts * Hkv);
-#define GO(DHV, F)                                                                                   \
-  do {                                                                                               \
-    if (waves == 1) attn_decode_mx_kernel<DHV, F, 1><<<units, 64, lds, stream()>>>(a);               \
-    else if (waves == 2) attn_decode_mx_kernel<DHV, F, 2><<<units, 128, lds, stream()>>>(a);         \
-    else attn_decode_mx_kernel<DHV, F, 4><<<units, 256, lds, stream()>>>(a);                         \
+  const unsigned units = (unsigned)(q.size(0) * nparts * Hkv);
+#define GO(DHV, F)                                                                                              \
+  do {                                                                                                          \
+    if (waves == 1) attn_mx_kernel<DHV, F, 1, 1, false><<<units, 64, lds, stream()>>>(a);                       \
+    else if (waves == 2) attn_mx_kernel<DHV, F, 2, 1, false><<<units, 128, lds, stream()>>>(a);                 \
+    else attn_mx_kernel<DHV, F, 4, 1, false><<<units, 256, lds, stream()>>>(a);                                 \
+  } while (0)
+  MX_GO(fp8, Dh, GO);
+#undef GO
+}
+
+constexpr int TURN_WAVES = 4, TURN_BLOCKS = 2;  // of 16 rows
+
+// new tokens against the pools themselves: blocks of 32 rows of (token, head), for prompts of few tokens behind long contexts
+void attn_turn_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables, const at::Tensor& cu_q,
+                  const at::Tensor& ctx_lens, at::Tensor& out, const c10::optional<at::Tensor>& ws_o, const c10::optional<at::Tensor>& ws_ml,
+                  const c10::optional<at::Tensor>& tickets, int64_t max_qlen, int64_t pages_per_part, int64_t nparts, double scale) {
+  const char* op = "attn_turn_mx";
+  XCHECK(q.is_cuda() && q.dim() == 3, op, ": q must be [T, H, Dh] on a GPU");
+  const c10::DeviceGuard guard(q.device());
+  bool fp8 = false;
+  const int64_t H = q.size(1), Dh = q.size(2), Hkv = k_cache.dim() == 3 ? k_cache.size(1) : 1, B = ctx_lens.numel();
+  XCHECK(max_qlen >= 0 && max_qlen < (1 << 24), op, ": max_qlen");
+  constexpr int64_t ROWS = 16 * TURN_BLOCKS;
+  const int64_t blocks = std::max<int64_t>(1, (max_qlen * (H / std::max<int64_t>(Hkv, 1)) + ROWS - 1) / ROWS);
+  const AttnArgs a = attn_args(op, fp8, q, k_cache, v_cache, tables, ctx_lens, &cu_q, out, ws_o, ws_ml, tickets, blocks, ROWS, pages_per_part, nparts, scale);
+  if (B == 0 || max_qlen == 0) return;
+  const size_t lds = (size_t)TURN_WAVES * ROWS * (Dh + 6) * sizeof(float);  // 67 KB at heads of 128
+  const unsigned units = (unsigned)(B * blocks * nparts * Hkv);
+#define GO(DHV, F)                                                                                                                         \
+  do {                                                                                                                                     \
+    auto* f = attn_mx_kernel<DHV, F, TURN_WAVES, TURN_BLOCKS, true>;                                                                       \
+    static const hipError_t set = hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);              \
+    XCHECK(set == hipSuccess, op, ": LDS");                                                                                                \
+    f<<<units, 64 * TURN_WAVES, lds, stream()>>>(a);                                                                                       \
   } while (0)
   MX_GO(fp8, Dh, GO);
 #undef GO
@@ -756,6 +923,7 @@ void bind_kv_mx(pybind11::module& m) {
   m.def("rope_kv_write_mx", &rope_kv_write_mx);
   m.def("kv_read_mx", &kv_read_mx);
   m.def("attn_decode_mx", &attn_decode_mx);
+  m.def("attn_turn_mx", &attn_turn_mx);
 }
 
 }  // namespace xot

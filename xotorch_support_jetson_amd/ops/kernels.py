@@ -388,7 +388,7 @@ def kv_read_mx(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch
   if not _gpu(k_cache):
     ref.kv_read_mx(k_cache, v_cache, block_tables, ctx_lens, k_out, v_out)
   else:
-    require().kv_read_mx(k_cache, v_cache, block_tables, ctx_lens, k_out, v_out, bool(skip))
+    require().kv_read_mx(k_cache, v_cache, block_tables, ctx_lens, k_out, v_out, bool(skip), None)
   return k_out, v_out
 
 
@@ -462,25 +462,53 @@ def attn_decode_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 
 # scratch of attn_prefill_mx's bf16 pages: at most this much, or one sequence's
 MX_READ_BYTES = 1 << 30
+MX_TURN_UNITS = 1536
+
+
+def mx_turn(B: int, T: int, max_qlen: int, G: int, Hkv: int) -> bool:
+  """Whether attn_prefill_mx reads the pools themselves, in units of 32 rows (token, head of a KV head) against all the keys: where they
+  are few, or the sequences' new tokens are (a turn of a chat, decode steps with a prompt among them), whose contexts would cost more to
+  read back than to attend to; not where a long prompt among many sequences would make most of the units empty.  us via bf16 pages /
+  from the pools, mxfp4, heads of 128: 4 sequences of 64 new tokens behind 1000, 32 heads on 8, 51 / 17 (behind 8000 287 / 65), of 256 58 / 41,
+  of 512 70 / 79 (2048 units); one of 512 behind 8000, 64 heads, 285 / 176; 12 of 128 and no more 22 / 29 (1536 units; behind 1000 61 / 56),
+  of 512 82 / 117."""
+  units = Hkv * -(-max_qlen * G // 32)
+  return B * units <= MX_TURN_UNITS or (T * G <= 256 * B and B * units <= 1 << 18)
 
 
 def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, cu_q: torch.Tensor,
                     ctx_lens: torch.Tensor, max_qlen: int, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
-  """attn_prefill over pools in 8 or 4 bits: the sequences' pages are read back into bf16 scratch (a group of sequences at a time), which
-  the prompt attention reads.  The products of a prompt outweigh that pass: 2 Dh bytes written a key and head against 4 Dh G flops for
-  each of its tokens."""
+  """attn_prefill over pools in 8 or 4 bits: q [T, H, Dh], the tokens cu_q[b] .. cu_q[b + 1] are the last of sequence b's ctx_lens[b] (at
+  most max_qlen of them), each attends to what lies before it and itself.  Few tokens read the pools themselves (mx_turn).  Others'
+  products outweigh a pass over the cache: the pages are read back into bf16 scratch, a group of sequences at a time, which the prompt
+  attention reads."""
   T, H, Dh = q.shape
   B, W = block_tables.shape
   Hkv = k_cache.shape[1]
   out = torch.empty_like(q) if out is None else out
-  per = max(1, min(B, MX_READ_BYTES // max(1, W * Hkv * PAGE * Dh * 4))) if q.is_cuda else max(1, B)
+  gpu = _gpu(q)
+  if gpu and B and H % Hkv == 0 and mx_turn(B, T, max_qlen, H // Hkv, Hkv):
+    units = B * Hkv * max(1, -(-max_qlen * (H // Hkv) // 32))
+    nparts = max(1, min(W // 16, 512 // max(1, units)))
+    ws = [None] * 3
+    if nparts > 1:
+      rows = units * nparts * 32
+      ws = [torch.empty(rows * Dh, dtype=torch.float32, device=q.device), torch.empty(rows * 2, dtype=torch.float32, device=q.device),
+            torch.zeros(units, dtype=torch.int32, device=q.device)]
+    require().attn_turn_mx(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, out, *ws, int(max_qlen), -(-W // nparts), nparts, float(scale))
+    return out
+  per = max(1, min(B, MX_READ_BYTES // max(1, W * Hkv * PAGE * Dh * 4))) if gpu else max(1, B)
   k = torch.empty(per * W, Hkv, PAGE, Dh, dtype=torch.bfloat16, device=q.device)
   v = torch.empty(per * W, Hkv, Dh, PAGE, dtype=torch.bfloat16, device=q.device)
-  own = torch.arange(per * W, dtype=torch.int32, device=q.device).view(per, W)
+  own = torch.empty(per, W, dtype=torch.int32, device=q.device) if gpu else torch.arange(per * W, dtype=torch.int32).view(per, W)
   for b in range(0, B, per):
     n = min(per, B - b)
-    kv_read_mx(k_cache, v_cache, block_tables[b:b + n], ctx_lens[b:b + n], Dh, k[:n * W], v[:n * W], skip=True)
-    attn_prefill(q, k, v, own[:n], cu_q[b:b + n + 1], ctx_lens[b:b + n], max_qlen, scale, out=out)
+    tables, ctx, cu = block_tables[b:b + n], ctx_lens[b:b + n], cu_q[b:b + n + 1]
+    if gpu:
+      require().kv_read_mx(k_cache, v_cache, tables, ctx, k[:n * W], v[:n * W], True, own[:n])
+    else:
+      ref.kv_read_mx(k_cache, v_cache, tables, ctx, k, v)
+    attn_prefill(q, k, v, own[:n], cu, ctx, max_qlen, scale, out=out)
   return out
 
 
