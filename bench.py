@@ -333,6 +333,8 @@ def main():
   ap.add_argument("--weight-dtype", default="bf16", choices=["bf16", "fp8"],
                   help="fp8: weight-only e4m3 projections (a separate, reduced-precision measurement; the headline "
                        "is bf16)")
+  ap.add_argument("--kv-dtype", default="bf16", choices=["bf16", "mxfp8", "mxfp4"],
+                  help="KV cache in 8 or 4 bits (a separate, reduced-precision measurement; the headline is bf16)")
   ap.add_argument("--mixers", default=None, metavar="SIZES",
                   help="instead of the headline: Tarepel-design layers beside a Llama-style stack at the named sizes "
                        f"(comma-separated, of {', '.join(MIXER_SIZES)}); one GPU")
@@ -358,6 +360,7 @@ def main():
                   help="--mixers / --hybrid / --latent / --memory / --chunked / --delta: sequences per step")
   args = ap.parse_args()
   os.environ["XOT_WEIGHT_DTYPE"] = args.weight_dtype
+  os.environ["XOT_KV_DTYPE"] = args.kv_dtype
   if args.mixers:
     return bench_mixers(args)
   if args.hybrid:
@@ -486,7 +489,8 @@ def main():
       "higher_is_better": True,
       "scaling": "weak",
       "vs_baseline": None,
-      "dtype": "bf16" if args.weight_dtype == "bf16" else "bf16 activations, fp8-e4m3 weights (NOT the headline)",
+      "dtype": ("bf16" if args.weight_dtype == "bf16" else "bf16 activations, fp8-e4m3 weights (NOT the headline)")
+               + ("" if args.kv_dtype == "bf16" else f", {args.kv_dtype} KV cache (NOT the headline)"),
       "data": f"synthetic prompts, random-init weights (exact {cfg_name(args.model)} architecture)",
       "config": {
         "model": args.model if not args.layers else f"{args.model}-TRUNCATED-{args.layers}L-INVALID",
@@ -499,6 +503,7 @@ def main():
         "decode_context": f"{args.prompt_len + args.warmup}..{args.prompt_len + args.warmup + args.steps}",
         "sampling": f"temperature {args.temperature}, top-k 35 (on-device)",
         "weight_dtype": args.weight_dtype,
+        "kv_dtype": args.kv_dtype,
       },
       "extra": {"prefill_s": round(t_prefill, 2), "init_s": round(t_init, 2),
                 "tokens_per_s_per_gpu": round(tps / world, 2),

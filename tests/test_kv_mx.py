@@ -252,6 +252,15 @@ def test_write_read_gpu(gpu, fmt, Dh, H, Hkv, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt,Dh,H,Hkv", [("mxfp4", 128, 21, 8), ("mxfp8", 64, 30, 4)])
+def test_write_many_heads_gpu(gpu, fmt, Dh, H, Hkv):
+  """Rows enough for several heads a wave, heads that are no whole groups of those (37, 38)."""
+  T = (1 << 17) // (H + 2 * Hkv) + 3
+  assert T * (H + 2 * Hkv) >= 1 << 17
+  check_write(fmt, Dh, H, Hkv, T, gpu)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FMTS)
 def test_write_format_gpu(gpu, fmt):
   """Ties, borders of the exponent, values that vanish, overflow and are not finite, written as values (no rotation)."""

@@ -104,20 +104,7 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 // by side in a page (keys 256 bytes, value units whole).  k is quantised from its rotation in fp32, v from its bf16; a group's largest
 // value is found among the lanes that hold it (on the bits: a NaN counts as larger than everything).  The rotation's products and sums are
 // rounded one by one, so that a value on the border between two elements falls the same way wherever it is computed.
-// Bound by its launch at a few tokens, by memory at many.
-template <int N>
-__device__ __forceinline__ void ld_bf16(const uint16_t* p, float (&x)[N]) {
-  static_assert(N == 2 || N == 4, "a dword or two");
-  if constexpr (N == 4) {
-    const uint64_t u = *reinterpret_cast<const uint64_t*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = bf2f((uint16_t)(u >> (16 * i)));
-  } else {
-    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
-    x[0] = bf2f((uint16_t)u);
-    x[1] = bf2f((uint16_t)(u >> 16));
-  }
-}
+// Bound by its launch at a few tokens (2.7 us up to 64), by memory at many: 4.8 to 5.3 TB/s at 8192 (a large copy: 4.9).
 // N values under one scale -> N bytes of e4m3 or N / 2 of e2m1
 template <bool FP8, int N>
 __device__ __forceinline__ uint32_t mx_elements(const float (&x)[N], int e, bool bad) {
@@ -135,86 +122,114 @@ __device__ __forceinline__ void st_bytes(uint8_t* p, uint64_t v) {
   else *p = (uint8_t)v;
 }
 
-template <int DH, bool FP8>
+template <int DH, bool FP8, int HB>
 __global__ __launch_bounds__(256) void rope_kv_write_mx_kernel(const uint16_t* __restrict__ qkv, const int32_t* __restrict__ pos,
                                                                const float* __restrict__ cos_sin, const int64_t* __restrict__ slots,
                                                                uint16_t* __restrict__ q_out, uint8_t* __restrict__ kc,
                                                                uint8_t* __restrict__ vc, int T, int H, int Hkv, int max_pos, long nslots) {
 #pragma clang fp contract(off)
   using M = Mx<DH, FP8>;
-  constexpr int E = DH / 32, HALF = DH / 2, KB = FP8 ? E : E / 2;  // dims a lane takes of each half; their bytes
-  const int N = H + 2 * Hkv, w = blockIdx.x * 4 + (threadIdx.x >> 6), quad = w / N, h = w - quad * N;
-  const int t = 4 * quad + ((threadIdx.x >> 4) & 3), r = threadIdx.x & 15;
-  if (t >= T) return;  // (sixteen lanes together, here and below)
-  const uint16_t* src = qkv + ((size_t)t * N + h) * DH;
-  long slot = -1;
-  if (h >= H) {
-    slot = slots[t];
-    if (slot < 0 || slot >= nslots) return;
+  constexpr int J = M::J, E = DH / 32, HALF = DH / 2, KB = FP8 ? E : E / 2;  // E: dims a lane takes of each half; KB: their bytes
+  const int N = H + 2 * Hkv, groups = (N + HB - 1) / HB, w = blockIdx.x * 4 + (threadIdx.x >> 6), quad = w / groups;
+  const int h0 = (w - quad * groups) * HB, t = 4 * quad + ((threadIdx.x >> 4) & 3), r = threadIdx.x & 15;
+  if (t >= T) return;  // (sixteen lanes together)
+  // a lane's share of a row is J dwords: E dims of each half to rotate, or two dims of each group of a value
+  uint32_t raw[HB][J];
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    const int h = min(h0 + i, N - 1);
+    const uint16_t* src = qkv + ((size_t)t * N + h) * DH;
+    if (h < H + Hkv) {
+      if constexpr (J == 4) {
+        const uint64_t a = *reinterpret_cast<const uint64_t*>(src + E * r), b = *reinterpret_cast<const uint64_t*>(src + HALF + E * r);
+        raw[i][0] = (uint32_t)a;
+        raw[i][1] = (uint32_t)(a >> 32);
+        raw[i][2] = (uint32_t)b;
+        raw[i][3] = (uint32_t)(b >> 32);
+      } else {
+        raw[i][0] = *reinterpret_cast<const uint32_t*>(src + E * r);
+        raw[i][1] = *reinterpret_cast<const uint32_t*>(src + HALF + E * r);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < J; ++j) raw[i][j] = *reinterpret_cast<const uint32_t*>(src + 32 * j + 2 * r);
+    }
   }
+  const int64_t slot = slots[t];
+  const bool kept = slot >= 0 && slot < nslots;
   const int off = (int)(slot & (PAGE - 1));
-  if (h < H + Hkv) {
+  float c[E], s[E];
+  if (h0 < H + Hkv) {
     int p = pos[t];
     p = p < 0 ? 0 : (p >= max_pos ? max_pos - 1 : p);
     const float* cs = cos_sin + (size_t)p * DH + E * r;
-    float x[E], y[E], lo[E], hi[E];
-    ld_bf16(src + E * r, x);
-    ld_bf16(src + HALF + E * r, y);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const float c = cs[i], s = cs[HALF + i];
-      lo[i] = x[i] * c - y[i] * s;
-      hi[i] = y[i] * c + x[i] * s;
+      c[i] = cs[i];
+      s[i] = cs[HALF + i];
     }
-    if (h < H) {
-      uint8_t* dst = reinterpret_cast<uint8_t*>(q_out + ((size_t)t * H + h) * DH + E * r);
-      uint64_t a = 0, b = 0;
+  }
+#pragma unroll
+  for (int n = 0; n < HB; ++n) {
+    const int h = h0 + n;
+    if (h >= N || (h >= H && !kept)) break;
+    auto at = [&](int i) { return bf2f((uint16_t)(raw[n][i >> 1] >> (16 * (i & 1)))); };
+    if (h < H + Hkv) {
+      float lo[E], hi[E];
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        a |= (uint64_t)f2bf(lo[i]) << (16 * i);
-        b |= (uint64_t)f2bf(hi[i]) << (16 * i);
+        const float x = at(i), y = at(E + i);
+        lo[i] = x * c[i] - y * s[i];
+        hi[i] = y * c[i] + x * s[i];
       }
-      st_bytes<2 * E>(dst, a);
-      st_bytes<2 * E>(dst + 2 * HALF, b);
-      return;
-    }
-    uint8_t* page = kc + ((size_t)(slot / PAGE) * Hkv + (h - H)) * M::BYTES;
-    uint32_t a = 0, b = 0;
+      if (h < H) {
+        uint8_t* dst = reinterpret_cast<uint8_t*>(q_out + ((size_t)t * H + h) * DH + E * r);
+        uint64_t a = 0, b = 0;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      a = max(a, __float_as_uint(lo[i]) & 0x7fffffffu);
-      b = max(b, __float_as_uint(hi[i]) & 0x7fffffffu);
+        for (int i = 0; i < E; ++i) {
+          a |= (uint64_t)f2bf(lo[i]) << (16 * i);
+          b |= (uint64_t)f2bf(hi[i]) << (16 * i);
+        }
+        st_bytes<2 * E>(dst, a);
+        st_bytes<2 * E>(dst + 2 * HALF, b);
+        continue;
+      }
+      uint8_t* page = kc + ((size_t)(slot / PAGE) * Hkv + (h - H)) * M::BYTES;
+      uint32_t a = 0, b = 0;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        a = max(a, __float_as_uint(lo[i]) & 0x7fffffffu);
+        b = max(b, __float_as_uint(hi[i]) & 0x7fffffffu);
+      }
+      a = lanes_max<32 / E>(a);
+      b = lanes_max<32 / E>(b);
+      const int ea = mx_exponent<DH, FP8>(a), eb = mx_exponent<DH, FP8>(b);
+      const bool na = mx_bad(a), nb = mx_bad(b);
+      uint8_t* dst = page + off * M::ROW + KB * r;
+      st_bytes<KB>(dst, mx_elements<FP8>(lo, ea, na));
+      st_bytes<KB>(dst + M::ROW / 2, mx_elements<FP8>(hi, eb, nb));
+      if (r % (32 / E) == 0) {
+        const int j = E * r / 32;
+        uint8_t* sc = page + M::ELEMS + mx_key_scale(off);
+        sc[64 * j] = (uint8_t)(na ? 255 : ea + 127);
+        sc[64 * (j + J / 2)] = (uint8_t)(nb ? 255 : eb + 127);
+      }
+      continue;
     }
-    a = lanes_max<32 / E>(a);
-    b = lanes_max<32 / E>(b);
-    const int ea = mx_exponent<DH, FP8>(a), eb = mx_exponent<DH, FP8>(b);
-    const bool na = mx_bad(a), nb = mx_bad(b);
-    uint8_t* dst = page + off * M::ROW + KB * r;
-    st_bytes<KB>(dst, mx_elements<FP8>(lo, ea, na));
-    st_bytes<KB>(dst + M::ROW / 2, mx_elements<FP8>(hi, eb, nb));
-    if (r % (32 / E) == 0) {
-      const int j = E * r / 32;
-      uint8_t* sc = page + M::ELEMS + mx_key_scale(off);
-      sc[64 * j] = (uint8_t)(na ? 255 : ea + 127);
-      sc[64 * (j + M::J / 2)] = (uint8_t)(nb ? 255 : eb + 127);
+    uint8_t* page = vc + ((size_t)(slot / PAGE) * Hkv + (h - H - Hkv)) * M::BYTES;
+    uint64_t y = 0;
+    uint32_t sc = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const float x[2] = {at(2 * j), at(2 * j + 1)};
+      const uint32_t a = lanes_max<16>(max(__float_as_uint(x[0]) & 0x7fffffffu, __float_as_uint(x[1]) & 0x7fffffffu));
+      const int e = mx_exponent<DH, FP8>(a);
+      y |= (uint64_t)mx_elements<FP8>(x, e, mx_bad(a)) << (FP8 ? 16 * j : 8 * j);
+      sc |= (uint32_t)(mx_bad(a) ? 255 : e + 127) << (8 * j);
     }
-    return;
+    st_bytes<M::NB>(page + mx_value_off<DH, FP8>(off, r), y);
+    if (r == 0) st_bytes<J>(page + M::ELEMS + off * J, sc);
   }
-  uint8_t* page = vc + ((size_t)(slot / PAGE) * Hkv + (h - H - Hkv)) * M::BYTES;
-  float x[M::J][2];
-#pragma unroll
-  for (int j = 0; j < M::J; ++j) ld_bf16(src + 32 * j + 2 * r, x[j]);
-  uint64_t y = 0;
-  uint32_t sc = 0;
-#pragma unroll
-  for (int j = 0; j < M::J; ++j) {
-    const uint32_t a = lanes_max<16>(max(__float_as_uint(x[j][0]) & 0x7fffffffu, __float_as_uint(x[j][1]) & 0x7fffffffu));
-    const int e = mx_exponent<DH, FP8>(a);
-    y |= (uint64_t)mx_elements<FP8>(x[j], e, mx_bad(a)) << (FP8 ? 16 * j : 8 * j);
-    sc |= (uint32_t)(mx_bad(a) ? 255 : e + 127) << (8 * j);
-  }
-  st_bytes<M::NB>(page + mx_value_off<DH, FP8>(off, r), y);
-  if (r == 0) st_bytes<M::J>(page + M::ELEMS + off * M::J, sc);
 }
 
 // ============================================================================ read
@@ -749,6 +764,11 @@ bool caches_ok(const char* op, const at::Tensor& k, const at::Tensor& v, int64_t
     }                                       \
   } while (0)
 
+// heads of a wave: four share its angles (which are as many bytes as its rows) where there are rows enough to fill the chip with fewer
+// waves.  us at 1 / 4, mxfp4, heads of 128: 8192 tokens of 64 + 16 heads 69.7 / 58.9 (5.3 TB/s), of 32 + 16 43.2 / 36.8, 2048 of 64 + 16
+// 16.2 / 15.0, of 32 + 16 10.9 / 11.2, 512 4.3 / 5.3, 1 2.7 / 4.0
+constexpr int WRITE_HEADS = 4, WRITE_HEADS_ROWS = 1 << 17;
+
 void rope_kv_write_mx(const at::Tensor& qkv, const at::Tensor& pos, const at::Tensor& cos_sin, const at::Tensor& slots, at::Tensor& q_out,
                       at::Tensor& k_cache, at::Tensor& v_cache, int64_t H, int64_t Hkv) {
   const char* op = "rope_kv_write_mx";
@@ -771,14 +791,21 @@ void rope_kv_write_mx(const at::Tensor& qkv, const at::Tensor& pos, const at::Te
   XCHECK((reinterpret_cast<uintptr_t>(qkv.data_ptr()) | reinterpret_cast<uintptr_t>(q_out.data_ptr()) | reinterpret_cast<uintptr_t>(cos_sin.data_ptr())) % 16 == 0,
          op, ": qkv, q_out and cos_sin must be aligned to 16 bytes");
   XCHECK(T < (1 << 26) && H + 2 * Hkv < (1 << 20) && (T + 3) / 4 * (H + 2 * Hkv) < (int64_t(1) << 26), op, ": too many tokens for one launch");
-  const unsigned blocks = (unsigned)(((T + 3) / 4 * (H + 2 * Hkv) + 3) / 4);
-#define GO(DHV, F)                                                                                                                      \
-  rope_kv_write_mx_kernel<DHV, F><<<blocks, 256, 0, stream()>>>(bf(qkv), pos.data_ptr<int32_t>(), cos_sin.data_ptr<float>(),            \
-                                                                slots.data_ptr<int64_t>(), bf(q_out), k_cache.data_ptr<uint8_t>(),      \
-                                                                v_cache.data_ptr<uint8_t>(), (int)T, (int)H, (int)Hkv,                  \
-                                                                (int)cos_sin.size(0), (long)k_cache.size(0) * PAGE)
+  const int64_t hb = T * (H + 2 * Hkv) >= WRITE_HEADS_ROWS ? WRITE_HEADS : 1;
+  const unsigned blocks = (unsigned)(((T + 3) / 4 * ((H + 2 * Hkv + hb - 1) / hb) + 3) / 4);
+#define GO_HB(DHV, F, HB)                                                                                                               \
+  rope_kv_write_mx_kernel<DHV, F, HB><<<blocks, 256, 0, stream()>>>(bf(qkv), pos.data_ptr<int32_t>(), cos_sin.data_ptr<float>(),        \
+                                                                    slots.data_ptr<int64_t>(), bf(q_out), k_cache.data_ptr<uint8_t>(),  \
+                                                                    v_cache.data_ptr<uint8_t>(), (int)T, (int)H, (int)Hkv,              \
+                                                                    (int)cos_sin.size(0), (long)k_cache.size(0) * PAGE)
+#define GO(DHV, F)                           \
+  do {                                       \
+    if (hb > 1) GO_HB(DHV, F, WRITE_HEADS);  \
+    else GO_HB(DHV, F, 1);                   \
+  } while (0)
   MX_GO(fp8, Dh, GO);
 #undef GO
+#undef GO_HB
 }
 
 void kv_read_mx(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables, const at::Tensor& ctx_lens, at::Tensor& k_out,

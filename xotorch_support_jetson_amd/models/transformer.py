@@ -100,11 +100,18 @@ class StepInputs:
 class KVCache:
   """Per-shard paged KV pool: K [L, pages, Hkv, 64, Dh] and V [L, pages, Hkv, Dh, 64] (V storage: each page chunk-major,
   [8 chunks][Dh][8 keys], ops/reference.py v_chunks).
-  MLA models (DeepSeek) keep one latent row per token instead: k = C [L, pages, 64, kv_lora + rope], v None."""
+  MLA models (DeepSeek) keep one latent row per token instead: k = C [L, pages, 64, kv_lora + rope], v None.
+  kv_dtype mxfp8 / mxfp4 (attention heads of 64 or 128): both [L, pages, Hkv, bytes of a page] uint8 (csrc/kv_mx.hip)."""
 
-  def __init__(self, c: ModelConfig, n_layers: int, num_pages: int, device, dtype=torch.bfloat16, layer_ids=None):
+  def __init__(self, c: ModelConfig, n_layers: int, num_pages: int, device, dtype=torch.bfloat16, layer_ids=None, kv_dtype: str = "bf16"):
     self.num_pages = num_pages
     self.device = torch.device(device)
+    self.kv_dtype = kv_dtype
+    if kv_dtype != "bf16":
+      self.check_mx(c, kv_dtype)
+      self.k, self.v = (torch.zeros(n_layers, num_pages, c.num_kv_heads, K.mx_page_bytes(kv_dtype, c.head_dim), device=device,
+                                    dtype=torch.uint8) for _ in range(2))
+      return
     if c.is_mixed:
       # one K [pages, G, 64, d] and one V [pages, G, d, 64] pool per layer that has an attention mixer (None for the others):
       # layers may differ in heads and sizes; the value pool holds whatever the layer's mixer stores as values
@@ -152,7 +159,19 @@ class KVCache:
     self.v = torch.zeros(n_layers, num_pages, c.num_kv_heads, c.head_dim, PAGE, device=device, dtype=dtype)
 
   @staticmethod
-  def bytes_per_page(c: ModelConfig, n_layers: int, layer_ids=None, itemsize: int = 2) -> int:
+  def check_mx(c: ModelConfig, kv_dtype: str) -> None:
+    """Refuses a cache in 8 or 4 bits for models whose attention does not read one."""
+    if kv_dtype not in K.MX_FORMATS:
+      raise ValueError(f"kv_dtype {kv_dtype!r}: bf16, {' or '.join(K.MX_FORMATS)}")
+    if c.is_mixed or c.is_mla or c.head_dim not in (64, 128) or c.num_heads > 16 * c.num_kv_heads:
+      raise ValueError(f"kv_dtype {kv_dtype}: {c.model_type} is not served from a cache in 8 or 4 bits (keys and values in heads of 64 or "
+                       "128, at most 16 query heads each)")
+
+  @staticmethod
+  def bytes_per_page(c: ModelConfig, n_layers: int, layer_ids=None, itemsize: int = 2, kv_dtype: str = "bf16") -> int:
+    if kv_dtype != "bf16":
+      KVCache.check_mx(c, kv_dtype)
+      return 2 * n_layers * c.num_kv_heads * K.mx_page_bytes(kv_dtype, c.head_dim)
     if c.is_mixed:
       ids = [i for i, _ in c.layer_runs(layer_ids if layer_ids is not None else range(n_layers))]
       n, seen = 0, set()
@@ -255,6 +274,8 @@ class ShardModel:
     if self.device.type == "cuda":
       if c.is_mla:
         self.ws = K.MLAWorkspace(max_batch, c.num_heads, c.kv_lora_rank, max_ctx, self.device)
+      elif kv.kv_dtype != "bf16":
+        self.ws = K.MXDecodeWorkspace(max_batch, c.num_heads, c.num_kv_heads, c.head_dim, max_ctx, self.device)
       else:
         self.ws = K.DecodeWorkspace(max_batch, c.num_heads, c.head_dim, max_ctx, self.device, routed=c.num_experts > 0)
     if c.is_mla:
@@ -277,6 +298,10 @@ class ShardModel:
   # ------------------------------------------------------------------ helpers
   def _attention(self, q: torch.Tensor, li: int, inp: StepInputs, ws=None, defer_merge: bool = False, plan=None):
     kc, vc = self.kv.k[li], self.kv.v[li]
+    if self.kv.kv_dtype != "bf16":
+      if inp.decode:
+        return K.attn_decode_mx(q, kc, vc, inp.block_tables, inp.ctx_lens, self.scale, ws or self.ws)
+      return K.attn_prefill_mx(q, kc, vc, inp.block_tables, inp.cu_q, inp.ctx_lens, inp.max_qlen, self.scale)
     if inp.decode:
       return K.attn_decode(q, kc, vc, inp.block_tables, inp.ctx_lens, self.scale, ws or self.ws,
                            defer_merge=defer_merge, plan=plan)
@@ -1160,7 +1185,8 @@ class ShardModel:
     hb = (h, torch.empty_like(h)) if fuse else None
     other = (lambda t: hb[1] if t is hb[0] else hb[0]) if fuse else (lambda t: None)
     plan = None  # of the step's attention, for all layers
-    if inp.decode and n and self.ws is not None and not c.is_mla:
+    mx = self.kv.kv_dtype != "bf16"
+    if inp.decode and n and self.ws is not None and not c.is_mla and not mx:
       plan = self.ws.plan(inp.block_tables, inp.ctx_lens, c.num_kv_heads)
     for j, li in enumerate(self.layer_ids):
       lw = w.layers[li]
@@ -1168,8 +1194,12 @@ class ShardModel:
         a = self._mla(xn, lw, j, inp)
       else:
         # QKV projection + RoPE + paged KV write (split-K slabs reduced inside the RoPE kernel)
-        q = linear_rope_kv(xn, lw.qkv_w, lw.qkv_b, inp.positions, self.cos_sin, inp.slots, self.kv.k[j],
-                           self.kv.v[j], c.num_heads, c.num_kv_heads, wide=not c.num_experts)
+        if mx:  # (quantised as they are written: csrc/kv_mx.hip)
+          q = K.rope_kv_write_mx(linear(xn, lw.qkv_w, bias=lw.qkv_b), inp.positions, self.cos_sin, inp.slots, self.kv.k[j], self.kv.v[j],
+                                 c.num_heads, c.num_kv_heads)
+        else:
+          q = linear_rope_kv(xn, lw.qkv_w, lw.qkv_b, inp.positions, self.cos_sin, inp.slots, self.kv.k[j],
+                             self.kv.v[j], c.num_heads, c.num_kv_heads, wide=not c.num_experts)
         if isinstance(xn, PendingNorm):
           h = xn.dst
         a = self._attention(q, j, inp, defer_merge=fuse and FUSE_MERGE and merge_fits(lw.o_w), plan=plan)

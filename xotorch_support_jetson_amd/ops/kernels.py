@@ -7,6 +7,7 @@ raises (see `ops._ext.require`).
 """
 from __future__ import annotations
 
+import contextlib
 import os
 
 import torch
@@ -508,7 +509,8 @@ def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
       require().kv_read_mx(k_cache, v_cache, tables, ctx, k[:n * W], v[:n * W], True, own[:n])
     else:
       ref.kv_read_mx(k_cache, v_cache, tables, ctx, k, v)
-    attn_prefill(q, k, v, own[:n], cu, ctx, max_qlen, scale, out=out)
+    with torch.cuda.device(q.device) if gpu else contextlib.nullcontext():
+      attn_prefill(q, k, v, own[:n], cu, ctx, max_qlen, scale, out=out)
   return out
 
 

@@ -782,7 +782,7 @@ def default_max_batch(cfg, world: int, avg_ctx: int = 512) -> int:
   layers = -(-cfg.num_layers // world)
   total = torch.cuda.get_device_properties(torch.cuda.current_device()).total_memory
   weights = 2 * (sum(cfg.params_per_layer(i) for i in range(layers)) + 2 * cfg.vocab_size * cfg.hidden_size)
-  per_tok = KVCache.bytes_per_page(cfg, layers) / 64
+  per_tok = KVCache.bytes_per_page(cfg, layers, kv_dtype=os.environ.get("XOT_KV_DTYPE") or "bf16") / 64
   pool_tokens = max(0.0, (total - weights - (4 << 30)) * 0.85) / per_tok
   return int(min(512 * world, max(64, pool_tokens // avg_ctx)))
 

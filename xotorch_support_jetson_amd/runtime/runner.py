@@ -108,13 +108,18 @@ class ShardRunner:
   def __init__(self, config: ModelConfig, shard: Shard, device: torch.device | str = "cpu",
                weights: Optional[ShardWeights] = None, num_pages: Optional[int] = None, max_batch: int = 128,
                max_ctx: int = 4096, kv_mem_fraction: float = 0.85, seed: int = 0, use_graphs: Optional[bool] = None,
-               dtype: torch.dtype = torch.bfloat16):
-    """dtype: the compute dtype of mixed-layer models (bfloat16, or float32 for an all-fp32 run: fp32 weights, caches
+               dtype: torch.dtype = torch.bfloat16, kv_dtype: Optional[str] = None):
+    """kv_dtype: what the KV cache holds, bf16 (default), mxfp8 or mxfp4: 8.25 or 4.25 bits a value (XOT_KV_DTYPE where not given), for
+    models with keys and values in heads of 64 or 128.
+    dtype: the compute dtype of mixed-layer models (bfloat16, or float32 for an all-fp32 run: fp32 weights, caches
     and vendor SGEMMs); the other architectures serve in bfloat16 only."""
     self.config = config
     self.dtype = dtype
     if dtype != torch.bfloat16 and not config.is_mixed:
       raise ValueError(f"{config.model_type} serves in bfloat16 only")
+    self.kv_dtype = kv_dtype or os.environ.get("XOT_KV_DTYPE") or "bf16"
+    if self.kv_dtype != "bf16":
+      KVCache.check_mx(config, self.kv_dtype)
     self.shard = shard
     self.device = torch.device(device)
     if self.device.type == "cuda":
@@ -135,7 +140,7 @@ class ShardRunner:
       prepare_for_decode(self.weights, keep_rowmajor=keep, fp8=self.weight_dtype == "fp8")
     n_layers = shard.get_layer_count()
     per_page = KVCache.bytes_per_page(config, n_layers, shard.layers(), torch.empty(0, dtype=dtype).element_size()) \
-      if config.is_mixed else KVCache.bytes_per_page(config, n_layers)
+      if config.is_mixed else KVCache.bytes_per_page(config, n_layers, kv_dtype=self.kv_dtype)
     if num_pages is None:
       if self.device.type == "cuda":
         free, _ = torch.cuda.mem_get_info(self.device)
@@ -145,7 +150,7 @@ class ShardRunner:
         num_pages = max(64, (max_batch * max_ctx) // PAGE // 4)
       num_pages = min(num_pages, max_batch * (-(-max_ctx // PAGE)) + 16)
     self.kv = KVCache(config, n_layers, num_pages, self.device, dtype, shard.layers()) if config.is_mixed else \
-      KVCache(config, n_layers, num_pages, self.device)
+      KVCache(config, n_layers, num_pages, self.device, kv_dtype=self.kv_dtype)
     self.bm = _block_manager(num_pages)
     # recurrent layers: one state slot per live request (max_batch of them), cleared on admission
     self.sm = _slot_manager(max_batch) if config.has_state else None
