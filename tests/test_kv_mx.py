@@ -308,7 +308,7 @@ def test_decode_stale_bytes_gpu(gpu, fmt, Dh):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("waves", [1, 2, 4])
+@pytest.mark.parametrize("waves", [(1, False), (2, False), (4, False), (4, True)])
 @pytest.mark.parametrize("fmt,Dh,H,Hkv", [("mxfp4", 128, 8, 1), ("mxfp8", 128, 32, 2), ("mxfp4", 64, 3, 3), ("mxfp8", 64, 14, 2)])
 def test_decode_parts_gpu(gpu, fmt, Dh, H, Hkv, waves, monkeypatch):
   """Contexts in parts, shorter ones than others and some without any: merged in the launch, the same whoever comes last, tickets left at

@@ -373,15 +373,20 @@ __device__ __forceinline__ void st_results(uint16_t* p, const f32x4& O, float L)
 }
 
 // One unit: 16 NB rows (tokens of a sequence x query heads of a KV head; single tokens: its G heads) against a part of the pages.
-// NW waves share the part, wave w takes pages w, w + NW, ... with the next one's loads in flight under this one's math, and meet in
-// LDS.  A context of several parts (at most nparts, of ppp pages and more) is merged by the workgroup that arrives last (a ticket a (rows,
-// KV head), zero between launches), in the parts' order whoever it is.
+// NW waves share the part, wave w takes pages w, w + NW, ..., and meet in LDS.  REFILL: a page's registers are loaded anew as soon as
+// they are consumed, keys behind the scores, values behind their products, so that a page's loads fly under the other half's math; without
+// it a page is loaded and then computed, in fewer registers (mxfp4 124, four waves a SIMD; 153, three).  Many pairs have waves enough to
+// hide the loads (512 sequences of 525 tokens 56 / 60 us with REFILL, 128 of 30 to 8000 103 / 110), few have not (64 of 30 to 2000 21.0 /
+// 19.9, 8 on 32 KV heads 9.3 / 8.4); mxfp8 pages of 128 dims have no registers left for it.  Two sets of a page's registers, and three,
+// leave two waves a SIMD: 59, 59, 107, 107 us of the first two.
+// A context of several parts (at most nparts, of ppp pages and more) is merged by the workgroup that arrives last (a ticket a (rows, KV
+// head), zero between launches), in the parts' order whoever it is.
 // Bound by memory where the pairs of single tokens fill the chip: 512 sequences of 1500 tokens, 32 heads of 128 on 8, mxfp8 1.66 GB in 257
-// us (6.5 TB/s), mxfp4 856 MB in 138 us (6.2 TB/s); of 525 tokens, 64 heads, mxfp4 58 us (5.0 TB/s of what counts).  A page of mxfp4 is
-// about 330 vector operations a wave, 190 of them making bf16 values; K needs none.  Without loads ahead and parts: 87 us, and 8
-// sequences of 32000 tokens 239 us, now 49.
-template <int DH, bool FP8, int NW, int NB, bool PROMPT>
-__global__ __launch_bounds__(64 * NW, 2) void attn_mx_kernel(const AttnArgs A) {
+// us (6.5 TB/s), mxfp4 856 MB in 138 us (6.2 TB/s); of 525 tokens, 64 heads, mxfp4 56 us (5.2 TB/s of what counts).  A page of mxfp4 is
+// about 330 vector operations a wave, 190 of them making bf16 values; K needs none.  Uncut contexts and no loads ahead: 8 sequences of
+// 32000 tokens 239 us, now 48.
+template <int DH, bool FP8, int NW, int NB, bool PROMPT, bool REFILL>
+__global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : 3) void attn_mx_kernel(const AttnArgs A) {
   static_assert(PROMPT || NB == 1, "a single token's heads are one column block");
   using M = Mx<DH, FP8>;
   using R = PageRegs<DH, FP8>;
@@ -464,26 +469,33 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_mx_kernel(const AttnArgs A) {
   auto ld = [](const uint8_t* p) -> u32x4 { return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)); };
   // page p of the sequence, which lies at `page`.  Rows past the context read its last row again: no bytes that do not count
   // (512 contexts of 525 tokens end 13 tokens into a page)
-  auto load = [&](int p, long page, R& x) {
+  auto load_k = [&](int p, long page, R& x) {
     const uint8_t* kp = A.kc + ((size_t)page * A.Hkv + kvh) * M::BYTES;
-    const uint8_t* vp = A.vc + ((size_t)page * A.Hkv + kvh) * M::BYTES;
     const int end = min(ctx - 1 - p * PAGE, PAGE - 1);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int i = 0; i < R::KV; ++i)
         x.k[t][i] = ld(kp + (uint32_t)(min(32 * (t >> 1) + 4 * (t & 1) + krow, end) * M::ROW + 16 * (DH == 64 && !FP8 ? g & 1 : g)) + 64 * i);
+    x.ks = *reinterpret_cast<const uint32_t*>(kp + M::ELEMS + 64 * (g & (J - 1)) + 4 * c);
+  };
+  auto load_v = [&](int p, long page, R& x) {
+    const uint8_t* vp = A.vc + ((size_t)page * A.Hkv + kvh) * M::BYTES;
+    const int end = min(ctx - 1 - p * PAGE, PAGE - 1);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
       for (int u = 0; u < R::VU; ++u)
         x.v[kk][u] = ld(vp + (uint32_t)((min(32 * kk + 8 * g + u * M::KC, end) / M::KC) * 256 + 16 * c));
-    x.ks = *reinterpret_cast<const uint32_t*>(kp + M::ELEMS + 64 * (g & (J - 1)) + 4 * c);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
       for (int u = 0; u < R::VS; ++u) x.vs[kk][u] = ld(vp + M::ELEMS + (32 * kk + 8 * g) * J + 16 * u);
     }
+  };
+  auto load = [&](int p, long page, R& x) {
+    load_k(p, page, x);
+    load_v(p, page, x);
   };
   // What lies past the context may be anything, NaN too: it becomes zeros (their probabilities are 0, but 0 NaN is NaN).
   // left: keys of this lane group inside the context
@@ -510,8 +522,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_mx_kernel(const AttnArgs A) {
         else puts(key >> 1, other, 0x7f7f7f7fu & ~other);
       }
   };
-  auto compute = [&](int p, R& x) {
-    f32x4 st[NB][4];
+  auto scores = [&](const R& x, f32x4 (&st)[NB][4]) {
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -519,6 +530,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_mx_kernel(const AttnArgs A) {
         st[nb][t] = score_mfma<DH, FP8>(x.k[t], qhi[nb], f32x4{0.f, 0.f, 0.f, 0.f}, x.ks, shi[nb], t);
         if (DH == 128) st[nb][t] = score_mfma<DH, FP8>(x.k[t], qlo[nb], st[nb][t], x.ks, slo[nb], t);
       }
+  };
+  auto weigh = [&](int p, R& x, f32x4 (&st)[NB][4]) {
     // keys that some row does not see: past the context (the last page), or past a new token
     if ((PROMPT ? pos0 + row0 / G + 1 : ctx) - p * PAGE < PAGE) {
 #pragma unroll
@@ -591,35 +604,27 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_mx_kernel(const AttnArgs A) {
       }
   };
 
-  // (two blocks of rows and mxfp8 pages of 128 dims: two register sets of a page would spill)
-  constexpr bool AHEAD = !(FP8 && DH == 128 && NB > 1);
-  if constexpr (AHEAD) {
-    R xa, xb;
-    int p = first + wave;
-    if (p < last) load(p, page_of(p), xa);
-    long nxt = last > first ? page_of(p + NW) : 0;  // (scalar reads of the table, ahead of the loads that need them)
-    while (p < last) {
-      if (p + NW < last) {
-        load(p + NW, nxt, xb);
-        nxt = page_of(p + 2 * NW);
-      }
-      compute(p, xa);
-      p += NW;
-      if (p >= last) break;
-      if (p + NW < last) {
-        load(p + NW, nxt, xa);
-        nxt = page_of(p + 2 * NW);
-      }
-      compute(p, xb);
-      p += NW;
-    }
-  } else {
-    R x;
-    long nxt = last > first ? page_of(first + wave) : 0;
-    for (int p = first + wave; p < last; p += NW) {
+  R x;
+  long nxt = last > first ? page_of(first + wave) : 0;  // (scalar reads of the table, ahead of the loads that need them)
+  if (REFILL && first + wave < last) {
+    load(first + wave, nxt, x);
+    nxt = page_of(first + wave + NW);
+  }
+  for (int p = first + wave; p < last; p += NW) {
+    if constexpr (REFILL) {
+      const bool more = p + NW < last;
+      f32x4 st[NB][4];
+      scores(x, st);
+      if (more) load_k(p + NW, nxt, x);
+      weigh(p, x, st);
+      if (more) load_v(p + NW, nxt, x);
+      nxt = page_of(p + 2 * NW);
+    } else {
       load(p, nxt, x);
       nxt = page_of(p + NW);
-      compute(p, x);
+      f32x4 st[NB][4];
+      scores(x, st);
+      weigh(p, x, st);
     }
   }
 
@@ -893,7 +898,7 @@ AttnArgs attn_args(const char* op, bool& fp8, const at::Tensor& q, const at::Ten
 
 void attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables,
                     const at::Tensor& ctx_lens, at::Tensor& out, const c10::optional<at::Tensor>& ws_o, const c10::optional<at::Tensor>& ws_ml,
-                    const c10::optional<at::Tensor>& tickets, int64_t pages_per_part, int64_t nparts, int64_t waves, double scale) {
+                    const c10::optional<at::Tensor>& tickets, int64_t pages_per_part, int64_t nparts, int64_t waves, bool refill, double scale) {
   const char* op = "attn_decode_mx";
   XCHECK(q.is_cuda() && q.dim() == 3, op, ": q must be [B, H, Dh] on a GPU");
   const c10::DeviceGuard guard(q.device());
@@ -907,9 +912,10 @@ void attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Te
   const unsigned units = (unsigned)(q.size(0) * nparts * Hkv);
 #define GO(DHV, F)                                                                                              \
   do {                                                                                                          \
-    if (waves == 1) attn_mx_kernel<DHV, F, 1, 1, false><<<units, 64, lds, stream()>>>(a);                       \
-    else if (waves == 2) attn_mx_kernel<DHV, F, 2, 1, false><<<units, 128, lds, stream()>>>(a);                 \
-    else attn_mx_kernel<DHV, F, 4, 1, false><<<units, 256, lds, stream()>>>(a);                                 \
+    if (waves == 1) attn_mx_kernel<DHV, F, 1, 1, false, false><<<units, 64, lds, stream()>>>(a);                \
+    else if (waves == 2) attn_mx_kernel<DHV, F, 2, 1, false, false><<<units, 128, lds, stream()>>>(a);          \
+    else if (refill && !(F && DHV == 128)) attn_mx_kernel<DHV, F, 4, 1, false, !(F && DHV == 128)><<<units, 256, lds, stream()>>>(a); \
+    else attn_mx_kernel<DHV, F, 4, 1, false, false><<<units, 256, lds, stream()>>>(a);                          \
   } while (0)
   MX_GO(fp8, Dh, GO);
 #undef GO
@@ -935,7 +941,7 @@ void attn_turn_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tens
   const unsigned units = (unsigned)(B * blocks * nparts * Hkv);
 #define GO(DHV, F)                                                                                                                         \
   do {                                                                                                                                     \
-    auto* f = attn_mx_kernel<DHV, F, TURN_WAVES, TURN_BLOCKS, true>;                                                                       \
+    auto* f = attn_mx_kernel<DHV, F, TURN_WAVES, TURN_BLOCKS, true, !(F && DHV == 128)>;                                                                       \
     static const hipError_t set = hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);              \
     XCHECK(set == hipSuccess, op, ": LDS");                                                                                                \
     f<<<units, 64 * TURN_WAVES, lds, stream()>>>(a);                                                                                       \

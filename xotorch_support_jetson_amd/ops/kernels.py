@@ -405,6 +405,7 @@ class MXDecodeWorkspace:
     self.o = torch.empty(max(1, rows * H * Dh), dtype=torch.float32, device=device)
     self.ml = torch.empty(max(1, rows * H * 2), dtype=torch.float32, device=device)
     self.tickets = torch.zeros(max_batch * Hkv, dtype=torch.int32, device=device)
+    self.chosen = {}  # (batch, pages, fp8) -> pages of a part, parts, waves, refilling
 
   @staticmethod
   def parts(batch: int, Hkv: int, pages: int):
@@ -428,16 +429,23 @@ class MXDecodeWorkspace:
       ppp = -(-pages // most)
     return ppp, most
 
+  def choose(self, batch: int, pages: int, fp8: bool):
+    key = (batch, pages, fp8)
+    if key not in self.chosen:
+      self.chosen[key] = (*self.partition(batch, pages), *mx_decode_waves(batch * self.Hkv, pages, fp8))
+    return self.chosen[key]
 
-def mx_decode_waves(pairs: int, pages: int, fp8: bool) -> int:
-  """Waves of an attn_decode_mx workgroup.  Four share the pages of a (sequence, KV head) where there are few of those, or many pages; many
-  with few pages each leave some of four waves idle.  us with 1 / 2 / 4, heads of 128, even contexts | ragged: mxfp4 1024 pairs of 520
-  tokens 18.3 / 17.9 / 19.6 | 16.7 / 14.1 / 16.6, 2048 of 200 16.9 / 18.5 / 20.9 | 14.1 / 14.8 / 19.0, 4096 of 520 57 / 58 / 67 | 40 / 40 /
-  50, of 1000 96 / 97 / 99 | 66 / 63 / 72, 512 of 520 16.5 / 13.2 / 11.5; mxfp8 4096 of 520 103 / 98 / 104 | 66 / 60 / 70, of 1500 265 / 257
-  / 253 | 175 / 156 / 162; 1024 of 30 to 8000 129 in 2, 106 in 4; 2048 of 100 to 1500, heads of 64, 33 / 29 / 28."""
+
+def mx_decode_waves(pairs: int, pages: int, fp8: bool):
+  """(waves of an attn_decode_mx workgroup, whether they refill a page's registers as they go).  Four share the pages of a (sequence, KV
+  head) where there are few of those, or many pages; many with few pages each leave some of four waves idle.  us with 1 / 2 / 4, heads of
+  128, even contexts | ragged: mxfp4 1024 pairs of 520 tokens 18.3 / 17.9 / 19.6 | 16.7 / 14.1 / 16.6, 2048 of 200 16.9 / 18.5 / 20.9 | 14.1 /
+  14.8 / 19.0, 4096 of 520 56 / 60 / 61 | 40 / 40 / 50, of 1000 96 / 97 / 99 | 66 / 63 / 72, 512 of 520 16.5 / 13.2 / 11.5; mxfp8 4096 of 520
+  100 / 105 / 108 | 66 / 60 / 70, of 1500 265 / 257 / 253 | 175 / 156 / 162; 1024 of 30 to 8000 129 in 2, 106 in 4; 2048 of 100 to 1500, heads of
+  64, 34 / 28 / 28.  Refilling pays where the waves are few (csrc/kv_mx.hip)."""
   if pairs < 1024 or pages > 16:
-    return 4
-  return 1 if pairs >= 2048 and pages <= 12 and not fp8 else 2
+    return 4, pairs < 1024
+  return (1 if pairs >= 2048 and pages <= 12 and not fp8 else 2), False
 
 
 def attn_decode_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
@@ -451,13 +459,14 @@ def attn_decode_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
       return out
     return y
   B, H, Dh = q.shape
-  Hkv, width = k_cache.shape[1], block_tables.shape[1]
+  width = block_tables.shape[1]
   if ws is None:
-    ws = MXDecodeWorkspace(B, H, Hkv, Dh, width * PAGE, q.device)
+    ws = MXDecodeWorkspace(B, H, k_cache.shape[1], Dh, width * PAGE, q.device)
+  elif ws.Hkv != k_cache.shape[1]:
+    raise RuntimeError(f"decode workspace for {ws.Hkv} KV heads, not {k_cache.shape[1]}")
   out = torch.empty_like(q) if out is None else out
-  ppp, nparts = ws.partition(B, width)
-  waves = mx_decode_waves(B * Hkv, width, k_cache.shape[2] > PAGE * Dh)
-  require().attn_decode_mx(q, k_cache, v_cache, block_tables, ctx_lens, out, ws.o, ws.ml, ws.tickets, ppp, nparts, waves, float(scale))
+  ppp, nparts, waves, refill = ws.choose(B, width, k_cache.shape[2] > PAGE * Dh)
+  require().attn_decode_mx(q, k_cache, v_cache, block_tables, ctx_lens, out, ws.o, ws.ml, ws.tickets, ppp, nparts, waves, refill, float(scale))
   return out
 
 
