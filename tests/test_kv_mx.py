@@ -390,8 +390,9 @@ def test_prompt_gpu(gpu, fmt, Dh, H, Hkv, monkeypatch):
   ctx, new = [70, 5, 300, 128, 64, 1], [10, 5, 260, 1, 64, 1]
   s = Seqs(fmt, ctx, Hkv, Dh, dev=gpu, width=6)
   s.spoil()
-  for direct in (True, False):  # from the pools, and through bf16 pages
-    monkeypatch.setattr(K, "mx_turn", lambda *a: direct)
+  for waves in (4, 1, 0):  # from the pools, and through bf16 pages
+    monkeypatch.setattr(K, "mx_prompt_direct", lambda *a: waves > 0)
+    monkeypatch.setattr(K, "mx_prompt_waves", lambda *a: waves)
     whole, end = check_prompt(s, new, H, Dh ** -0.5)
     assert (whole[end:] == 7).all()
   for limit in (1, 2 * 6 * Hkv * PAGE * Dh * 4):  # a sequence, two sequences at a time
@@ -406,13 +407,15 @@ def test_turns_gpu(gpu, fmt, Dh, H, Hkv, monkeypatch):
   s = Seqs(fmt, [1500, 2200, 33, 64, 1, 700], Hkv, Dh, dev=gpu, width=36)
   s.spoil()
   new = [3, 17, 0, 5, 1, 16]
-  a, end = check_prompt(s, new, H, Dh ** -0.5)
-  assert (a[end:] == 7).all()
-  for _ in range(3):
-    assert torch.equal(a, check_prompt(s, new, H, Dh ** -0.5)[0])
+  for waves in (4, 1):
+    monkeypatch.setattr(K, "mx_prompt_waves", lambda *a: waves)
+    a, end = check_prompt(s, new, H, Dh ** -0.5)
+    assert (a[end:] == 7).all()
+    for _ in range(3):
+      assert torch.equal(a, check_prompt(s, new, H, Dh ** -0.5)[0])
   s = Seqs(fmt, [3, 0], Hkv, Dh, dev=gpu)  # (rows before the first key: zeros, as in attn_prefill)
   for direct in (True, False):
-    monkeypatch.setattr(K, "mx_turn", lambda *a: direct)
+    monkeypatch.setattr(K, "mx_prompt_direct", lambda *a: direct)
     q = torch.randn(7, H, Dh, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
     out = K.attn_prefill_mx(q.to(gpu), s.k, s.v, s.tables, torch.tensor([0, 5, 7], dtype=torch.int32, device=gpu), s.ctx, 5, Dh ** -0.5)
     close(out[2:5], *attend64(q[2:5], *s.kv[0], Dh ** -0.5, 0))

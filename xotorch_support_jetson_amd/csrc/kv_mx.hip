@@ -325,7 +325,8 @@ __global__ __launch_bounds__(256) void kv_read_mx_kernel(const uint8_t* __restri
 // & 1) + r, so that a lane's scores of tiles 2 kk and 2 kk + 1 are the eight keys 32 kk + 8 g .. that it holds in the B operand of
 // O^T = V^T . P^T: probabilities stay in their registers.
 // Values: two e2m1 / e4m3 of a key become two bf16 (exact, scaled on the way), and two keys' pairs change halves: tile (j, e) of O^T
-// has dims 32 j + 2 row + e.  P is rounded to bf16, the values' own type; sums, maxima and the output are fp32.
+// has dims 32 j + 2 row + e.  P is rounded to bf16, the values' own
+// type; sums, maxima and the output are fp32.
 template <int DH, bool FP8>
 struct PageRegs {
   using M = Mx<DH, FP8>;
@@ -364,59 +365,54 @@ struct AttnArgs {
   float scale_log2;
 };
 
-// Four results O / L in bf16.
-__device__ __forceinline__ void st_results(uint16_t* p, const f32x4& O, float L) {
+// Four results O / L in bf16 (inv = 1 / L: the product is within 2^-23 of the quotient, far below bf16's step).
+__device__ __forceinline__ void st_results(uint16_t* p, const f32x4& O, float inv) {
   s16x4 y;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) y[r] = (short)f2bf(O[r] / L);
+  for (int r = 0; r < 4; ++r) y[r] = (short)f2bf(O[r] * inv);
   *reinterpret_cast<s16x4*>(p) = y;
 }
 
-// One unit: 16 NB rows (tokens of a sequence x query heads of a KV head; single tokens: its G heads) against a part of the pages.
-// NW waves share the part, wave w takes pages w, w + NW, ..., and meet in LDS.  REFILL: a page's registers are loaded anew as soon as
-// they are consumed, keys behind the scores, values behind their products, so that a page's loads fly under the other half's math; without
-// it a page is loaded and then computed, in fewer registers (mxfp4 124, four waves a SIMD; 153, three).  Many pairs have waves enough to
-// hide the loads (512 sequences of 525 tokens 56 / 60 us with REFILL, 128 of 30 to 8000 103 / 110), few have not (64 of 30 to 2000 21.0 /
-// 19.9, 8 on 32 KV heads 9.3 / 8.4); mxfp8 pages of 128 dims have no registers left for it.  Two sets of a page's registers, and three,
-// leave two waves a SIMD: 59, 59, 107, 107 us of the first two.
-// A context of several parts (at most nparts, of ppp pages and more) is merged by the workgroup that arrives last (a ticket a (rows, KV
-// head), zero between launches), in the parts' order whoever it is.
-// Bound by memory where the pairs of single tokens fill the chip: 512 sequences of 1500 tokens, 32 heads of 128 on 8, mxfp8 1.66 GB in 257
-// us (6.5 TB/s), mxfp4 856 MB in 138 us (6.2 TB/s); of 525 tokens, 64 heads, mxfp4 56 us (5.2 TB/s of what counts).  A page of mxfp4 is
-// about 330 vector operations a wave, 190 of them making bf16 values; K needs none.  Uncut contexts and no loads ahead: 8 sequences of
-// 32000 tokens 239 us, now 48.
-template <int DH, bool FP8, int NW, int NB, bool PROMPT, bool REFILL>
-__global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : 3) void attn_mx_kernel(const AttnArgs A) {
-  static_assert(PROMPT || NB == 1, "a single token's heads are one column block");
+// What a lane's eight keys hold past the context may be anything, NaN too: it becomes zeros (their probabilities are 0, but 0 NaN is
+// NaN).  left: how many of the eight count
+template <int DH, bool FP8, class V, class S>
+__device__ __forceinline__ void cut_values(V& v, S& vs, int left) {  // u32x4 [VU], [VS]
+  using M = Mx<DH, FP8>;
+#pragma unroll
+  for (int key = 0; key < 8; ++key) {
+    const bool dead = key >= left;
+    const uint32_t other = key & 1 ? 0xffffu : 0xffff0000u;
+    if constexpr (M::NB >= 4) {
+#pragma unroll
+      for (int i = key * (M::NB / 4); i < (key + 1) * (M::NB / 4); ++i) v[i >> 2][i & 3] = dead ? 0u : v[i >> 2][i & 3];
+    } else {
+      v[key >> 3][(key >> 1) & 3] = dead ? v[key >> 3][(key >> 1) & 3] & other : v[key >> 3][(key >> 1) & 3];
+    }
+    if constexpr (M::J == 4) vs[key >> 2][key & 3] = dead ? 0x7f7f7f7fu : vs[key >> 2][key & 3];
+    else vs[0][key >> 1] = dead ? (vs[0][key >> 1] & other) | (0x7f7f7f7fu & ~other) : vs[0][key >> 1];
+  }
+}
+
+// A wave's 16 NB rows (queries) and what it has of them.  ONES: the weights are summed as products with ones, which costs registers and
+// saves vector operations.
+template <int DH, bool FP8, int NB, bool ONES>
+struct Rows {
   using M = Mx<DH, FP8>;
   using R = PageRegs<DH, FP8>;
-  constexpr int J = M::J, LD = DH + 4;
-  extern __shared__ __attribute__((aligned(16))) float sm[];
-  const int kvh = blockIdx.x % A.Hkv, bp = blockIdx.x / A.Hkv, part = bp % A.nparts, bu = bp / A.nparts;
-  const int b = PROMPT ? bu / A.blocks : bu, row0 = PROMPT ? (bu - b * A.blocks) * 16 * NB : 0;
-  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, G = A.H / A.Hkv;
-  const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int q0 = PROMPT ? min(max(A.cu_q[b], 0), A.T) : b, qlen = PROMPT ? min(max(A.cu_q[b + 1], q0), A.T) - q0 : 1, nrows = qlen * G;
-  if (PROMPT && row0 >= nrows) return;  // the whole workgroup, here and below
-  const int RN = PROMPT ? min(16 * NB, nrows - row0) : G, RS = PROMPT ? 16 * NB : G;  // rows, and from unit to unit
-  const int ctx = min(max(A.ctx_lens[b], 0), A.width * PAGE), pos0 = ctx - qlen;       // pos0: keys before the new tokens
-  const int seen = PROMPT ? max(0, pos0 + (row0 + RN - 1) / G + 1) : ctx;              // keys that the unit's last row sees
-  const int pages = (seen + PAGE - 1) / PAGE;
-  const int parts = max(1, min(A.nparts, (pages + A.ppp - 1) / A.ppp));
-  if (part >= parts) return;
-  const int share = pages / parts, rest = pages - share * parts;
-  const int first = part * share + min(part, rest), last = first + share + (part < rest ? 1 : 0);
-
-  // the queries in two parts
+  static constexpr int J = M::J;
   i32x8 qhi[NB], qlo[NB];
-  int shi[NB], slo[NB], sees[NB];  // sees: the last key of the lane's row
+  int shi[NB], slo[NB];
+  float m[NB], l[NB];
+  f32x4 o[NB][J][2], lacc[NB];
+
+  // row c of block nb: the query at qp (dims 16 g ..) in two parts; !ok: zeros
+  __device__ __forceinline__ void query(int nb, const uint16_t* qp, bool ok, int g) {
+    m[nb] = NEG_BIG;
+    l[nb] = 0.f;
+    lacc[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int row = row0 + 16 * nb + c, ti = PROMPT ? min(row, nrows - 1) / G : 0, hi_ = PROMPT ? min(row, nrows - 1) - ti * G : min(c, G - 1);
-    const bool ok = row < nrows;
-    sees[nb] = pos0 + ti;
+    for (int j = 0; j < J; ++j) o[nb][j][0] = o[nb][j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     qhi[nb] = qlo[nb] = i32x8{0, 0, 0, 0, 0, 0, 0, 0};
-    const uint16_t* qp = A.q + ((size_t)(q0 + ti) * A.H + kvh * G + hi_) * DH + 16 * g;
     s16x8 x[DH / 32];
     uint32_t a = 0;
 #pragma unroll
@@ -452,21 +448,168 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : 3) void attn_mx_
     if (DH == 64 && g >= 2) shi[nb] = slo[nb];
   }
 
-  float m[NB], l[NB];
-  f32x4 o[NB][J][2];
+  // kt(t, k): this lane's share of score tile t
+  template <class K>
+  __device__ __forceinline__ void scores(K kt, uint32_t ks, f32x4 (&st)[NB][4]) const {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      u32x4 k[R::KV];
+      kt(t, k);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        st[nb][t] = score_mfma<DH, FP8>(k, qhi[nb], f32x4{0.f, 0.f, 0.f, 0.f}, ks, shi[nb], t);
+        if (DH == 128) st[nb][t] = score_mfma<DH, FP8>(k, qlo[nb], st[nb][t], ks, slo[nb], t);
+      }
+    }
+  }
+  // scores of keys that block nb's row does not see; left: how many of the keys from the lane's first on it does
+  __device__ __forceinline__ static void mask(f32x4 (&st)[4], int left) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st[t][r] = 32 * (t >> 1) + 4 * (t & 1) + r < left ? st[t][r] : -INFINITY;
+  }
+  // The page's weights and their products with its values; vv(kk, v, vs): eight keys' units and scales.
+  template <class V>
+  __device__ __forceinline__ void weigh(V vv, const f32x4 (&st)[NB][4], float scale_log2) {
+    s16x8 pf[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[nb][t][r]);
+      mx = xor_max<16>(mx);
+      mx = xor_max<32>(mx);
+      const float mn = fmaxf(m[nb], mx * scale_log2);  // (the scale is positive)
+      const float alpha = __builtin_amdgcn_exp2f(m[nb] - mn);
+      m[nb] = mn;
+      if (__ballot(alpha != 1.f)) {  // a row's maximum moved
+        if constexpr (ONES) lacc[nb] *= alpha;
+        else l[nb] *= alpha;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          o[nb][j][0] *= alpha;
+          o[nb][j][1] *= alpha;
+        }
+      }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        u32x4 pw;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(st[nb][2 * kk + (e >> 2)][e & 3], scale_log2, -mn));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(st[nb][2 * kk + (e >> 2)][(e & 3) + 1], scale_log2, -mn));
+          if constexpr (!ONES) l[nb] += p0 + p1;
+          pw[e >> 1] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p0, p1}), bf16x2_t));
+        }
+        pf[nb][kk] = __builtin_bit_cast(s16x8, pw);
+        constexpr short ONE = 0x3f80;
+        if constexpr (ONES) lacc[nb] = mfma16(s16x8{ONE, ONE, ONE, ONE, ONE, ONE, ONE, ONE}, pf[nb][kk], lacc[nb]);
+      }
+    }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      u32x4 v[R::VU], vs[R::VS];
+      vv(kk, v, vs);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        u32x4 ae, ao;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          uint32_t y[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int key = 2 * n + i, at = key * M::NB + (FP8 ? 2 * j : j), sa = key * J + j;  // bytes among the eight keys'
+            const uint32_t w = v[at >> 4][(at >> 2) & 3];
+            const float s = scale_of(vs[sa >> 4][(sa >> 2) & 3], sa & 3);
+            y[i] = FP8 ? from_fp8(w, s, (at >> 1) & 1) : from_fp4(w, s, at & 3);
+          }
+          ae[n] = low_halves(y[0], y[1]);
+          ao[n] = high_halves(y[0], y[1]);
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          o[nb][j][0] = mfma16(__builtin_bit_cast(s16x8, ae), pf[nb][kk], o[nb][j][0]);
+          o[nb][j][1] = mfma16(__builtin_bit_cast(s16x8, ao), pf[nb][kk], o[nb][j][1]);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      if constexpr (ONES) {
+        l[nb] = lacc[nb][0];  // (every row of the product is the column's sum)
+      } else {
+        l[nb] = xor_sum<16>(l[nb]);
+        l[nb] = xor_sum<32>(l[nb]);
+      }
+    }
+  }
+  // four neighbouring dims of block nb's row c: 32 j + 8 g + 4 half ..
+  __device__ __forceinline__ f32x4 dims(int nb, int j, int half) const {
+    const f32x4 &e = o[nb][j][0], &d = o[nb][j][1];
+    return half ? f32x4{e[2], d[2], e[3], d[3]} : f32x4{e[0], d[0], e[1], d[1]};
+  }
+};
+
+// One unit: 16 NB rows (tokens of a sequence x query heads of a KV head; single tokens: its G heads) against a part of the pages.
+// NW waves share the part, wave w takes pages w, w + NW, ..., and meet in LDS.  REFILL: a page's registers are loaded anew as soon as
+// they are consumed, keys behind the scores, values behind their products, so that a page's loads fly under the other half's math; without
+// it a page is loaded and then computed, in fewer registers (mxfp4 124, four waves a SIMD; 153, three).  Many pairs have waves enough to
+// hide the loads (512 sequences of 525 tokens 56 / 60 us with REFILL, 128 of 30 to 8000 103 / 110), few have not (64 of 30 to 2000 21.0 /
+// 19.9, 8 on 32 KV heads 9.3 / 8.4); mxfp8 pages of 128 dims have no registers left for it.  Two sets of a page's registers, and three,
+// leave two waves a SIMD: 59, 59, 107, 107 us of the first two.
+// A context of several parts (at most nparts, of ppp pages and more) is merged by the workgroup that arrives last (a ticket a (rows, KV
+// head), zero between launches), in the parts' order whoever it is.
+// Bound by memory where the pairs of single tokens fill the chip: 512 sequences of 1500 tokens, 32 heads of 128 on 8, mxfp8 1.66 GB in 257
+// us (6.5 TB/s), mxfp4 856 MB in 138 us (6.2 TB/s); of 525 tokens, 64 heads, mxfp4 56 us (5.2 TB/s of what counts).  A page of mxfp4 is
+// about 330 vector operations a wave, 190 of them making bf16 values; K needs none.  Uncut contexts and no loads ahead: 8 sequences of
+// 32000 tokens 239 us, now 48.
+// Prompts are bound by the vector unit: a page of 32 rows is 64 matrix instructions (1100 cycles) and 400 vector operations (1600, and the
+// exponentials' 400 more).  4096 tokens of 32 heads of 128 on 8, mxfp4, in units of one wave: 158 us, 868 TFLOP/s (the bf16 kernel behind
+// kv_read_mx 164); mxfp8 195 (no refilling; 164).  Pages through LDS, shared by four waves of 32 rows each: 172, 178.  Units start with the
+// last rows, which see the most keys.
+template <int DH, bool FP8, int NW, int NB, bool PROMPT, bool REFILL>
+__global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : 3) void attn_mx_kernel(const AttnArgs A) {
+  static_assert(PROMPT || NB == 1, "a single token's heads are one column block");
+  using M = Mx<DH, FP8>;
+  using R = PageRegs<DH, FP8>;
+  constexpr int J = M::J, LD = DH + 4;
+  extern __shared__ __attribute__((aligned(16))) float sm[];
+  const int kvh = blockIdx.x % A.Hkv, bp = blockIdx.x / A.Hkv, part = bp % A.nparts, bu = bp / A.nparts;
+  const int b = PROMPT ? bu / A.blocks : bu, row0 = PROMPT ? (A.blocks - 1 - (bu - b * A.blocks)) * 16 * NB : 0;
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, G = A.H / A.Hkv;
+  const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int q0 = PROMPT ? min(max(A.cu_q[b], 0), A.T) : b, qlen = PROMPT ? min(max(A.cu_q[b + 1], q0), A.T) - q0 : 1, nrows = qlen * G;
+  if (PROMPT && row0 >= nrows) return;  // the whole workgroup, here and below
+  const int RN = PROMPT ? min(16 * NB, nrows - row0) : G, RS = PROMPT ? 16 * NB : G;  // rows, and from unit to unit
+  const int ctx = min(max(A.ctx_lens[b], 0), A.width * PAGE), pos0 = ctx - qlen;       // pos0: keys before the new tokens
+  const int seen = PROMPT ? max(0, pos0 + (row0 + RN - 1) / G + 1) : ctx;              // keys that the unit's last row sees
+  const int pages = (seen + PAGE - 1) / PAGE;
+  const int parts = max(1, min(A.nparts, (pages + A.ppp - 1) / A.ppp));
+  if (part >= parts) return;
+  const int share = pages / parts, rest = pages - share * parts;
+  const int first = part * share + min(part, rest), last = first + share + (part < rest ? 1 : 0);
+
+  Rows<DH, FP8, NB, PROMPT> rows;
+  int sees[NB];  // the last key of the lane's row
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    m[nb] = NEG_BIG;
-    l[nb] = 0.f;
-#pragma unroll
-    for (int j = 0; j < J; ++j) o[nb][j][0] = o[nb][j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int row = row0 + 16 * nb + c, ti = PROMPT ? min(row, nrows - 1) / G : 0, hq = PROMPT ? min(row, nrows - 1) - ti * G : min(c, G - 1);
+    sees[nb] = pos0 + ti;
+    rows.query(nb, A.q + ((size_t)(q0 + ti) * A.H + kvh * G + hq) * DH + 16 * g, row < nrows, g);
   }
+
   const int32_t* bt = A.tables + (size_t)b * A.width;
   const int krow = 8 * (c >> 2) + (c & 3);
-
   auto page_of = [&](int p) -> long { return min(max(bt[min(p, last - 1)], 0), A.num_pages - 1); };  // (last > first)
   // (read once a launch: non-temporal, as fast as plain loads for small caches and up to 11 % faster for large ones)
-  auto ld = [](const uint8_t* p) -> u32x4 { return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)); };
+  auto ld = [](const uint8_t* p) -> u32x4 {
+    return PROMPT ? *reinterpret_cast<const u32x4*>(p) : __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+  };
   // page p of the sequence, which lies at `page`.  Rows past the context read its last row again: no bytes that do not count
   // (512 contexts of 525 tokens end 13 tokens into a page)
   auto load_k = [&](int p, long page, R& x) {
@@ -483,195 +626,100 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : 3) void attn_mx_
     const uint8_t* vp = A.vc + ((size_t)page * A.Hkv + kvh) * M::BYTES;
     const int end = min(ctx - 1 - p * PAGE, PAGE - 1);
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+    for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
       for (int u = 0; u < R::VU; ++u)
         x.v[kk][u] = ld(vp + (uint32_t)((min(32 * kk + 8 * g + u * M::KC, end) / M::KC) * 256 + 16 * c));
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-#pragma unroll
       for (int u = 0; u < R::VS; ++u) x.vs[kk][u] = ld(vp + M::ELEMS + (32 * kk + 8 * g) * J + 16 * u);
     }
   };
-  auto load = [&](int p, long page, R& x) {
-    load_k(p, page, x);
-    load_v(p, page, x);
+  R x;
+  auto scores = [&](f32x4 (&st)[NB][4]) {
+    rows.scores([&](int t, u32x4 (&k)[R::KV]) {
+#pragma unroll
+      for (int i = 0; i < R::KV; ++i) k[i] = x.k[t][i];
+    }, x.ks, st);
   };
-  // What lies past the context may be anything, NaN too: it becomes zeros (their probabilities are 0, but 0 NaN is NaN).
-  // left: keys of this lane group inside the context
-  auto cut = [&](R& x, int left) {
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-      for (int key = 0; key < 8; ++key) {
-        const bool dead = 32 * kk + key >= left;
-        auto put = [&](u32x4 (&w)[R::VU], int i, uint32_t keep, uint32_t or_) {
-          w[i >> 2][i & 3] = dead ? (w[i >> 2][i & 3] & keep) | or_ : w[i >> 2][i & 3];
-        };
-        auto puts = [&](int i, uint32_t keep, uint32_t or_) {
-          x.vs[kk][i >> 2][i & 3] = dead ? (x.vs[kk][i >> 2][i & 3] & keep) | or_ : x.vs[kk][i >> 2][i & 3];
-        };
-        const uint32_t other = key & 1 ? 0xffffu : 0xffff0000u;
-        if constexpr (M::NB >= 4) {
-#pragma unroll
-          for (int i = 0; i < M::NB / 4; ++i) put(x.v[kk], key * (M::NB / 4) + i, 0u, 0u);
-        } else {
-          put(x.v[kk], key >> 1, other, 0u);
-        }
-        if constexpr (J == 4) puts(key, 0u, 0x7f7f7f7fu);
-        else puts(key >> 1, other, 0x7f7f7f7fu & ~other);
-      }
-  };
-  auto scores = [&](const R& x, f32x4 (&st)[NB][4]) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        st[nb][t] = score_mfma<DH, FP8>(x.k[t], qhi[nb], f32x4{0.f, 0.f, 0.f, 0.f}, x.ks, shi[nb], t);
-        if (DH == 128) st[nb][t] = score_mfma<DH, FP8>(x.k[t], qlo[nb], st[nb][t], x.ks, slo[nb], t);
-      }
-  };
-  auto weigh = [&](int p, R& x, f32x4 (&st)[NB][4]) {
+  auto weigh = [&](int p, f32x4 (&st)[NB][4]) {
+    const int left = ctx - p * PAGE - 8 * g;  // keys of the context from the lane's first on
     // keys that some row does not see: past the context (the last page), or past a new token
     if ((PROMPT ? pos0 + row0 / G + 1 : ctx) - p * PAGE < PAGE) {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int left = (PROMPT ? sees[nb] + 1 : ctx) - p * PAGE - 8 * g;
+      for (int nb = 0; nb < NB; ++nb) rows.mask(st[nb], (PROMPT ? sees[nb] + 1 : ctx) - p * PAGE - 8 * g);
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) st[nb][t][r] = 32 * (t >> 1) + 4 * (t & 1) + r < left ? st[nb][t][r] : -INFINITY;
-      }
-      cut(x, ctx - p * PAGE - 8 * g);
+      for (int kk = 0; kk < 2; ++kk) cut_values<DH, FP8>(x.v[kk], x.vs[kk], left - 32 * kk);
     }
-    s16x8 pf[NB][2];
+    rows.weigh([&](int kk, u32x4 (&v)[R::VU], u32x4 (&vs)[R::VS]) {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      float mx = -INFINITY;
+      for (int u = 0; u < R::VU; ++u) v[u] = x.v[kk][u];
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[nb][t][r]);
-      mx = xor_max<16>(mx);
-      mx = xor_max<32>(mx);
-      const float mn = fmaxf(m[nb], mx * A.scale_log2);  // (the scale is positive)
-      const float alpha = __builtin_amdgcn_exp2f(m[nb] - mn);
-      m[nb] = mn;
-      if (__ballot(alpha != 1.f)) {  // a row's maximum moved
-        l[nb] *= alpha;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          o[nb][j][0] *= alpha;
-          o[nb][j][1] *= alpha;
-        }
-      }
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        u32x4 pw;
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(st[nb][2 * kk + (e >> 2)][e & 3], A.scale_log2, -mn));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(st[nb][2 * kk + (e >> 2)][(e & 3) + 1], A.scale_log2, -mn));
-          l[nb] += p0 + p1;
-          pw[e >> 1] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p0, p1}), bf16x2_t));
-        }
-        pf[nb][kk] = __builtin_bit_cast(s16x8, pw);
-      }
-    }
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        u32x4 ae, ao;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          uint32_t y[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int key = 2 * n + i, at = key * M::NB + (FP8 ? 2 * j : j), sa = key * J + j;  // bytes among the eight keys'
-            const uint32_t w = x.v[kk][at >> 4][(at >> 2) & 3];
-            const float s = scale_of(x.vs[kk][sa >> 4][(sa >> 2) & 3], sa & 3);
-            y[i] = FP8 ? from_fp8(w, s, (at >> 1) & 1) : from_fp4(w, s, at & 3);
-          }
-          ae[n] = low_halves(y[0], y[1]);
-          ao[n] = high_halves(y[0], y[1]);
-        }
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          o[nb][j][0] = mfma16(__builtin_bit_cast(s16x8, ae), pf[nb][kk], o[nb][j][0]);
-          o[nb][j][1] = mfma16(__builtin_bit_cast(s16x8, ao), pf[nb][kk], o[nb][j][1]);
-        }
-      }
+      for (int u = 0; u < R::VS; ++u) vs[u] = x.vs[kk][u];
+    }, st, A.scale_log2);
   };
 
-  R x;
   long nxt = last > first ? page_of(first + wave) : 0;  // (scalar reads of the table, ahead of the loads that need them)
   if (REFILL && first + wave < last) {
-    load(first + wave, nxt, x);
+    load_k(first + wave, nxt, x);
+    load_v(first + wave, nxt, x);
     nxt = page_of(first + wave + NW);
   }
   for (int p = first + wave; p < last; p += NW) {
+    f32x4 st[NB][4];
     if constexpr (REFILL) {
       const bool more = p + NW < last;
-      f32x4 st[NB][4];
-      scores(x, st);
+      scores(st);
       if (more) load_k(p + NW, nxt, x);
-      weigh(p, x, st);
+      weigh(p, st);
       if (more) load_v(p + NW, nxt, x);
       nxt = page_of(p + 2 * NW);
     } else {
-      load(p, nxt, x);
+      load_k(p, nxt, x);
+      load_v(p, nxt, x);
       nxt = page_of(p + NW);
-      f32x4 st[NB][4];
-      scores(x, st);
-      weigh(p, x, st);
+      scores(st);
+      weigh(p, st);
     }
   }
+  rows.finish();
 
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    l[nb] = xor_sum<16>(l[nb]);
-    l[nb] = xor_sum<32>(l[nb]);
-  }
   const size_t row_ws = ((size_t)bu * A.nparts * A.Hkv + kvh) * RS, step = (size_t)A.Hkv * RS;  // partial results: part 0's first row, from part to part
-  auto result = [&](int rw, int d, const f32x4& O, float L) {
+  auto result = [&](int rw, int d, const f32x4& O, float inv) {
     const int row = row0 + rw, ti = PROMPT ? row / G : 0, hq = row - ti * G;
     uint16_t* p = A.out + ((size_t)(q0 + ti) * A.H + kvh * G + hq) * DH + d;
-    if (pos0 + ti >= 0) st_results(p, O, L);
+    if (pos0 + ti >= 0) st_results(p, O, inv);
     else *reinterpret_cast<s16x4*>(p) = s16x4{0, 0, 0, 0};  // a row without keys
   };
-  auto leave = [&](int rw, int d, const f32x4& O, float mm, float L) {
-    if (parts == 1) return result(rw, d, O, L);
+  auto leave = [&](int rw, int d, const f32x4& O, float mm, float L, float inv) {
+    if (parts == 1) return result(rw, d, O, inv);
     const size_t row = row_ws + part * step + rw;
     agent_store4(A.ws_o + row * DH + d, O);
     if (d == 0) agent_store2(A.ws_ml + row * 2, mm, L);
   };
   if constexpr (NW == 1) {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int nb = 0; nb < NB; ++nb) {
+      const float inv = 1.f / rows.l[nb];
       if (16 * nb + c < RN)
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const f32x4 &e = o[nb][j][0], &d = o[nb][j][1];
-          leave(16 * nb + c, 32 * j + 8 * g, f32x4{e[0], d[0], e[1], d[1]}, m[nb], l[nb]);
-          leave(16 * nb + c, 32 * j + 8 * g + 4, f32x4{e[2], d[2], e[3], d[3]}, m[nb], l[nb]);
-        }
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            leave(16 * nb + c, 32 * j + 8 * g + 4 * half, rows.dims(nb, j, half), rows.m[nb], rows.l[nb], inv);
+    }
   } else {  // the waves meet in LDS: [NW][RS][LD] sums, [NW][RS][2] maxima and sums of weights
     float* ml = sm + NW * RS * LD;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
       if (16 * nb + c < RN) {
         const int at = wave * RS + 16 * nb + c;
-        float* so = sm + at * LD + 8 * g;
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const f32x4 &e = o[nb][j][0], &d = o[nb][j][1];
-          *reinterpret_cast<f32x4*>(so + 32 * j) = f32x4{e[0], d[0], e[1], d[1]};
-          *reinterpret_cast<f32x4*>(so + 32 * j + 4) = f32x4{e[2], d[2], e[3], d[3]};
-        }
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) *reinterpret_cast<f32x4*>(sm + at * LD + 32 * j + 8 * g + 4 * half) = rows.dims(nb, j, half);
         if (g == 0) {
-          ml[at * 2] = m[nb];
-          ml[at * 2 + 1] = l[nb];
+          ml[at * 2] = rows.m[nb];
+          ml[at * 2 + 1] = rows.l[nb];
         }
       }
     __syncthreads();
@@ -688,7 +736,7 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : 3) void attn_mx_
         L += ml[(w * RS + rw) * 2 + 1] * f;
         O += *reinterpret_cast<const f32x4*>(sm + (w * RS + rw) * LD + d) * f;
       }
-      leave(rw, d, O, mm, L);
+      leave(rw, d, O, mm, L, 1.f / L);
     }
   }
   if (parts == 1) return;
@@ -728,7 +776,7 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : 3) void attn_mx_
           O += po[i] * f;
         }
     }
-    result(rw, d, O, L);
+    result(rw, d, O, 1.f / L);
   }
 }
 
@@ -921,30 +969,35 @@ void attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Te
 #undef GO
 }
 
-constexpr int TURN_WAVES = 4, TURN_BLOCKS = 2;  // of 16 rows
+constexpr int PROMPT_WAVES = 4, PROMPT_BLOCKS = 2;  // of 16 rows
 
-// new tokens against the pools themselves: blocks of 32 rows of (token, head), for prompts of few tokens behind long contexts
-void attn_turn_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables, const at::Tensor& cu_q,
+// new tokens against the pools: units of 32 rows of (token, head), of four waves that share the pages or one that has them all
+void attn_prompt_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables, const at::Tensor& cu_q,
                   const at::Tensor& ctx_lens, at::Tensor& out, const c10::optional<at::Tensor>& ws_o, const c10::optional<at::Tensor>& ws_ml,
-                  const c10::optional<at::Tensor>& tickets, int64_t max_qlen, int64_t pages_per_part, int64_t nparts, double scale) {
-  const char* op = "attn_turn_mx";
+                  const c10::optional<at::Tensor>& tickets, int64_t max_qlen, int64_t pages_per_part, int64_t nparts, int64_t waves, double scale) {
+  const char* op = "attn_prompt_mx";
   XCHECK(q.is_cuda() && q.dim() == 3, op, ": q must be [T, H, Dh] on a GPU");
   const c10::DeviceGuard guard(q.device());
   bool fp8 = false;
   const int64_t H = q.size(1), Dh = q.size(2), Hkv = k_cache.dim() == 3 ? k_cache.size(1) : 1, B = ctx_lens.numel();
   XCHECK(max_qlen >= 0 && max_qlen < (1 << 24), op, ": max_qlen");
-  constexpr int64_t ROWS = 16 * TURN_BLOCKS;
+  constexpr int64_t ROWS = 16 * PROMPT_BLOCKS;
   const int64_t blocks = std::max<int64_t>(1, (max_qlen * (H / std::max<int64_t>(Hkv, 1)) + ROWS - 1) / ROWS);
   const AttnArgs a = attn_args(op, fp8, q, k_cache, v_cache, tables, ctx_lens, &cu_q, out, ws_o, ws_ml, tickets, blocks, ROWS, pages_per_part, nparts, scale);
   if (B == 0 || max_qlen == 0) return;
-  const size_t lds = (size_t)TURN_WAVES * ROWS * (Dh + 6) * sizeof(float);  // 67 KB at heads of 128
+  XCHECK(waves == 1 || waves == PROMPT_WAVES, op, ": 1 or 4 waves");
+  const size_t lds = waves == 1 ? 0 : (size_t)PROMPT_WAVES * ROWS * (Dh + 6) * sizeof(float);  // 67 KB at heads of 128
   const unsigned units = (unsigned)(B * blocks * nparts * Hkv);
 #define GO(DHV, F)                                                                                                                         \
   do {                                                                                                                                     \
-    auto* f = attn_mx_kernel<DHV, F, TURN_WAVES, TURN_BLOCKS, true, !(F && DHV == 128)>;                                                                       \
+    if (waves == 1) {                                                                                                                      \
+      attn_mx_kernel<DHV, F, 1, PROMPT_BLOCKS, true, !(F && DHV == 128)><<<units, 64, 0, stream()>>>(a);                                     \
+      break;                                                                                                                               \
+    }                                                                                                                                      \
+    auto* f = attn_mx_kernel<DHV, F, PROMPT_WAVES, PROMPT_BLOCKS, true, !(F && DHV == 128)>;                                                   \
     static const hipError_t set = hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);              \
     XCHECK(set == hipSuccess, op, ": LDS");                                                                                                \
-    f<<<units, 64 * TURN_WAVES, lds, stream()>>>(a);                                                                                       \
+    f<<<units, 64 * PROMPT_WAVES, lds, stream()>>>(a);                                                                                       \
   } while (0)
   MX_GO(fp8, Dh, GO);
 #undef GO
@@ -956,7 +1009,7 @@ void bind_kv_mx(pybind11::module& m) {
   m.def("rope_kv_write_mx", &rope_kv_write_mx);
   m.def("kv_read_mx", &kv_read_mx);
   m.def("attn_decode_mx", &attn_decode_mx);
-  m.def("attn_turn_mx", &attn_turn_mx);
+  m.def("attn_prompt_mx", &attn_prompt_mx);
 }
 
 }  // namespace xot

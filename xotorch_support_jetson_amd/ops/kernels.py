@@ -472,40 +472,53 @@ def attn_decode_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 
 # scratch of attn_prefill_mx's bf16 pages: at most this much, or one sequence's
 MX_READ_BYTES = 1 << 30
-MX_TURN_UNITS = 1536
 
 
-def mx_turn(B: int, T: int, max_qlen: int, G: int, Hkv: int) -> bool:
-  """Whether attn_prefill_mx reads the pools themselves, in units of 32 rows (token, head of a KV head) against all the keys: where they
-  are few, or the sequences' new tokens are (a turn of a chat, decode steps with a prompt among them), whose contexts would cost more to
-  read back than to attend to; not where a long prompt among many sequences would make most of the units empty.  us via bf16 pages /
-  from the pools, mxfp4, heads of 128: 4 sequences of 64 new tokens behind 1000, 32 heads on 8, 51 / 17 (behind 8000 287 / 65), of 256 58 / 41,
-  of 512 70 / 79 (2048 units); one of 512 behind 8000, 64 heads, 285 / 176; 12 of 128 and no more 22 / 29 (1536 units; behind 1000 61 / 56),
-  of 512 82 / 117."""
-  units = Hkv * -(-max_qlen * G // 32)
-  return B * units <= MX_TURN_UNITS or (T * G <= 256 * B and B * units <= 1 << 18)
+def mx_prompt_units(B: int, max_qlen: int, G: int, Hkv: int) -> int:
+  """Units (32 rows of token and head) of a launch over B sequences of at most max_qlen new tokens; those past a sequence's end are empty."""
+  return B * Hkv * max(1, -(-max_qlen * G // 32))
+
+
+def mx_prompt_direct(B: int, T: int, max_qlen: int, G: int, Hkv: int, Dh: int, fp8: bool) -> bool:
+  """Whether attn_prefill_mx reads the pools themselves.  Not where a long prompt among many sequences would make most of the units
+  empty, nor long prompts in mxfp8 of 128 dims, whose kernel has too few registers to load ahead.  us via bf16 pages / from the pools, heads
+  of 128: mxfp4 4 sequences of 64 new tokens behind 1000, 32 heads on 8, 50 / 15, one of 128 behind 8000 270 / 41, 12 of 512 82 / 65, behind
+  1000 186 / 168, one of 4096 164 / 158, with 64 heads 311 / 309; mxfp8 12 of 512 behind 1000 192 / 185, with 64 heads 339 / 355, one of
+  2048 81 / 67, of 4096 164 / 195, with 64 heads 310 / 348; heads of 64, mxfp8, 4096 120 / 120."""
+  units = mx_prompt_units(B, max_qlen, G, Hkv)
+  if units > 1 << 18:
+    return False
+  return not (fp8 and Dh == 128 and units >= 4096 and T * G >= 8192 * B)
+
+
+def mx_prompt_waves(units: int) -> int:
+  """Waves of a unit: four share its pages where the units are few, one takes them all where they fill the chip.  us with 4 / 1, mxfp4, heads
+  of 128: 256 units of 1064 keys 15 / 30, 512 21 / 31, 1536 of 1128 56 / 56, of 128 29 / 19, 2048 of up to 2048 64 / 65, of up to 512 40 / 31,
+  6144 201 / 168."""
+  return 4 if units < 1536 else 1
 
 
 def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, cu_q: torch.Tensor,
                     ctx_lens: torch.Tensor, max_qlen: int, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
   """attn_prefill over pools in 8 or 4 bits: q [T, H, Dh], the tokens cu_q[b] .. cu_q[b + 1] are the last of sequence b's ctx_lens[b] (at
-  most max_qlen of them), each attends to what lies before it and itself.  Few tokens read the pools themselves (mx_turn).  Others'
-  products outweigh a pass over the cache: the pages are read back into bf16 scratch, a group of sequences at a time, which the prompt
-  attention reads."""
+  most max_qlen of them), each attends to what lies before it and itself; a token without keys gives zeros.  From the pools themselves
+  (mx_prompt_direct), or their pages are read back into bf16 scratch, a group of sequences at a time, which the bf16 prompt attention
+  reads.  As there, a NaN among a later token's values reaches the earlier ones of its page."""
   T, H, Dh = q.shape
   B, W = block_tables.shape
   Hkv = k_cache.shape[1]
   out = torch.empty_like(q) if out is None else out
   gpu = _gpu(q)
-  if gpu and B and H % Hkv == 0 and mx_turn(B, T, max_qlen, H // Hkv, Hkv):
-    units = B * Hkv * max(1, -(-max_qlen * (H // Hkv) // 32))
-    nparts = max(1, min(W // 16, 512 // max(1, units)))
+  G = max(1, H // Hkv)
+  if gpu and mx_prompt_direct(max(B, 1), T, max_qlen, G, Hkv, Dh, k_cache.shape[2] > PAGE * Dh):
+    units = mx_prompt_units(max(B, 1), max_qlen, G, Hkv)
+    nparts = max(1, min(W // 16, 512 // units))
     ws = [None] * 3
-    if nparts > 1:
-      rows = units * nparts * 32
-      ws = [torch.empty(rows * Dh, dtype=torch.float32, device=q.device), torch.empty(rows * 2, dtype=torch.float32, device=q.device),
-            torch.zeros(units, dtype=torch.int32, device=q.device)]
-    require().attn_turn_mx(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, out, *ws, int(max_qlen), -(-W // nparts), nparts, float(scale))
+    if nparts > 1:  # few rows behind long contexts
+      ws = [torch.empty(units * nparts * 32 * n, dtype=torch.float32, device=q.device) for n in (Dh, 2)]
+      ws.append(torch.zeros(units, dtype=torch.int32, device=q.device))
+    require().attn_prompt_mx(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, out, *ws, int(max_qlen), -(-W // nparts), nparts,
+                             mx_prompt_waves(units), float(scale))
     return out
   per = max(1, min(B, MX_READ_BYTES // max(1, W * Hkv * PAGE * Dh * 4))) if gpu else max(1, B)
   k = torch.empty(per * W, Hkv, PAGE, Dh, dtype=torch.bfloat16, device=q.device)
