@@ -326,6 +326,22 @@ def test_decode_parts_gpu(gpu, fmt, Dh, H, Hkv, waves, monkeypatch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("order", [1, 2])
+@pytest.mark.parametrize("B", [1, 2, 9, 63, 64])
+def test_decode_order_gpu(gpu, B, order, monkeypatch):
+  """Whatever order the sequences are taken in, each gets its own result: lengths alike, all but one, some of them 0, the same as given."""
+  g = torch.Generator().manual_seed(B)
+  for lens in ([130] * B, [130] * (B - 1) + [500], torch.randint(0, 300, (B,), generator=g).tolist()):
+    s = Seqs("mxfp4", lens, 1, 64, dev=gpu, width=8)
+    monkeypatch.setattr(K, "mx_decode_order", lambda *a: 0)
+    a = check_decode(s, 2, 0.125, ws=K.MXDecodeWorkspace(B, 2, 1, 64, 512, gpu)) if B <= 9 else None
+    monkeypatch.setattr(K, "mx_decode_order", lambda *a: order)
+    monkeypatch.setattr(K.MXDecodeWorkspace, "parts", staticmethod(lambda b, h, pages: (pages, 1)))
+    b = check_decode(s, 2, 0.125, ws=K.MXDecodeWorkspace(B, 2, 1, 64, 512, gpu))
+    assert a is None or torch.allclose(a.float(), b.float(), rtol=2.0 ** -6, atol=2.0 ** -6)
+
+
+@pytest.mark.gpu
 def test_decode_workspace_gpu(gpu):
   """Wider tables than the workspace was made for, fewer sequences, and the rule's own choice at many sizes."""
   s = Seqs("mxfp4", [70, 1200, 0], 2, 64, dev=gpu, width=40)

@@ -361,7 +361,7 @@ struct AttnArgs {
   uint16_t* out;
   float *ws_o, *ws_ml;
   int* tickets;
-  int T, width, H, Hkv, ppp, nparts, num_pages, blocks;
+  int T, width, H, Hkv, ppp, nparts, num_pages, blocks, order;
   float scale_log2;
 };
 
@@ -371,6 +371,22 @@ __device__ __forceinline__ void st_results(uint16_t* p, const f32x4& O, float in
 #pragma unroll
   for (int r = 0; r < 4; ++r) y[r] = (short)f2bf(O[r] * inv);
   *reinterpret_cast<s16x4*>(p) = y;
+}
+
+// The sequence at place p of a decode step of at most 64.  order 1: the longest first, so that none starts late.  2 (units that all start at
+// once, up to three a CU): the longer half, longest first, then the shorter, shortest first: the units that a CU gets, one of each round, are
+// then of about the same length together.  Figures beside ops.kernels.mx_decode_order; finding the place costs a unit about 1 us.
+__device__ __forceinline__ int sequence_at(const AttnArgs& A, int p) {
+  const int lane = threadIdx.x & 63, B = A.T, half = (B + 1) >> 1;
+  const int pages = lane < B ? (min(max(A.ctx_lens[lane], 0), A.width * PAGE) + PAGE - 1) / PAGE : 0;
+  if (__ballot(lane < B && pages != __builtin_amdgcn_readfirstlane(pages)) == 0) return p;  // (all as long: as they are given)
+  const uint32_t key = lane < B ? (uint32_t)pages * 64u + 63u - lane : 0;  // no two alike
+  int rank = 0;
+  for (int j0 = 0; j0 < B; j0 += 8)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) rank += (uint32_t)__builtin_amdgcn_readlane((int)key, j0 + j) > key ? 1 : 0;
+  const int want = A.order == 1 || p < half ? p : B - 1 - (p - half);
+  return __builtin_ctzll(__ballot(lane < B && rank == want));
 }
 
 // What a lane's eight keys hold past the context may be anything, NaN too: it becomes zeros (their probabilities are 0, but 0 NaN is
@@ -580,7 +596,7 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : 3) void attn_mx_
   constexpr int J = M::J, LD = DH + 4;
   extern __shared__ __attribute__((aligned(16))) float sm[];
   const int kvh = blockIdx.x % A.Hkv, bp = blockIdx.x / A.Hkv, part = bp % A.nparts, bu = bp / A.nparts;
-  const int b = PROMPT ? bu / A.blocks : bu, row0 = PROMPT ? (A.blocks - 1 - (bu - b * A.blocks)) * 16 * NB : 0;
+  const int b = PROMPT ? bu / A.blocks : A.order != 0 ? sequence_at(A, bu) : bu, row0 = PROMPT ? (A.blocks - 1 - (bu - b * A.blocks)) * 16 * NB : 0;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, G = A.H / A.Hkv;
   const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q0 = PROMPT ? min(max(A.cu_q[b], 0), A.T) : b, qlen = PROMPT ? min(max(A.cu_q[b + 1], q0), A.T) - q0 : 1, nrows = qlen * G;
@@ -822,8 +838,8 @@ bool caches_ok(const char* op, const at::Tensor& k, const at::Tensor& v, int64_t
 // 16.2 / 15.0, of 32 + 16 10.9 / 11.2, 512 4.3 / 5.3, 1 2.7 / 4.0
 constexpr int WRITE_HEADS = 4, WRITE_HEADS_ROWS = 1 << 17;
 
-void rope_kv_write_mx(const at::Tensor& qkv, const at::Tensor& pos, const at::Tensor& cos_sin, const at::Tensor& slots, at::Tensor& q_out,
-                      at::Tensor& k_cache, at::Tensor& v_cache, int64_t H, int64_t Hkv) {
+at::Tensor rope_kv_write_mx(const at::Tensor& qkv, const at::Tensor& pos, const at::Tensor& cos_sin, const at::Tensor& slots,
+                            const c10::optional<at::Tensor>& out, at::Tensor& k_cache, at::Tensor& v_cache, int64_t H, int64_t Hkv) {
   const char* op = "rope_kv_write_mx";
   XCHECK(qkv.is_cuda() && qkv.dim() == 2, op, ": qkv must be [T, (H + 2 Hkv) Dh] on a GPU");
   const at::Device dev = qkv.device();
@@ -835,12 +851,13 @@ void rope_kv_write_mx(const at::Tensor& qkv, const at::Tensor& pos, const at::Te
   on_gpu(op, pos, at::kInt, "pos", dev);
   on_gpu(op, cos_sin, at::kFloat, "cos_sin", dev);
   on_gpu(op, slots, at::kLong, "slots", dev);
+  at::Tensor q_out = out.has_value() ? *out : at::empty({T, H, Dh}, qkv.options());
   on_gpu(op, q_out, at::kBFloat16, "q_out", dev);
   const bool fp8 = caches_ok(op, k_cache, v_cache, Dh, dev);
   XCHECK(k_cache.size(1) == Hkv, op, ": the caches have ", k_cache.size(1), " heads");
   XCHECK(pos.numel() == T && slots.numel() == T && q_out.numel() == T * H * Dh, op, ": pos, slots or q_out of another length");
   XCHECK(cos_sin.dim() == 2 && cos_sin.size(1) == Dh && cos_sin.size(0) >= 1, op, ": cos_sin must be [positions, Dh]");
-  if (T == 0) return;
+  if (T == 0) return q_out;
   XCHECK((reinterpret_cast<uintptr_t>(qkv.data_ptr()) | reinterpret_cast<uintptr_t>(q_out.data_ptr()) | reinterpret_cast<uintptr_t>(cos_sin.data_ptr())) % 16 == 0,
          op, ": qkv, q_out and cos_sin must be aligned to 16 bytes");
   XCHECK(T < (1 << 26) && H + 2 * Hkv < (1 << 20) && (T + 3) / 4 * (H + 2 * Hkv) < (int64_t(1) << 26), op, ": too many tokens for one launch");
@@ -859,22 +876,26 @@ void rope_kv_write_mx(const at::Tensor& qkv, const at::Tensor& pos, const at::Te
   MX_GO(fp8, Dh, GO);
 #undef GO
 #undef GO_HB
+  return q_out;
 }
 
-void kv_read_mx(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables, const at::Tensor& ctx_lens, at::Tensor& k_out,
-                at::Tensor& v_out, bool skip, const c10::optional<at::Tensor>& own) {
+std::tuple<at::Tensor, at::Tensor> kv_read_mx(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables, const at::Tensor& ctx_lens,
+                int64_t Dh, const c10::optional<at::Tensor>& k_opt, const c10::optional<at::Tensor>& v_opt, bool skip, const c10::optional<at::Tensor>& own) {
   const char* op = "kv_read_mx";
   XCHECK(k_cache.is_cuda(), op, ": k_cache must be on a GPU");
   const at::Device dev = k_cache.device();
   const c10::DeviceGuard guard(dev);
   on_gpu(op, tables, at::kInt, "block_tables", dev);
   on_gpu(op, ctx_lens, at::kInt, "ctx_lens", dev);
+  XCHECK(tables.dim() == 2 && ctx_lens.numel() == tables.size(0), op, ": a row of block_tables for each of ctx_lens");
+  const int64_t n = tables.numel(), Hkv = k_cache.dim() == 3 ? k_cache.size(1) : 0;
+  const bool fp8 = caches_ok(op, k_cache, v_cache, Dh, dev);
+  const auto bf16 = k_cache.options().dtype(at::kBFloat16);
+  at::Tensor k_out = k_opt.has_value() ? *k_opt : at::empty({n, Hkv, PAGE, Dh}, bf16);
+  at::Tensor v_out = v_opt.has_value() ? *v_opt : at::empty({n, Hkv, Dh, PAGE}, bf16);
   on_gpu(op, k_out, at::kBFloat16, "k_out", dev);
   on_gpu(op, v_out, at::kBFloat16, "v_out", dev);
-  XCHECK(tables.dim() == 2 && ctx_lens.numel() == tables.size(0), op, ": a row of block_tables for each of ctx_lens");
-  XCHECK(k_out.dim() == 4 && v_out.dim() == 4, op, ": k_out and v_out must be 4-D");
-  const int64_t Dh = k_out.size(3), n = tables.numel(), Hkv = k_cache.dim() == 3 ? k_cache.size(1) : 0;
-  const bool fp8 = caches_ok(op, k_cache, v_cache, Dh, dev);
+  XCHECK(k_out.dim() == 4 && v_out.dim() == 4 && k_out.size(3) == Dh, op, ": k_out and v_out must be 4-D");
   XCHECK(k_out.size(0) == n && k_out.size(1) == Hkv && k_out.size(2) == PAGE && v_out.size(0) == n && v_out.size(1) == Hkv &&
              v_out.size(2) == Dh && v_out.size(3) == PAGE,
          op, ": k_out must be [entries, Hkv, 64, Dh], v_out [entries, Hkv, Dh, 64]");
@@ -884,7 +905,7 @@ void kv_read_mx(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::
     on_gpu(op, *own, at::kInt, "own", dev);
     XCHECK(own->numel() == n, op, ": own must be of the entries' length");
   }
-  if (n == 0) return;
+  if (n == 0) return {k_out, v_out};
   XCHECK(n < (int64_t(1) << 24) && n * Hkv < (int64_t(1) << 24), op, ": too many pages for one launch");
 #define GO(DHV, F)                                                                                                                         \
   kv_read_mx_kernel<DHV, F><<<(unsigned)(n * Hkv), 256, 0, stream()>>>(                                                                    \
@@ -892,13 +913,14 @@ void kv_read_mx(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::
       bf(k_out), bf(v_out), (int)Hkv, (int)k_cache.size(0), skip, own.has_value() ? own->data_ptr<int32_t>() : nullptr)
   MX_GO(fp8, Dh, GO);
 #undef GO
+  return {k_out, v_out};
 }
 
 // what both forms of the attention check; cu_q: several tokens a sequence
 AttnArgs attn_args(const char* op, bool& fp8, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables,
                    const at::Tensor& ctx_lens, const at::Tensor* cu_q, at::Tensor& out, const c10::optional<at::Tensor>& ws_o,
                    const c10::optional<at::Tensor>& ws_ml, const c10::optional<at::Tensor>& tickets, int64_t blocks, int64_t block_rows,
-                   int64_t pages_per_part, int64_t nparts, double scale) {
+                   int64_t pages_per_part, int64_t nparts, double scale, int order = 0) {
   const at::Device dev = q.device();
   on_gpu(op, q, at::kBFloat16, "q", dev);
   on_gpu(op, out, at::kBFloat16, "out", dev);
@@ -941,21 +963,23 @@ AttnArgs attn_args(const char* op, bool& fp8, const at::Tensor& q, const at::Ten
   }
   return {bf(q), k_cache.data_ptr<uint8_t>(), v_cache.data_ptr<uint8_t>(), tables.data_ptr<int32_t>(), ctx_lens.data_ptr<int32_t>(),
           cu_q == nullptr ? nullptr : cu_q->data_ptr<int32_t>(), bf(out), o, ml, tk, (int)T, (int)tables.size(1), (int)H, (int)Hkv, (int)pages_per_part,
-          (int)nparts, (int)k_cache.size(0), (int)blocks, (float)scale * LOG2E};
+          (int)nparts, (int)k_cache.size(0), (int)blocks, order, (float)scale * LOG2E};
 }
 
-void attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables,
-                    const at::Tensor& ctx_lens, at::Tensor& out, const c10::optional<at::Tensor>& ws_o, const c10::optional<at::Tensor>& ws_ml,
-                    const c10::optional<at::Tensor>& tickets, int64_t pages_per_part, int64_t nparts, int64_t waves, bool refill, double scale) {
+at::Tensor attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables,
+                    const at::Tensor& ctx_lens, const c10::optional<at::Tensor>& out_opt, const c10::optional<at::Tensor>& ws_o, const c10::optional<at::Tensor>& ws_ml,
+                    const c10::optional<at::Tensor>& tickets, int64_t pages_per_part, int64_t nparts, int64_t waves, bool refill, int64_t order, double scale) {
   const char* op = "attn_decode_mx";
   XCHECK(q.is_cuda() && q.dim() == 3, op, ": q must be [B, H, Dh] on a GPU");
   const c10::DeviceGuard guard(q.device());
   bool fp8 = false;
+  at::Tensor out = out_opt.has_value() ? *out_opt : at::empty_like(q);
   const int64_t H = q.size(1), Dh = q.size(2), Hkv = k_cache.dim() == 3 ? k_cache.size(1) : 1;
   const AttnArgs a = attn_args(op, fp8, q, k_cache, v_cache, tables, ctx_lens, nullptr, out, ws_o, ws_ml, tickets, 1, H / std::max<int64_t>(Hkv, 1),
-                               pages_per_part, nparts, scale);
+                               pages_per_part, nparts, scale, (int)order);
+  XCHECK(order == 0 || (order >= 1 && order <= 2 && q.size(0) <= 64), op, ": an order of at most 64 sequences");
   XCHECK(waves == 1 || waves == 2 || waves == 4, op, ": 1, 2 or 4 waves");
-  if (q.size(0) == 0) return;
+  if (q.size(0) == 0) return out;
   const size_t lds = waves == 1 ? 0 : (size_t)waves * (H / Hkv) * (Dh + 6) * sizeof(float);  // at most 34 KB
   const unsigned units = (unsigned)(q.size(0) * nparts * Hkv);
 #define GO(DHV, F)                                                                                              \
@@ -967,6 +991,7 @@ void attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Te
   } while (0)
   MX_GO(fp8, Dh, GO);
 #undef GO
+  return out;
 }
 
 constexpr int PROMPT_WAVES = 4, PROMPT_BLOCKS = 2;  // of 16 rows

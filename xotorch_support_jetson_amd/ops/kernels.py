@@ -362,34 +362,29 @@ def rope_kv_write_mx(qkv: torch.Tensor, pos: torch.Tensor, cos_sin: torch.Tensor
                      v_cache: torch.Tensor, H: int, Hkv: int, q_out: torch.Tensor | None = None) -> torch.Tensor:
   """qkv [T, (H+2Hkv)*Dh] -> rotated q [T, H, Dh]; rotated k (quantised from fp32) and v into the pools at `slots` (distinct; one
   outside the pools is not written)."""
-  T = qkv.shape[0]
-  Dh = qkv.shape[1] // (H + 2 * Hkv)
   if not _gpu(qkv):
-    x = qkv.view(T, H + 2 * Hkv, Dh)
+    x = qkv.unflatten(1, (H + 2 * Hkv, -1))
     q = ref.rope(x[:, :H], pos, cos_sin)
     ref.mx_write(ref.rope(x[:, H:H + Hkv].float(), pos, cos_sin), x[:, H + Hkv:], slots, k_cache, v_cache)
     if q_out is not None:
       q_out.copy_(q.view(q_out.shape))
       return q_out
     return q
-  q_out = torch.empty(T, H, Dh, dtype=qkv.dtype, device=qkv.device) if q_out is None else q_out
-  require().rope_kv_write_mx(qkv, pos, cos_sin, slots, q_out, k_cache, v_cache, int(H), int(Hkv))
-  return q_out
+  return require().rope_kv_write_mx(qkv, pos, cos_sin, slots, q_out, k_cache, v_cache, int(H), int(Hkv))
 
 
 def kv_read_mx(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor, Dh: int,
                k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None, skip: bool = False):
   """The pages that block_tables [B, W] names, exactly as bf16: (K [B*W, Hkv, 64, Dh], V [B*W, Hkv, Dh, 64] in the bf16 pool's layout).
   Keys past a sequence's context are zeros; skip: pages wholly past it are left as they are."""
+  if _gpu(k_cache):
+    return require().kv_read_mx(k_cache, v_cache, block_tables, ctx_lens, int(Dh), k_out, v_out, bool(skip), None)
   n, Hkv = block_tables.numel(), k_cache.shape[1]
   if k_out is None:
     k_out = torch.empty(n, Hkv, PAGE, Dh, dtype=torch.bfloat16, device=k_cache.device)
   if v_out is None:
     v_out = torch.empty(n, Hkv, Dh, PAGE, dtype=torch.bfloat16, device=k_cache.device)
-  if not _gpu(k_cache):
-    ref.kv_read_mx(k_cache, v_cache, block_tables, ctx_lens, k_out, v_out)
-  else:
-    require().kv_read_mx(k_cache, v_cache, block_tables, ctx_lens, k_out, v_out, bool(skip), None)
+  ref.kv_read_mx(k_cache, v_cache, block_tables, ctx_lens, k_out, v_out)
   return k_out, v_out
 
 
@@ -405,7 +400,7 @@ class MXDecodeWorkspace:
     self.o = torch.empty(max(1, rows * H * Dh), dtype=torch.float32, device=device)
     self.ml = torch.empty(max(1, rows * H * 2), dtype=torch.float32, device=device)
     self.tickets = torch.zeros(max_batch * Hkv, dtype=torch.int32, device=device)
-    self.chosen = {}  # (batch, pages, fp8) -> pages of a part, parts, waves, refilling
+    self.chosen = {}  # (batch, pages, fp8) -> pages of a part, parts, waves, refilling, order
 
   @staticmethod
   def parts(batch: int, Hkv: int, pages: int):
@@ -416,7 +411,7 @@ class MXDecodeWorkspace:
     sequences of up to 700 tokens on 32 KV heads 7.5 uncut, 8.4 in 2, 64 of 30 to 2000 on 8 20.8, 26 in 2.  Past 128 pages every context is
     cut: its longest part ends the launch."""
     pairs = max(1, batch * Hkv)
-    most = min(512 // pairs, pages // (4 if pages <= 16 else 8)) if pairs < 256 or pages >= 64 else 1
+    most = min(512 // pairs, -(-pages // 4) if pages <= 16 else pages // 8) if pairs < 256 or pages >= 64 else 1
     most = max(1, most, -(-pages // 128))
     return -(-pages // most), most
 
@@ -432,7 +427,8 @@ class MXDecodeWorkspace:
   def choose(self, batch: int, pages: int, fp8: bool):
     key = (batch, pages, fp8)
     if key not in self.chosen:
-      self.chosen[key] = (*self.partition(batch, pages), *mx_decode_waves(batch * self.Hkv, pages, fp8))
+      parts = self.partition(batch, pages)
+      self.chosen[key] = (*parts, *mx_decode_waves(batch * self.Hkv, pages, fp8), mx_decode_order(batch, self.Hkv, parts[1]))
     return self.chosen[key]
 
 
@@ -446,6 +442,17 @@ def mx_decode_waves(pairs: int, pages: int, fp8: bool):
   if pairs < 1024 or pages > 16:
     return 4, pairs < 1024
   return (1 if pairs >= 2048 and pages <= 12 and not fp8 else 2), False
+
+
+def mx_decode_order(batch: int, Hkv: int, parts: int) -> int:
+  """The order of an attn_decode_mx launch's sequences (csrc/kv_mx.hip sequence_at): 0 as given, 1 the longest first, 2 paired by length.
+  us with 0 / 1 / 2, ragged contexts up to 2000 tokens: 64 sequences on 8 KV heads of 128 (512 units) mxfp8 35.1 / 31.9 / 27.6, another draw
+  36.9 / 33.4 / 29.8, mxfp4 21.1 / 18.6 / 18.0; 60 on 32 (1920) mxfp8 91.7 / 81.5 / 86.3; 40 on 8 (320) 26.5 / 25.6 / 26.4; 10 on 32 (320)
+  mxfp4 15.3 / 15.9 / 16.3."""
+  units = batch * Hkv
+  if batch > 64 or parts > 1 or units <= 384:
+    return 0
+  return 2 if units <= 768 else 1
 
 
 def attn_decode_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
@@ -464,10 +471,8 @@ def attn_decode_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     ws = MXDecodeWorkspace(B, H, k_cache.shape[1], Dh, width * PAGE, q.device)
   elif ws.Hkv != k_cache.shape[1]:
     raise RuntimeError(f"decode workspace for {ws.Hkv} KV heads, not {k_cache.shape[1]}")
-  out = torch.empty_like(q) if out is None else out
-  ppp, nparts, waves, refill = ws.choose(B, width, k_cache.shape[2] > PAGE * Dh)
-  require().attn_decode_mx(q, k_cache, v_cache, block_tables, ctx_lens, out, ws.o, ws.ml, ws.tickets, ppp, nparts, waves, refill, float(scale))
-  return out
+  return require().attn_decode_mx(q, k_cache, v_cache, block_tables, ctx_lens, out, ws.o, ws.ml, ws.tickets,
+                                  *ws.choose(B, width, k_cache.shape[2] > PAGE * Dh), float(scale))
 
 
 # scratch of attn_prefill_mx's bf16 pages: at most this much, or one sequence's
@@ -528,7 +533,7 @@ def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     n = min(per, B - b)
     tables, ctx, cu = block_tables[b:b + n], ctx_lens[b:b + n], cu_q[b:b + n + 1]
     if gpu:
-      require().kv_read_mx(k_cache, v_cache, tables, ctx, k[:n * W], v[:n * W], True, own[:n])
+      require().kv_read_mx(k_cache, v_cache, tables, ctx, Dh, k[:n * W], v[:n * W], True, own[:n])
     else:
       ref.kv_read_mx(k_cache, v_cache, tables, ctx, k, v)
     with torch.cuda.device(q.device) if gpu else contextlib.nullcontext():
