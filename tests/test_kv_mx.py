@@ -439,6 +439,97 @@ def test_turns_gpu(gpu, fmt, Dh, H, Hkv, monkeypatch):
 
 
 @pytest.mark.gpu
+def test_far_pages_gpu(gpu):
+  """Pages whose bytes lie past 2^32 of their pool: written, read back, attended to by single tokens and prompts."""
+  Hkv, Dh, fmt = 8, 128, "mxfp8"
+  pool = (1 << 32) // (Hkv * K.mx_page_bytes(fmt, Dh)) + 9
+  k, v = (torch.empty(pool, Hkv, K.mx_page_bytes(fmt, Dh), dtype=torch.uint8, device=gpu) for _ in range(2))
+  T, H = 70, 16
+  x, cs = qkv_of(T, H, Hkv, Dh), build_cos_sin(Dh, T, 10000.0)
+  pages = torch.tensor([pool - 1, pool - 4])
+  t = torch.arange(T)
+  slots = pages[t // PAGE] * PAGE + t % PAGE
+  q = K.rope_kv_write_mx(x.to(gpu), t.int().to(gpu), cs.to(gpu), slots.to(gpu), k, v, H, Hkv)
+  rows = x.view(T, H + 2 * Hkv, Dh)
+  kw, vw = held(rotated(rows[:, H:H + Hkv], t, cs), fmt), held(rows[:, H + Hkv:], fmt)
+  tables, ctx = pages.int()[None].to(gpu), torch.tensor([T], dtype=torch.int32, device=gpu)
+  kb, vb = K.kv_read_mx(k, v, tables, ctx, Dh)
+  assert torch.equal(kb.cpu().transpose(1, 2).flatten(0, 1)[:T].double(), kw)
+  assert torch.equal(ref.v_chunks(vb.cpu()).transpose(3, 4).flatten(2, 3).transpose(1, 2).flatten(0, 1)[:T].double(), vw)
+  qc = q.cpu()
+  close(K.attn_decode_mx(q[-1:], k, v, tables, ctx, 0.1), *attend64(qc[-1:], kw, vw, 0.1, T - 1))
+  close(K.attn_prefill_mx(q[-9:].contiguous(), k, v, tables, torch.tensor([0, 9], dtype=torch.int32, device=gpu), ctx, 9, 0.1),
+        *attend64(qc[-9:], kw, vw, 0.1, T - 9))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,Dh", [("mxfp4", 128), ("mxfp8", 64)])
+def test_captured_steps_gpu(gpu, fmt, Dh):
+  """A decode step (write, attention in parts) and a prompt's attention in one graph, replayed with new inputs between eager work of the
+  same kind, on a stream of its own; every replay against eager calls."""
+  H, Hkv, B = 8, 2, 3
+  s = Seqs(fmt, [300, 70, 900], Hkv, Dh, dev=gpu, width=16)
+  cs = build_cos_sin(Dh, 1024, 10000.0).to(gpu)
+  g = torch.Generator().manual_seed(0)
+  pos = s.ctx - 1
+  slots = (s.tables.gather(1, (pos // PAGE).long()[:, None])[:, 0].long() * PAGE + pos % PAGE)
+  x = torch.zeros(B, (H + 2 * Hkv) * Dh, dtype=torch.bfloat16, device=gpu)
+  qp = torch.zeros(12, H, Dh, dtype=torch.bfloat16, device=gpu)
+  cu = torch.tensor([0, 5, 6, 12], dtype=torch.int32, device=gpu)
+  ws = K.MXDecodeWorkspace(B, H, Hkv, Dh, 1024, gpu)
+  assert ws.partition(B, 16)[1] > 1
+
+  def step(ws):
+    q = K.rope_kv_write_mx(x, pos, cs, slots, s.k, s.v, H, Hkv)
+    return K.attn_decode_mx(q, s.k, s.v, s.tables, s.ctx, 0.1, ws), K.attn_prefill_mx(qp, s.k, s.v, s.tables, cu, s.ctx, 6, 0.1)
+  stream = torch.cuda.Stream(gpu)
+  stream.wait_stream(torch.cuda.current_stream(gpu))
+  with torch.cuda.stream(stream):
+    step(ws)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+      outs = step(ws)
+  torch.cuda.synchronize()
+  for i in range(5):
+    x.copy_(qkv_of(B, H, Hkv, Dh, i).to(gpu))
+    qp.copy_(torch.randn(qp.shape, generator=g).to(torch.bfloat16))
+    graph.replay()
+    got = [t.clone() for t in outs]
+    torch.cuda.synchronize()
+    for a, b in zip(got, step(K.MXDecodeWorkspace(B, H, Hkv, Dh, 1024, gpu))):
+      assert torch.equal(a, b), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_queries_not_finite_gpu(gpu, fmt):
+  """A query that is not finite makes its own row NaN and no other; zeros weigh all keys alike."""
+  s = Seqs(fmt, [100, 33], 2, 128, dev=gpu)
+  q = torch.randn(2, 8, 128, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
+  q[0, 1, 7], q[1, 6, 100], q[1, 2] = float("nan"), float("inf"), 0.0
+  out = K.attn_decode_mx(q.to(gpu), s.k, s.v, s.tables, s.ctx, 0.1).cpu()
+  bad = torch.zeros(2, 8, dtype=torch.bool)
+  bad[0, 1] = bad[1, 6] = True
+  assert torch.equal(torch.isnan(out).any(-1), bad) and torch.isnan(out[bad]).all()
+  assert torch.allclose(out[1, 2].double(), s.kv[1][1][:, 0].mean(0), rtol=2.0 ** -7, atol=2.0 ** -7)
+  cu = torch.tensor([0, 1, 2], dtype=torch.int32, device=gpu)
+  out = K.attn_prefill_mx(q.to(gpu), s.k, s.v, s.tables, cu, s.ctx, 1, 0.1).cpu()
+  assert torch.equal(torch.isnan(out).any(-1), bad)
+
+
+@pytest.mark.gpu
+def test_nothing_to_do_gpu(gpu):
+  s = Seqs("mxfp4", [70, 5], 2, 128, dev=gpu)
+  none = lambda *shape, dt=torch.bfloat16: torch.zeros(*shape, dtype=dt, device=gpu)  # noqa: E731
+  assert K.attn_decode_mx(none(0, 4, 128), s.k, s.v, none(0, 3, dt=torch.int32), none(0, dt=torch.int32), 1.0).shape == (0, 4, 128)
+  assert K.rope_kv_write_mx(none(0, 8 * 128), none(0, dt=torch.int32), none(9, 128, dt=torch.float32), none(0, dt=torch.int64), s.k, s.v, 4, 2).shape == (0, 4, 128)
+  assert K.kv_read_mx(s.k, s.v, none(0, 3, dt=torch.int32), none(0, dt=torch.int32), 128)[0].shape == (0, 2, 64, 128)
+  out = torch.ones(3, 4, 128, dtype=torch.bfloat16, device=gpu)
+  K.attn_prefill_mx(none(3, 4, 128), s.k, s.v, s.tables, none(3, dt=torch.int32), s.ctx, 0, 1.0, out=out)
+  assert (out == 1).all()
+
+
+@pytest.mark.gpu
 def test_refusals_gpu(gpu):
   s = Seqs("mxfp4", [70, 5], 2, 128, dev=gpu)
   q = torch.zeros(2, 4, 128, dtype=torch.bfloat16, device=gpu)
