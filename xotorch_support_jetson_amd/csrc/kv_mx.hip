@@ -997,19 +997,20 @@ at::Tensor attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const 
 constexpr int PROMPT_WAVES = 4, PROMPT_BLOCKS = 2;  // of 16 rows
 
 // new tokens against the pools: units of 32 rows of (token, head), of four waves that share the pages or one that has them all
-void attn_prompt_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables, const at::Tensor& cu_q,
-                  const at::Tensor& ctx_lens, at::Tensor& out, const c10::optional<at::Tensor>& ws_o, const c10::optional<at::Tensor>& ws_ml,
+at::Tensor attn_prompt_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables, const at::Tensor& cu_q,
+                          const at::Tensor& ctx_lens, const c10::optional<at::Tensor>& out_opt, const c10::optional<at::Tensor>& ws_o, const c10::optional<at::Tensor>& ws_ml,
                   const c10::optional<at::Tensor>& tickets, int64_t max_qlen, int64_t pages_per_part, int64_t nparts, int64_t waves, double scale) {
   const char* op = "attn_prompt_mx";
   XCHECK(q.is_cuda() && q.dim() == 3, op, ": q must be [T, H, Dh] on a GPU");
   const c10::DeviceGuard guard(q.device());
   bool fp8 = false;
+  at::Tensor out = out_opt.has_value() ? *out_opt : at::empty_like(q);
   const int64_t H = q.size(1), Dh = q.size(2), Hkv = k_cache.dim() == 3 ? k_cache.size(1) : 1, B = ctx_lens.numel();
   XCHECK(max_qlen >= 0 && max_qlen < (1 << 24), op, ": max_qlen");
   constexpr int64_t ROWS = 16 * PROMPT_BLOCKS;
   const int64_t blocks = std::max<int64_t>(1, (max_qlen * (H / std::max<int64_t>(Hkv, 1)) + ROWS - 1) / ROWS);
   const AttnArgs a = attn_args(op, fp8, q, k_cache, v_cache, tables, ctx_lens, &cu_q, out, ws_o, ws_ml, tickets, blocks, ROWS, pages_per_part, nparts, scale);
-  if (B == 0 || max_qlen == 0) return;
+  if (B == 0 || max_qlen == 0) return out;
   XCHECK(waves == 1 || waves == PROMPT_WAVES, op, ": 1 or 4 waves");
   const size_t lds = waves == 1 ? 0 : (size_t)PROMPT_WAVES * ROWS * (Dh + 6) * sizeof(float);  // 67 KB at heads of 128
   const unsigned units = (unsigned)(B * blocks * nparts * Hkv);
@@ -1026,6 +1027,7 @@ void attn_prompt_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Te
   } while (0)
   MX_GO(fp8, Dh, GO);
 #undef GO
+  return out;
 }
 
 }  // namespace

@@ -481,7 +481,7 @@ MX_READ_BYTES = 1 << 30
 
 def mx_prompt_units(B: int, max_qlen: int, G: int, Hkv: int) -> int:
   """Units (32 rows of token and head) of a launch over B sequences of at most max_qlen new tokens; those past a sequence's end are empty."""
-  return B * Hkv * max(1, -(-max_qlen * G // 32))
+  return max(1, B) * Hkv * max(1, -(-max_qlen * G // 32))
 
 
 def mx_prompt_direct(B: int, T: int, max_qlen: int, G: int, Hkv: int, Dh: int, fp8: bool) -> bool:
@@ -512,19 +512,18 @@ def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
   T, H, Dh = q.shape
   B, W = block_tables.shape
   Hkv = k_cache.shape[1]
-  out = torch.empty_like(q) if out is None else out
   gpu = _gpu(q)
   G = max(1, H // Hkv)
-  if gpu and mx_prompt_direct(max(B, 1), T, max_qlen, G, Hkv, Dh, k_cache.shape[2] > PAGE * Dh):
-    units = mx_prompt_units(max(B, 1), max_qlen, G, Hkv)
+  if gpu and mx_prompt_direct(B, T, max_qlen, G, Hkv, Dh, k_cache.shape[2] > PAGE * Dh):
+    units = mx_prompt_units(B, max_qlen, G, Hkv)
     nparts = max(1, min(W // 16, 512 // units))
     ws = [None] * 3
     if nparts > 1:  # few rows behind long contexts
       ws = [torch.empty(units * nparts * 32 * n, dtype=torch.float32, device=q.device) for n in (Dh, 2)]
       ws.append(torch.zeros(units, dtype=torch.int32, device=q.device))
-    require().attn_prompt_mx(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, out, *ws, int(max_qlen), -(-W // nparts), nparts,
-                             mx_prompt_waves(units), float(scale))
-    return out
+    return require().attn_prompt_mx(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, out, *ws, int(max_qlen), -(-W // nparts), nparts,
+                                    mx_prompt_waves(units), float(scale))
+  out = torch.empty_like(q) if out is None else out
   per = max(1, min(B, MX_READ_BYTES // max(1, W * Hkv * PAGE * Dh * 4))) if gpu else max(1, B)
   k = torch.empty(per * W, Hkv, PAGE, Dh, dtype=torch.bfloat16, device=q.device)
   v = torch.empty(per * W, Hkv, Dh, PAGE, dtype=torch.bfloat16, device=q.device)
