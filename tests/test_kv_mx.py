@@ -406,8 +406,8 @@ def test_prompt_gpu(gpu, fmt, Dh, H, Hkv, monkeypatch):
   ctx, new = [70, 5, 300, 128, 64, 1], [10, 5, 260, 1, 64, 1]
   s = Seqs(fmt, ctx, Hkv, Dh, dev=gpu, width=6)
   s.spoil()
-  for waves in (4, 1, 0):  # from the pools, and through bf16 pages
-    monkeypatch.setattr(K, "mx_prompt_direct", lambda *a: waves > 0)
+  for waves in (4, 1, 0, -1):  # from the pools, and through bf16 pages
+    monkeypatch.setattr(K, "mx_prompt_direct", lambda *a: waves >= 0)
     monkeypatch.setattr(K, "mx_prompt_waves", lambda *a: waves)
     whole, end = check_prompt(s, new, H, Dh ** -0.5)
     assert (whole[end:] == 7).all()
@@ -436,6 +436,37 @@ def test_turns_gpu(gpu, fmt, Dh, H, Hkv, monkeypatch):
     out = K.attn_prefill_mx(q.to(gpu), s.k, s.v, s.tables, torch.tensor([0, 5, 7], dtype=torch.int32, device=gpu), s.ctx, 5, Dh ** -0.5)
     close(out[2:5], *attend64(q[2:5], *s.kv[0], Dh ** -0.5, 0))
     assert (out[:2] == 0).all() and (out[5:] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,Dh,H,Hkv", [("mxfp4", 128, 4, 1), ("mxfp8", 128, 16, 1), ("mxfp4", 64, 7, 1), ("mxfp8", 64, 3, 3)])
+def test_prompts_in_lds_gpu(gpu, fmt, Dh, H, Hkv, monkeypatch):
+  """The kernel of four units: one page to many, waves without rows or without keys, tokens before the first key, a replayed result."""
+  monkeypatch.setattr(K, "mx_prompt_waves", lambda *a: 0)
+  s = Seqs(fmt, [1000, 470, 33, 64, 1, 129, 200], Hkv, Dh, dev=gpu, width=16)  # (16: in one part)
+  s.spoil()
+  a, end = check_prompt(s, [1000, 17, 0, 64, 1, 129, 5], H, Dh ** -0.5)
+  assert (a[end:] == 7).all()
+  assert torch.equal(a, check_prompt(s, [1000, 17, 0, 64, 1, 129, 5], H, Dh ** -0.5)[0])
+  s = Seqs(fmt, [3, 0, 100], Hkv, Dh, dev=gpu)
+  q = torch.randn(210, H, Dh, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+  out = K.attn_prefill_mx(q.to(gpu), s.k, s.v, s.tables, torch.tensor([0, 5, 7, 210], dtype=torch.int32, device=gpu), s.ctx, 203, Dh ** -0.5)
+  close(out[2:5], *attend64(q[2:5], *s.kv[0], Dh ** -0.5, 0))
+  close(out[110:], *attend64(q[110:], *s.kv[2], Dh ** -0.5, 0))
+  assert (out[:2] == 0).all() and (out[5:110] == 0).all()
+
+
+@pytest.mark.gpu
+def test_prompts_of_many_sequences_gpu(gpu):
+  """More sequences than a grid dimension holds: few unlike ones over and over."""
+  s = Seqs("mxfp4", [70, 1, 64, 130, 0], 1, 64, dev=gpu)
+  n, H = 14000, 2
+  q = torch.randn(5, H, 64, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
+  cu = torch.arange(5 * n + 1, dtype=torch.int32, device=gpu)
+  out = K.attn_prefill_mx(q.to(gpu).repeat(n, 1, 1), s.k, s.v, s.tables.repeat(n, 1), cu, s.ctx.repeat(n), 1, 0.125).view(n, 5, H, 64)
+  assert (out == out[:1]).all() and (out[0, 4] == 0).all()
+  for b in range(4):
+    close(out[0, b:b + 1], *attend64(q[b:b + 1], *s.kv[b], 0.125, s.lens[b] - 1))
 
 
 @pytest.mark.gpu

@@ -409,6 +409,25 @@ __device__ __forceinline__ void cut_values(V& v, S& vs, int left) {  // u32x4 [V
   }
 }
 
+// group j of a lane's eight keys: the A operands of O^T's tiles (j, even dims) and (j, odd)
+template <int DH, bool FP8, class V, class S>
+__device__ __forceinline__ void value_pairs(const V& v, const S& vs, int j, u32x4& ae, u32x4& ao) {  // u32x4 [VU], [VS]
+  using M = Mx<DH, FP8>;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    uint32_t y[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int key = 2 * n + i, at = key * M::NB + (FP8 ? 2 * j : j), sa = key * M::J + j;  // bytes among the eight keys'
+      const uint32_t w = v[at >> 4][(at >> 2) & 3];
+      const float s = scale_of(vs[sa >> 4][(sa >> 2) & 3], sa & 3);
+      y[i] = FP8 ? from_fp8(w, s, (at >> 1) & 1) : from_fp4(w, s, at & 3);
+    }
+    ae[n] = low_halves(y[0], y[1]);
+    ao[n] = high_halves(y[0], y[1]);
+  }
+}
+
 // A wave's 16 NB rows (queries) and what it has of them.  ONES: the weights are summed as products with ones, which costs registers and
 // saves vector operations.
 template <int DH, bool FP8, int NB, bool ONES>
@@ -485,10 +504,8 @@ struct Rows {
 #pragma unroll
       for (int r = 0; r < 4; ++r) st[t][r] = 32 * (t >> 1) + 4 * (t & 1) + r < left ? st[t][r] : -INFINITY;
   }
-  // The page's weights and their products with its values; vv(kk, v, vs): eight keys' units and scales.
-  template <class V>
-  __device__ __forceinline__ void weigh(V vv, const f32x4 (&st)[NB][4], float scale_log2) {
-    s16x8 pf[NB][2];
+  // The page's weights in bf16, B operands of the products with its values; what the rows have so far is brought to the new maxima.
+  __device__ __forceinline__ void weights(const f32x4 (&st)[NB][4], float scale_log2, s16x8 (&pf)[NB][2]) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       float mx = -INFINITY;
@@ -525,6 +542,12 @@ struct Rows {
         if constexpr (ONES) lacc[nb] = mfma16(s16x8{ONE, ONE, ONE, ONE, ONE, ONE, ONE, ONE}, pf[nb][kk], lacc[nb]);
       }
     }
+  }
+  // The page's weights and their products with its values; vv(kk, v, vs): eight keys' units and scales.
+  template <class V>
+  __device__ __forceinline__ void weigh(V vv, const f32x4 (&st)[NB][4], float scale_log2) {
+    s16x8 pf[NB][2];
+    weights(st, scale_log2, pf);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       u32x4 v[R::VU], vs[R::VS];
@@ -532,19 +555,7 @@ struct Rows {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         u32x4 ae, ao;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          uint32_t y[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int key = 2 * n + i, at = key * M::NB + (FP8 ? 2 * j : j), sa = key * J + j;  // bytes among the eight keys'
-            const uint32_t w = v[at >> 4][(at >> 2) & 3];
-            const float s = scale_of(vs[sa >> 4][(sa >> 2) & 3], sa & 3);
-            y[i] = FP8 ? from_fp8(w, s, (at >> 1) & 1) : from_fp4(w, s, at & 3);
-          }
-          ae[n] = low_halves(y[0], y[1]);
-          ao[n] = high_halves(y[0], y[1]);
-        }
+        value_pairs<DH, FP8>(v, vs, j, ae, ao);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           o[nb][j][0] = mfma16(__builtin_bit_cast(s16x8, ae), pf[nb][kk], o[nb][j][0]);
@@ -584,12 +595,12 @@ struct Rows {
 // us (6.5 TB/s), mxfp4 856 MB in 138 us (6.2 TB/s); of 525 tokens, 64 heads, mxfp4 56 us (5.2 TB/s of what counts).  A page of mxfp4 is
 // about 330 vector operations a wave, 190 of them making bf16 values; K needs none.  Uncut contexts and no loads ahead: 8 sequences of
 // 32000 tokens 239 us, now 48.
-// Prompts are bound by the vector unit: a page of 32 rows is 64 matrix instructions (1100 cycles) and 400 vector operations (1600, and the
-// exponentials' 400 more).  4096 tokens of 32 heads of 128 on 8, mxfp4, in units of one wave: 158 us, 868 TFLOP/s (the bf16 kernel behind
-// kv_read_mx 164); mxfp8 195 (no refilling; 164).  Pages through LDS, shared by four waves of 32 rows each: 172, 178.  Units start with the
-// last rows, which see the most keys.
+// Prompts (PROMPT) start with their last rows, which see the most keys.  In units of one wave they are bound by the vector unit: a page of 32
+// rows is 64 matrix instructions (1100 cycles) and 400 vector operations (1600, and the exponentials' 400 more).  4096 tokens of 32 heads of
+// 128 on 8, mxfp4: 158 us, 868 TFLOP/s.
+// Bounds: four waves a SIMD where the registers suffice (single tokens of mxfp4, 128 dims: 54 us at 512 of 525 keys, 61 in three).
 template <int DH, bool FP8, int NW, int NB, bool PROMPT, bool REFILL>
-__global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : 3) void attn_mx_kernel(const AttnArgs A) {
+__global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : FP8 || REFILL || PROMPT ? 3 : 4) void attn_mx_kernel(const AttnArgs A) {
   static_assert(PROMPT || NB == 1, "a single token's heads are one column block");
   using M = Mx<DH, FP8>;
   using R = PageRegs<DH, FP8>;
@@ -796,6 +807,178 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : 3) void attn_mx_
   }
 }
 
+// ============================================================================ attention of prompts
+// 128 rows (token, head) of a (sequence, KV head) a workgroup, 32 a wave.  The pages they see pass through LDS: the keys as the cache holds
+// them, their rows' 16-byte pieces exchanged so that the 16 rows of a score tile lie in 16 different pieces of 256 bytes (mx_swizzle; the
+// loads' source addresses do it), the values made bf16 by the four waves together, once for all their rows: half of the vector
+// operations of a unit that makes them for its own 32.  One barrier a page: behind it page p's values are there and page p + 1 has landed,
+// page p + 1 + AHEAD is asked for, the values of p + 1 are made, page p is computed.
+// 4096 tokens of 32 heads on 8: heads of 64, mxfp4 98 us (705 TFLOP/s; 109 in units of one wave, 120 by the bf16 kernel behind kv_read_mx), mxfp8 of
+// 128 174 (195; 164), mxfp4 167 (158; 164).  The matrix instructions (1100 cycles a page and wave) and the vector ones (1450) do not overlap as
+// two waves a SIMD let hope; three a SIMD, and weaving the next page's scores between the exponentials, cost registers and were slower.
+template <int DH, bool FP8>
+struct PromptLds {
+  using M = Mx<DH, FP8>;
+  static constexpr int AHEAD = FP8 && DH == 128 ? 1 : 2;     // pages in flight (two workgroups a CU: 80 KB each)
+  static constexpr int KG = M::BYTES / 16;                   // pieces of a page's keys, and of its values
+  static constexpr int NCH = (KG + 63) / 64;                 // loads of 64 pieces (1 KB of LDS) that hold them
+  static constexpr int N = (2 * NCH + 3) / 4;                // loads a wave and page
+  static constexpr int RAW = NCH * 1024;
+  static constexpr int VBUF = PAGE * DH * 2;                 // values in bf16: [half of the keys][group][even / odd][eight keys][16 dims][8]
+  static constexpr int K0 = 0, V0 = (AHEAD + 2) * RAW, B0 = V0 + (AHEAD + 1) * RAW, TOTAL = B0 + 2 * VBUF;
+};
+// which pieces of row r change places: x of its piece r (row / 16) + i becomes that number ^ x
+template <int DH, bool FP8>
+__device__ __forceinline__ int mx_swizzle(int r) {
+  constexpr int RG = Mx<DH, FP8>::ROW / 16;
+  const int q = (r >> 3) & 3;
+  return RG == 8 ? 2 * q + ((r >> 1) & 1) : RG == 4 ? q : (q & 1) | (q & 2) << 2;
+}
+
+template <int DH, bool FP8>
+__global__ __launch_bounds__(256, 2) void attn_prompt_mx_kernel(const AttnArgs A) {
+  using M = Mx<DH, FP8>;
+  using R = PageRegs<DH, FP8>;
+  using L = PromptLds<DH, FP8>;
+  constexpr int J = M::J, NB = 2, RG = M::ROW / 16, AHEAD = L::AHEAD;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const PromptWork work = prompt_work(A.ctx_lens);
+  const int b = __builtin_amdgcn_readfirstlane(work.seq), kvh = work.head, row0 = work.tile * 128;
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, G = A.H / A.Hkv;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int q0 = min(max(A.cu_q[b], 0), A.T), qlen = min(max(A.cu_q[b + 1], q0), A.T) - q0, nrows = qlen * G;
+  if (row0 >= nrows) return;  // the whole workgroup
+  const int ctx = min(max(A.ctx_lens[b], 0), A.width * PAGE), pos0 = ctx - qlen;  // pos0: keys before the new tokens
+  const int pages = (max(0, pos0 + (min(row0 + 128, nrows) - 1) / G + 1) + PAGE - 1) / PAGE;
+  const int wrow0 = row0 + 32 * wave, wend = min(wrow0 + 32, nrows);
+  const int wmin = pos0 + wrow0 / G, wmax = wend > wrow0 ? pos0 + (wend - 1) / G : -1;  // last keys of the wave's first and last rows
+
+  // this lane's pieces of a page: load i of the wave brings chunk ch of the keys' or (from NCH on) the values' bytes
+  int from[L::N], chunk[L::N];
+#pragma unroll
+  for (int i = 0; i < L::N; ++i) {
+    chunk[i] = min(L::N * wave + i, 2 * L::NCH - 1);  // (one too many: the last again)
+    const bool v = chunk[i] >= L::NCH;
+    const int at = min(64 * (v ? chunk[i] - L::NCH : chunk[i]) + lane, L::KG - 1);  // (past the page: its last piece again)
+    from[i] = 16 * (v || at >= M::ELEMS / 16 ? at : at ^ mx_swizzle<DH, FP8>(at / RG));
+  }
+  // the table's entries as scalar loads, one page ahead of the loads that need them (a vector load there would be waited for behind the
+  // pages in flight)
+  typedef const __attribute__((address_space(4))) int32_t* table_t;
+  const table_t bt = (table_t)(uintptr_t)(A.tables + (size_t)b * A.width);
+  auto page_of = [&](int p) -> int { return min(max(bt[min(p, pages - 1)], 0), A.num_pages - 1); };  // (pages > 0)
+  auto issue = [&](int p, long page) {
+    const uint8_t* kp = A.kc + ((size_t)page * A.Hkv + kvh) * M::BYTES;
+    const uint8_t* vp = A.vc + ((size_t)page * A.Hkv + kvh) * M::BYTES;
+    uint8_t* kd = lds + L::K0 + p % (AHEAD + 2) * L::RAW;
+    uint8_t* vd = lds + L::V0 + p % (AHEAD + 1) * L::RAW;
+#pragma unroll
+    for (int i = 0; i < L::N; ++i) {
+      const bool v = chunk[i] >= L::NCH;
+      __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)((v ? vp : kp) + (uint32_t)from[i]),
+                                       (__attribute__((address_space(3))) void*)((v ? vd - L::NCH * 1024 : kd) + chunk[i] * 1024), 16, 0, 0);
+    }
+  };
+  // values of page p, landed, into bf16: the wave takes four octets of keys (lane group: octet) of some groups of dims
+  auto make_values = [&](int p) {
+    const uint8_t* raw = lds + L::V0 + p % (AHEAD + 1) * L::RAW;
+    uint8_t* to = lds + L::B0 + (p & 1) * L::VBUF;
+    const int oct = 4 * (wave & 1) + g, left = ctx - p * PAGE - 8 * oct;
+    u32x4 v[R::VU], vs[R::VS];
+#pragma unroll
+    for (int u = 0; u < R::VU; ++u) v[u] = *reinterpret_cast<const u32x4*>(raw + (8 * oct / M::KC + u) * 256 + 16 * c);
+#pragma unroll
+    for (int u = 0; u < R::VS; ++u) vs[u] = *reinterpret_cast<const u32x4*>(raw + M::ELEMS + 8 * oct * J + 16 * u);
+    if (ctx - p * PAGE < PAGE) cut_values<DH, FP8>(v, vs, left);
+    auto group = [&](auto jc) {
+      constexpr int j = decltype(jc)::value;
+      u32x4 ae, ao;
+      value_pairs<DH, FP8>(v, vs, j, ae, ao);
+      uint8_t* t = to + ((oct >> 2) * J + j) * 2048 + (oct & 3) * 256 + 16 * c;
+      *reinterpret_cast<u32x4*>(t) = ae;
+      *reinterpret_cast<u32x4*>(t + 1024) = ao;
+    };
+    if (wave < 2) {
+      group(std::integral_constant<int, 0>{});
+      if constexpr (J == 4) group(std::integral_constant<int, 1>{});
+    } else {
+      group(std::integral_constant<int, J / 2>{});
+      if constexpr (J == 4) group(std::integral_constant<int, 3>{});
+    }
+  };
+  auto meet = [] {  // LDS of this wave done, all waves here
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+
+#pragma unroll
+  for (int p = 0; p <= AHEAD; ++p)
+    if (p < pages) issue(p, page_of(p));
+  Rows<DH, FP8, NB, true> rows;
+  int sees[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int row = min(wrow0 + 16 * nb + c, nrows - 1), ti = row / G;
+    sees[nb] = pos0 + ti;
+    rows.query(nb, A.q + ((size_t)(q0 + ti) * A.H + kvh * G + row - ti * G) * DH + 16 * g, wrow0 + 16 * nb + c < nrows, g);
+  }
+  int nxt = pages > AHEAD + 1 ? page_of(AHEAD + 1) : 0;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the queries came behind the first pages)
+  meet();
+  if (pages > 0) make_values(0);
+  for (int p = 0; p < pages; ++p) {
+    if (AHEAD > 1 && p + AHEAD < pages)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * L::N) : "memory");  // this wave's share of page p + 1 has landed
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    meet();
+    if (p + 1 + AHEAD < pages) {
+      issue(p + 1 + AHEAD, nxt);
+      nxt = page_of(p + 2 + AHEAD);
+    }
+    if (p + 1 < pages) make_values(p + 1);
+    if (p * PAGE > wmax) continue;  // every row of this wave is before the page
+    const uint8_t* kr = lds + L::K0 + p % (AHEAD + 2) * L::RAW;
+    const uint8_t* vb = lds + L::B0 + (p & 1) * L::VBUF;
+    f32x4 st[NB][4];
+    rows.scores([&](int t, u32x4 (&k)[R::KV]) {
+      const int r = 32 * (t >> 1) + 4 * (t & 1) + 8 * (c >> 2) + (c & 3);
+#pragma unroll
+      for (int i = 0; i < R::KV; ++i)
+        k[i] = *reinterpret_cast<const u32x4*>(kr + 16 * ((r * RG + (DH == 64 && !FP8 ? g & 1 : g) + 4 * i) ^ mx_swizzle<DH, FP8>(r)));
+    }, *reinterpret_cast<const uint32_t*>(kr + M::ELEMS + 64 * (g & (J - 1)) + 4 * c), st);
+    if (wmin + 1 - p * PAGE < PAGE) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) rows.mask(st[nb], sees[nb] + 1 - p * PAGE - 8 * g);
+    }
+    s16x8 pf[NB][2];
+    rows.weights(st, A.scale_log2, pf);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const s16x8 v = ld16(vb + ((kk * J + j) * 2 + e) * 1024 + g * 256 + 16 * c);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) rows.o[nb][j][e] = mfma16(v, pf[nb][kk], rows.o[nb][j][e]);
+        }
+  }
+  rows.finish();
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int row = wrow0 + 16 * nb + c, ti = row / G;
+    if (row >= nrows) continue;
+    const float inv = pos0 + ti >= 0 ? 1.f / rows.l[nb] : 0.f;  // a row without keys: zeros (its sums are)
+    uint16_t* p = A.out + ((size_t)(q0 + ti) * A.H + kvh * G + row - ti * G) * DH + 8 * g;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) st_results(p + 32 * j + 4 * half, rows.dims(nb, j, half), inv);
+  }
+}
+
 // ============================================================================ bindings
 #define XCHECK(cond, ...) TORCH_CHECK(cond, "xot kernel: ", __VA_ARGS__)
 inline hipStream_t stream() { return at::hip::getCurrentHIPStream().stream(); }
@@ -996,7 +1179,8 @@ at::Tensor attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const 
 
 constexpr int PROMPT_WAVES = 4, PROMPT_BLOCKS = 2;  // of 16 rows
 
-// new tokens against the pools: units of 32 rows of (token, head), of four waves that share the pages or one that has them all
+// new tokens against the pools: units of 32 rows of (token, head), of four waves that share the pages or one that has them all; or (waves 0)
+// attn_prompt_mx_kernel's of 128
 at::Tensor attn_prompt_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables, const at::Tensor& cu_q,
                           const at::Tensor& ctx_lens, const c10::optional<at::Tensor>& out_opt, const c10::optional<at::Tensor>& ws_o, const c10::optional<at::Tensor>& ws_ml,
                   const c10::optional<at::Tensor>& tickets, int64_t max_qlen, int64_t pages_per_part, int64_t nparts, int64_t waves, double scale) {
@@ -1011,12 +1195,28 @@ at::Tensor attn_prompt_mx(const at::Tensor& q, const at::Tensor& k_cache, const 
   const int64_t blocks = std::max<int64_t>(1, (max_qlen * (H / std::max<int64_t>(Hkv, 1)) + ROWS - 1) / ROWS);
   const AttnArgs a = attn_args(op, fp8, q, k_cache, v_cache, tables, ctx_lens, &cu_q, out, ws_o, ws_ml, tickets, blocks, ROWS, pages_per_part, nparts, scale);
   if (B == 0 || max_qlen == 0) return out;
-  XCHECK(waves == 1 || waves == PROMPT_WAVES, op, ": 1 or 4 waves");
-  const size_t lds = waves == 1 ? 0 : (size_t)PROMPT_WAVES * ROWS * (Dh + 6) * sizeof(float);  // 67 KB at heads of 128
+  XCHECK(waves == 0 || waves == 1 || waves == PROMPT_WAVES, op, ": 1 or 4 waves, or 0");
+  XCHECK(waves != 0 || nparts == 1, op, ": parts are of units of 1 or 4 waves");
+  if (waves == 0 && Hkv < 65536 && B < 65536) {  // (the grid's limits)
+    const int64_t tiles = (blocks * ROWS + 127) / 128;
+    const dim3 grid((unsigned)tiles, (unsigned)Hkv, (unsigned)B);
+#define GO(DHV, F)                                                                                                                         \
+  do {                                                                                                                                     \
+    auto* f = attn_prompt_mx_kernel<DHV, F>;                                                                                               \
+    constexpr int lds = PromptLds<DHV, F>::TOTAL;                                                                                          \
+    static const hipError_t set = hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, lds);                    \
+    XCHECK(set == hipSuccess, op, ": LDS");                                                                                                \
+    f<<<grid, 256, lds, stream()>>>(a);                                                                                                    \
+  } while (0)
+    MX_GO(fp8, Dh, GO);
+#undef GO
+    return out;
+  }
+  const size_t lds = waves < PROMPT_WAVES ? 0 : (size_t)PROMPT_WAVES * ROWS * (Dh + 6) * sizeof(float);  // 67 KB at heads of 128
   const unsigned units = (unsigned)(B * blocks * nparts * Hkv);
 #define GO(DHV, F)                                                                                                                         \
   do {                                                                                                                                     \
-    if (waves == 1) {                                                                                                                      \
+    if (waves < PROMPT_WAVES) {                                                                                                            \
       attn_mx_kernel<DHV, F, 1, PROMPT_BLOCKS, true, !(F && DHV == 128)><<<units, 64, 0, stream()>>>(a);                                     \
       break;                                                                                                                               \
     }                                                                                                                                      \
