@@ -406,9 +406,9 @@ def test_prompt_gpu(gpu, fmt, Dh, H, Hkv, monkeypatch):
   ctx, new = [70, 5, 300, 128, 64, 1], [10, 5, 260, 1, 64, 1]
   s = Seqs(fmt, ctx, Hkv, Dh, dev=gpu, width=6)
   s.spoil()
-  for waves in (4, 1, 0, -1):  # from the pools, and through bf16 pages
-    monkeypatch.setattr(K, "mx_prompt_direct", lambda *a: waves >= 0)
-    monkeypatch.setattr(K, "mx_prompt_waves", lambda *a: waves)
+  for direct, tiles in ((True, False), (True, True), (False, False)):  # from the pools, and through bf16 pages
+    monkeypatch.setattr(K, "mx_prompt_direct", lambda *a: direct)
+    monkeypatch.setattr(K, "mx_prompt_tiles", lambda *a: tiles)
     whole, end = check_prompt(s, new, H, Dh ** -0.5)
     assert (whole[end:] == 7).all()
   for limit in (1, 2 * 6 * Hkv * PAGE * Dh * 4):  # a sequence, two sequences at a time
@@ -423,12 +423,10 @@ def test_turns_gpu(gpu, fmt, Dh, H, Hkv, monkeypatch):
   s = Seqs(fmt, [1500, 2200, 33, 64, 1, 700], Hkv, Dh, dev=gpu, width=36)
   s.spoil()
   new = [3, 17, 0, 5, 1, 16]
-  for waves in (4, 1):
-    monkeypatch.setattr(K, "mx_prompt_waves", lambda *a: waves)
-    a, end = check_prompt(s, new, H, Dh ** -0.5)
-    assert (a[end:] == 7).all()
-    for _ in range(3):
-      assert torch.equal(a, check_prompt(s, new, H, Dh ** -0.5)[0])
+  a, end = check_prompt(s, new, H, Dh ** -0.5)
+  assert (a[end:] == 7).all()
+  for _ in range(3):
+    assert torch.equal(a, check_prompt(s, new, H, Dh ** -0.5)[0])
   s = Seqs(fmt, [3, 0], Hkv, Dh, dev=gpu)  # (rows before the first key: zeros, as in attn_prefill)
   for direct in (True, False):
     monkeypatch.setattr(K, "mx_prompt_direct", lambda *a: direct)
@@ -442,7 +440,7 @@ def test_turns_gpu(gpu, fmt, Dh, H, Hkv, monkeypatch):
 @pytest.mark.parametrize("fmt,Dh,H,Hkv", [("mxfp4", 128, 4, 1), ("mxfp8", 128, 16, 1), ("mxfp4", 64, 7, 1), ("mxfp8", 64, 3, 3)])
 def test_prompts_in_lds_gpu(gpu, fmt, Dh, H, Hkv, monkeypatch):
   """The kernel of four units: one page to many, waves without rows or without keys, tokens before the first key, a replayed result."""
-  monkeypatch.setattr(K, "mx_prompt_waves", lambda *a: 0)
+  monkeypatch.setattr(K, "mx_prompt_tiles", lambda *a: True)
   s = Seqs(fmt, [1000, 470, 33, 64, 1, 129, 200], Hkv, Dh, dev=gpu, width=16)  # (16: in one part)
   s.spoil()
   a, end = check_prompt(s, [1000, 17, 0, 64, 1, 129, 5], H, Dh ** -0.5)
@@ -454,6 +452,35 @@ def test_prompts_in_lds_gpu(gpu, fmt, Dh, H, Hkv, monkeypatch):
   close(out[2:5], *attend64(q[2:5], *s.kv[0], Dh ** -0.5, 0))
   close(out[110:], *attend64(q[110:], *s.kv[2], Dh ** -0.5, 0))
   assert (out[:2] == 0).all() and (out[5:110] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,Dh", [("mxfp4", 128), ("mxfp8", 64)])
+def test_rising_scores_gpu(gpu, fmt, Dh, monkeypatch):
+  """Scores that rise along the context, slowly, fast, then fall: weights against a maximum that is behind."""
+  H, Hkv, n = 4, 2, 700
+  s = Seqs(fmt, [n, 333], Hkv, Dh, dev=gpu)
+  c = torch.randint(0, 2, (Dh,), generator=torch.Generator().manual_seed(0)) * 2.0 - 1
+  t = torch.arange(n).float()
+  rise = torch.where(t < 400, t / 100, torch.where(t < 600, 4 + (t - 400) / 8, 29 - (t - 600) / 16))  # scores in powers of e, at q = c
+  s.kv = []
+  for b, m in enumerate(s.lens):
+    v = torch.randn(m, Hkv, Dh, generator=torch.Generator().manual_seed(b))
+    k = (rise[:m, None, None] * c).expand(m, Hkv, Dh)
+    at = s.tables[b].cpu().long()[torch.arange(m) // PAGE] * PAGE + torch.arange(m) % PAGE
+    kc, vc = s.k.cpu(), s.v.cpu()
+    ref.mx_write(k, v, at, kc, vc)
+    s.k, s.v = kc.to(gpu), vc.to(gpu)
+    s.kv.append((held(k, fmt), held(v, fmt)))
+  q = (c + 0.05 * torch.randn(n + 333, H, Dh, generator=torch.Generator().manual_seed(9))).to(torch.bfloat16)
+  out = K.attn_decode_mx(q[:2].to(gpu), s.k, s.v, s.tables, s.ctx, 1 / Dh)
+  for b, m in enumerate(s.lens):
+    close(out[b:b + 1], *attend64(q[b:b + 1], *s.kv[b], 1 / Dh, m - 1))
+  for tiles in (True, False):
+    monkeypatch.setattr(K, "mx_prompt_tiles", lambda *a: tiles)
+    out = K.attn_prefill_mx(q.to(gpu), s.k, s.v, s.tables, torch.tensor([0, n, n + 333], dtype=torch.int32, device=gpu), s.ctx, n, 1 / Dh)
+    for a, m, kv in ((0, n, s.kv[0]), (n, 333, s.kv[1])):
+      close(out[a:a + m], *attend64(q[a:a + m], *kv, 1 / Dh, 0))
 
 
 @pytest.mark.gpu

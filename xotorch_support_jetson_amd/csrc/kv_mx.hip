@@ -435,6 +435,9 @@ struct Rows {
   using M = Mx<DH, FP8>;
   using R = PageRegs<DH, FP8>;
   static constexpr int J = M::J;
+  // A row's weights are 2^(score - m).  m follows the largest score only once that is past it by more than this: weights stay below 2^8, sums far
+  // from overflow, and what the rows have is brought to a new m a few times, not at every second page (4096 tokens 158 -> 150 us).
+  static constexpr float LAZY = 8.f;
   i32x8 qhi[NB], qlo[NB];
   int shi[NB], slo[NB];
   float m[NB], l[NB];
@@ -512,13 +515,12 @@ struct Rows {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[nb][t][r]);
+        for (int r = 0; r < 4; ++r) mx = __builtin_elementwise_maximum(mx, st[nb][t][r]);
       mx = xor_max<16>(mx);
-      mx = xor_max<32>(mx);
-      const float mn = fmaxf(m[nb], mx * scale_log2);  // (the scale is positive)
-      const float alpha = __builtin_amdgcn_exp2f(m[nb] - mn);
-      m[nb] = mn;
-      if (__ballot(alpha != 1.f)) {  // a row's maximum moved
+      mx = xor_max<32>(mx) * scale_log2;  // (the scale is positive)
+      if (__ballot(mx > m[nb] + LAZY)) {
+        const float mn = fmaxf(m[nb], mx), alpha = __builtin_amdgcn_exp2f(m[nb] - mn);
+        m[nb] = mn;
         if constexpr (ONES) lacc[nb] *= alpha;
         else l[nb] *= alpha;
 #pragma unroll
@@ -532,8 +534,8 @@ struct Rows {
         u32x4 pw;
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(st[nb][2 * kk + (e >> 2)][e & 3], scale_log2, -mn));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(st[nb][2 * kk + (e >> 2)][(e & 3) + 1], scale_log2, -mn));
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(st[nb][2 * kk + (e >> 2)][e & 3], scale_log2, -m[nb]));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(st[nb][2 * kk + (e >> 2)][(e & 3) + 1], scale_log2, -m[nb]));
           if constexpr (!ONES) l[nb] += p0 + p1;
           pw[e >> 1] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p0, p1}), bf16x2_t));
         }
@@ -595,9 +597,8 @@ struct Rows {
 // us (6.5 TB/s), mxfp4 856 MB in 138 us (6.2 TB/s); of 525 tokens, 64 heads, mxfp4 56 us (5.2 TB/s of what counts).  A page of mxfp4 is
 // about 330 vector operations a wave, 190 of them making bf16 values; K needs none.  Uncut contexts and no loads ahead: 8 sequences of
 // 32000 tokens 239 us, now 48.
-// Prompts (PROMPT) start with their last rows, which see the most keys.  In units of one wave they are bound by the vector unit: a page of 32
-// rows is 64 matrix instructions (1100 cycles) and 400 vector operations (1600, and the exponentials' 400 more).  4096 tokens of 32 heads of
-// 128 on 8, mxfp4: 158 us, 868 TFLOP/s.
+// Prompts (PROMPT) start with their last rows, which see the most keys; here where they are few (attn_prompt_mx_kernel): 4 sequences of 64 new
+// tokens behind 1000, 32 heads of 128 on 8, mxfp4, 15 us.
 // Bounds: four waves a SIMD where the registers suffice (single tokens of mxfp4, 128 dims: 54 us at 512 of 525 keys, 61 in three).
 template <int DH, bool FP8, int NW, int NB, bool PROMPT, bool REFILL>
 __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : FP8 || REFILL || PROMPT ? 3 : 4) void attn_mx_kernel(const AttnArgs A) {
@@ -808,21 +809,25 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : FP8 || REFILL ||
 }
 
 // ============================================================================ attention of prompts
-// 128 rows (token, head) of a (sequence, KV head) a workgroup, 32 a wave.  The pages they see pass through LDS: the keys as the cache holds
-// them, their rows' 16-byte pieces exchanged so that the 16 rows of a score tile lie in 16 different pieces of 256 bytes (mx_swizzle; the
-// loads' source addresses do it), the values made bf16 by the four waves together, once for all their rows: half of the vector
-// operations of a unit that makes them for its own 32.  One barrier a page: behind it page p's values are there and page p + 1 has landed,
-// page p + 1 + AHEAD is asked for, the values of p + 1 are made, page p is computed.
-// 4096 tokens of 32 heads on 8: heads of 64, mxfp4 98 us (705 TFLOP/s; 109 in units of one wave, 120 by the bf16 kernel behind kv_read_mx), mxfp8 of
-// 128 174 (195; 164), mxfp4 167 (158; 164).  The matrix instructions (1100 cycles a page and wave) and the vector ones (1450) do not overlap as
-// two waves a SIMD let hope; three a SIMD, and weaving the next page's scores between the exponentials, cost registers and were slower.
+// 128 rows (token, head) of a (sequence, KV head) a workgroup: eight waves of 16, or four of 32 for heads of 64 (two workgroups a CU, three or
+// four).  The pages they see pass through LDS: the keys as the cache holds them, their rows' 16-byte pieces exchanged so that the 16 rows of a
+// score tile lie in 16 different pieces of 256 bytes (mx_swizzle; the loads' source addresses do it), the values made bf16 by the waves
+// together, once for all their rows.  One barrier a page: behind it page p's values are there and page p + 1 has landed, page p + 1 + AHEAD is
+// asked for, the values of p + 1 are made, page p is computed.
+// Bound by the vector unit and the waits for each other: 32 rows of a page are 1100 cycles of matrix instructions and 1300 of vector ones
+// (512 of them exponentials'), which overlap in part (46 % and 59 % busy; LDS 44 %).  One prompt, 32 heads on 8: of 128 dims, mxfp4, 4096
+// tokens 150 us (900 TFLOP/s), 8192 535 (1030), mxfp8 164 and 598; of 64 dims 93 and 305, 95 and 344; the bf16 kernel behind kv_read_mx 165
+// and 577, 165 and 583, 121 and 421, 120 and 422.  us of others, 4096 of 128 dims, mxfp4 / mxfp8: units of one wave that make their own values
+// 149 / 192 (12 prompts of 512 62 / 68, here 56 / 59), four waves of 32 rows 158 / 164, half of the waves making values behind their products
+// instead of before 156 / 171, six waves of 32 rows 244; mxfp4 of 64 dims eight waves of 16 rows 92, 12 prompts of 512 37 (36).
 template <int DH, bool FP8>
 struct PromptLds {
   using M = Mx<DH, FP8>;
-  static constexpr int AHEAD = FP8 && DH == 128 ? 1 : 2;     // pages in flight (two workgroups a CU: 80 KB each)
+  static constexpr int NB = DH == 128 ? 1 : 2, NW = 8 / NB;   // blocks of 16 rows of a wave, waves: four a SIMD and two
+  static constexpr int AHEAD = FP8 && DH == 128 ? 1 : 2;     // pages in flight (two workgroups a CU have 80 KB each)
   static constexpr int KG = M::BYTES / 16;                   // pieces of a page's keys, and of its values
   static constexpr int NCH = (KG + 63) / 64;                 // loads of 64 pieces (1 KB of LDS) that hold them
-  static constexpr int N = (2 * NCH + 3) / 4;                // loads a wave and page
+  static constexpr int N = (2 * NCH + NW - 1) / NW;                // loads a wave and page
   static constexpr int RAW = NCH * 1024;
   static constexpr int VBUF = PAGE * DH * 2;                 // values in bf16: [half of the keys][group][even / odd][eight keys][16 dims][8]
   static constexpr int K0 = 0, V0 = (AHEAD + 2) * RAW, B0 = V0 + (AHEAD + 1) * RAW, TOTAL = B0 + 2 * VBUF;
@@ -836,11 +841,11 @@ __device__ __forceinline__ int mx_swizzle(int r) {
 }
 
 template <int DH, bool FP8>
-__global__ __launch_bounds__(256, 2) void attn_prompt_mx_kernel(const AttnArgs A) {
+__global__ __launch_bounds__(DH == 128 ? 512 : 256, 4) void attn_prompt_mx_kernel(const AttnArgs A) {
   using M = Mx<DH, FP8>;
   using R = PageRegs<DH, FP8>;
   using L = PromptLds<DH, FP8>;
-  constexpr int J = M::J, NB = 2, RG = M::ROW / 16, AHEAD = L::AHEAD;
+  constexpr int J = M::J, NB = L::NB, RG = M::ROW / 16, AHEAD = L::AHEAD;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const PromptWork work = prompt_work(A.ctx_lens);
   const int b = __builtin_amdgcn_readfirstlane(work.seq), kvh = work.head, row0 = work.tile * 128;
@@ -850,7 +855,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_mx_kernel(const AttnArgs A
   if (row0 >= nrows) return;  // the whole workgroup
   const int ctx = min(max(A.ctx_lens[b], 0), A.width * PAGE), pos0 = ctx - qlen;  // pos0: keys before the new tokens
   const int pages = (max(0, pos0 + (min(row0 + 128, nrows) - 1) / G + 1) + PAGE - 1) / PAGE;
-  const int wrow0 = row0 + 32 * wave, wend = min(wrow0 + 32, nrows);
+  const int wrow0 = row0 + 16 * NB * wave, wend = min(wrow0 + 16 * NB, nrows);
   const int wmin = pos0 + wrow0 / G, wmax = wend > wrow0 ? pos0 + (wend - 1) / G : -1;  // last keys of the wave's first and last rows
 
   // this lane's pieces of a page: load i of the wave brings chunk ch of the keys' or (from NCH on) the values' bytes
@@ -879,7 +884,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_mx_kernel(const AttnArgs A
                                        (__attribute__((address_space(3))) void*)((v ? vd - L::NCH * 1024 : kd) + chunk[i] * 1024), 16, 0, 0);
     }
   };
-  // values of page p, landed, into bf16: the wave takes four octets of keys (lane group: octet) of some groups of dims
+  // values of page p, landed, into bf16: the wave takes four octets of keys (lane group: octet) of one group of dims
   auto make_values = [&](int p) {
     const uint8_t* raw = lds + L::V0 + p % (AHEAD + 1) * L::RAW;
     uint8_t* to = lds + L::B0 + (p & 1) * L::VBUF;
@@ -898,12 +903,11 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_mx_kernel(const AttnArgs A
       *reinterpret_cast<u32x4*>(t) = ae;
       *reinterpret_cast<u32x4*>(t + 1024) = ao;
     };
-    if (wave < 2) {
-      group(std::integral_constant<int, 0>{});
-      if constexpr (J == 4) group(std::integral_constant<int, 1>{});
-    } else {
-      group(std::integral_constant<int, J / 2>{});
-      if constexpr (J == 4) group(std::integral_constant<int, 3>{});
+    if (wave < 2) group(std::integral_constant<int, 0>{});
+    else if (wave < 4) group(std::integral_constant<int, 1>{});
+    else if constexpr (J == 4) {
+      if (wave < 6) group(std::integral_constant<int, 2>{});
+      else group(std::integral_constant<int, 3>{});
     }
   };
   auto meet = [] {  // LDS of this wave done, all waves here
@@ -1179,11 +1183,10 @@ at::Tensor attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const 
 
 constexpr int PROMPT_WAVES = 4, PROMPT_BLOCKS = 2;  // of 16 rows
 
-// new tokens against the pools: units of 32 rows of (token, head), of four waves that share the pages or one that has them all; or (waves 0)
-// attn_prompt_mx_kernel's of 128
+// new tokens against the pools: units of 32 rows of (token, head), of four waves that share the pages, or (tiles) attn_prompt_mx_kernel's of 128
 at::Tensor attn_prompt_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables, const at::Tensor& cu_q,
                           const at::Tensor& ctx_lens, const c10::optional<at::Tensor>& out_opt, const c10::optional<at::Tensor>& ws_o, const c10::optional<at::Tensor>& ws_ml,
-                  const c10::optional<at::Tensor>& tickets, int64_t max_qlen, int64_t pages_per_part, int64_t nparts, int64_t waves, double scale) {
+                  const c10::optional<at::Tensor>& tickets, int64_t max_qlen, int64_t pages_per_part, int64_t nparts, bool tiles, double scale) {
   const char* op = "attn_prompt_mx";
   XCHECK(q.is_cuda() && q.dim() == 3, op, ": q must be [T, H, Dh] on a GPU");
   const c10::DeviceGuard guard(q.device());
@@ -1195,35 +1198,29 @@ at::Tensor attn_prompt_mx(const at::Tensor& q, const at::Tensor& k_cache, const 
   const int64_t blocks = std::max<int64_t>(1, (max_qlen * (H / std::max<int64_t>(Hkv, 1)) + ROWS - 1) / ROWS);
   const AttnArgs a = attn_args(op, fp8, q, k_cache, v_cache, tables, ctx_lens, &cu_q, out, ws_o, ws_ml, tickets, blocks, ROWS, pages_per_part, nparts, scale);
   if (B == 0 || max_qlen == 0) return out;
-  XCHECK(waves == 0 || waves == 1 || waves == PROMPT_WAVES, op, ": 1 or 4 waves, or 0");
-  XCHECK(waves != 0 || nparts == 1, op, ": parts are of units of 1 or 4 waves");
-  if (waves == 0 && Hkv < 65536 && B < 65536) {  // (the grid's limits)
-    const int64_t tiles = (blocks * ROWS + 127) / 128;
-    const dim3 grid((unsigned)tiles, (unsigned)Hkv, (unsigned)B);
-#define GO(DHV, F)                                                                                                                         \
-  do {                                                                                                                                     \
-    auto* f = attn_prompt_mx_kernel<DHV, F>;                                                                                               \
-    constexpr int lds = PromptLds<DHV, F>::TOTAL;                                                                                          \
-    static const hipError_t set = hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, lds);                    \
-    XCHECK(set == hipSuccess, op, ": LDS");                                                                                                \
-    f<<<grid, 256, lds, stream()>>>(a);                                                                                                    \
+  if (tiles && Hkv < 65536 && B < 65536) {  // (the grid's limits)
+    XCHECK(nparts == 1, op, ": parts are of units");
+    const dim3 grid((unsigned)((blocks * ROWS + 127) / 128), (unsigned)Hkv, (unsigned)B);
+#define GO(DHV, F)                                                                                                             \
+  do {                                                                                                                         \
+    using L = PromptLds<DHV, F>;                                                                                               \
+    auto* f = attn_prompt_mx_kernel<DHV, F>;                                                                                   \
+    static const hipError_t set = hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);   \
+    XCHECK(set == hipSuccess, op, ": LDS");                                                                                    \
+    f<<<grid, 64 * L::NW, L::TOTAL, stream()>>>(a);                                                                            \
   } while (0)
     MX_GO(fp8, Dh, GO);
 #undef GO
     return out;
   }
-  const size_t lds = waves < PROMPT_WAVES ? 0 : (size_t)PROMPT_WAVES * ROWS * (Dh + 6) * sizeof(float);  // 67 KB at heads of 128
+  const size_t lds = (size_t)PROMPT_WAVES * ROWS * (Dh + 6) * sizeof(float);  // 67 KB at heads of 128
   const unsigned units = (unsigned)(B * blocks * nparts * Hkv);
 #define GO(DHV, F)                                                                                                                         \
   do {                                                                                                                                     \
-    if (waves < PROMPT_WAVES) {                                                                                                            \
-      attn_mx_kernel<DHV, F, 1, PROMPT_BLOCKS, true, !(F && DHV == 128)><<<units, 64, 0, stream()>>>(a);                                     \
-      break;                                                                                                                               \
-    }                                                                                                                                      \
-    auto* f = attn_mx_kernel<DHV, F, PROMPT_WAVES, PROMPT_BLOCKS, true, !(F && DHV == 128)>;                                                   \
+    auto* f = attn_mx_kernel<DHV, F, PROMPT_WAVES, PROMPT_BLOCKS, true, !(F && DHV == 128)>;                                               \
     static const hipError_t set = hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);              \
     XCHECK(set == hipSuccess, op, ": LDS");                                                                                                \
-    f<<<units, 64 * PROMPT_WAVES, lds, stream()>>>(a);                                                                                       \
+    f<<<units, 64 * PROMPT_WAVES, lds, stream()>>>(a);                                                                                     \
   } while (0)
   MX_GO(fp8, Dh, GO);
 #undef GO

@@ -484,24 +484,21 @@ def mx_prompt_units(B: int, max_qlen: int, G: int, Hkv: int) -> int:
   return max(1, B) * Hkv * max(1, -(-max_qlen * G // 32))
 
 
-def mx_prompt_direct(units: int, rows: float, Dh: int, fp8: bool) -> bool:
-  """Whether attn_prefill_mx reads the pools themselves (rows: of a sequence, on average): not where a long prompt among many sequences would
-  make most of the units empty, nor for long prompts in mxfp8 of 128 dims: us via bf16 pages / from the pools, 32 heads on 8, one of 4096
-  164 / 174, but one of 2048 81 / 67, 12 of 512 behind 1000 192 / 173.  mxfp4: 4 sequences of 64 new tokens behind 1000 50 / 15, one of
-  128 behind 8000 270 / 41, 12 of 512 82 / 61, one of 4096 164 / 158."""
-  return units <= 1 << 18 and not (fp8 and Dh == 128 and units >= 4096 and rows >= 16384)
+def mx_prompt_direct(units: int) -> bool:
+  """Whether attn_prefill_mx reads the pools themselves: not where a long prompt among many sequences would make most of the units empty.
+  us via bf16 pages / from the pools, 32 heads of 128 on 8: 4 sequences of 64 new tokens behind 1000 50 / 15, 12 of 512 82 / 56, one of 4096
+  165 / 150; mxfp8 50 / 17, 82 / 59, 165 / 164."""
+  return units <= 1 << 18
 
 
-def mx_prompt_waves(units: int, rows: float, Dh: int, fp8: bool) -> int:
-  """Which kernel (csrc/kv_mx.hip): 4, a unit's waves share its pages, where the units are few or a prompt's last ones would run alone; 0, four
-  units together with their pages and bf16 values in LDS; 1, a unit is a wave that makes its own values: long prompts in mxfp4 of 128 dims.
-  us with 4 / 1 / 0, 32 heads on 8, of 128 then 64 dims, mxfp4: 4 x 64 tokens behind 1000 15 / 31 / 34; 24 x 30 behind 300 20 / 17 / 18 and 12 /
-  12 / 13; 8 x 100 20 / 12 / 11 and 11 / 8 / 8; one of 1000 28 / 31 / 34 and 17 / 22 / 25; 12 x 128 28 / 16 / 15 and 15 / 11 / 10; 12 x 512 107 / 64 /
-  61 and 59 / 42 / 37; one of 2048 65 / 65 / 64 and 38 / 42 / 44, of 4096 189 / 158 / 167 and 115 / 109 / 98; mxfp8 12 x 512 behind 1000 225 /
-  188 / 173 and 130 / 117 / 107."""
-  if units <= (2048 if rows > 2048 else 768):
-    return 4
-  return 1 if not fp8 and Dh == 128 and rows >= 8192 else 0
+def mx_prompt_tiles(units: int, rows: float, Dh: int) -> bool:
+  """Which kernel (csrc/kv_mx.hip) takes prompts of on average so many rows (token and head): a unit's waves share its pages, where the units
+  are few; or (True) four units lie together in a workgroup, whose pages and bf16 values are in LDS.  us, 32 heads on 8, mxfp4, of 128 dims:
+  256 units (4 sequences of 64 new tokens behind 1000) 15 / 29, 704 (700 behind 700) 29 / 37, 768 (24 of 30 behind 300) 20 / 16, 1000 (one
+  prompt) 27 / 28, 1536 (12 of 128 behind 1000) 51 / 45, 2048 (one; 4 of 512) 63 / 55 and 39 / 26, 6144 (12 of 512) 107 / 56.  Of 64 dims,
+  where few prompts' longest workgroups run alone: 256 10 / 24, 768 12 / 13, 832 (8 of 100) 11 / 8, 1000 17 / 24, 2000 (2 of 1000) 29 / 31,
+  2048 (one; 4 of 512) 39 / 43 and 23 / 19, 6144 58 / 36."""
+  return units >= 768 and (Dh == 128 or rows <= 2048 or units > 2048)
 
 
 def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, cu_q: torch.Tensor,
@@ -515,15 +512,15 @@ def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
   Hkv = k_cache.shape[1]
   gpu = _gpu(q)
   G = max(1, H // Hkv)
-  units, rows, fp8 = mx_prompt_units(B, max_qlen, G, Hkv), T * G / max(1, B), k_cache.shape[2] > PAGE * Dh
-  if gpu and mx_prompt_direct(units, rows, Dh, fp8):
+  units = mx_prompt_units(B, max_qlen, G, Hkv)
+  if gpu and mx_prompt_direct(units):
     nparts = max(1, min(W // 16, 512 // units))
     ws = [None] * 3
     if nparts > 1:  # few rows behind long contexts
       ws = [torch.empty(units * nparts * 32 * n, dtype=torch.float32, device=q.device) for n in (Dh, 2)]
       ws.append(torch.zeros(units, dtype=torch.int32, device=q.device))
     return require().attn_prompt_mx(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, out, *ws, int(max_qlen), max(1, -(-W // nparts)), nparts,
-                                    mx_prompt_waves(units, rows, Dh, fp8), float(scale))
+                                    mx_prompt_tiles(units, T * G / max(1, B), Dh), float(scale))
   out = torch.empty_like(q) if out is None else out
   per = max(1, min(B, MX_READ_BYTES // max(1, W * Hkv * PAGE * Dh * 4))) if gpu else max(1, B)
   k = torch.empty(per * W, Hkv, PAGE, Dh, dtype=torch.bfloat16, device=q.device)
