@@ -497,6 +497,46 @@ def test_prompts_of_many_sequences_gpu(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B", [6, 63, 64, 65, 130, 4200])
+def test_steps_of_unlike_lengths_gpu(gpu, B):
+  """One long prompt among short turns, single tokens and sequences without any: every unit finds its sequence."""
+  H, Hkv, Dh = 6, 2, 64
+  s = Seqs("mxfp4", [70, 33, 130, 5, 64, 800], Hkv, Dh, dev=gpu)
+  new = [1, 0, 21, 5, 1, 790]
+  g = torch.Generator().manual_seed(B)
+  qs = [torch.randn(n, H, Dh, generator=g).to(torch.bfloat16) for n in new]
+  which = [i % 5 for i in range(B)]
+  which[B // 2] = 5
+  cu = [0]
+  for i in which:
+    cu.append(cu[-1] + new[i])
+  q = torch.cat([qs[i] for i in which]).to(gpu)
+  at = torch.tensor(which, device=gpu)
+  out = K.attn_prefill_mx(q, s.k, s.v, s.tables[at], torch.tensor(cu, dtype=torch.int32, device=gpu), s.ctx[at], 790, 0.125).cpu()
+  first = {}
+  for b, i in enumerate(which):
+    o = out[cu[b]:cu[b + 1]]
+    if i not in first:
+      first[i] = o
+      if new[i]:
+        close(o, *attend64(qs[i], *s.kv[i], 0.125, s.lens[i] - new[i]))
+    else:
+      assert torch.equal(o, first[i]), b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cu", [[0, 30, 20, 40], [5, 5, 900, 3], [-7, 2, 3, 1 << 30], [40, 30, 20, 10]])
+def test_starts_that_fall_gpu(gpu, cu):
+  """Starts that are not in order (nothing a caller should give) read and write within the tensors, whatever they give."""
+  s = Seqs("mxfp4", [70, 33, 130], 2, 64, dev=gpu)
+  q = torch.randn(40, 4, 64, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).to(gpu)
+  whole = torch.full((80, 4, 64), 7.0, dtype=torch.bfloat16, device=gpu)
+  for most in (40, 400):
+    K.attn_prefill_mx(q, s.k, s.v, s.tables, torch.tensor(cu, dtype=torch.int32, device=gpu), s.ctx, most, 0.125, out=whole[20:60])
+    assert (whole[:20] == 7).all() and (whole[60:] == 7).all()
+
+
+@pytest.mark.gpu
 def test_far_pages_gpu(gpu):
   """Pages whose bytes lie past 2^32 of their pool: written, read back, attended to by single tokens and prompts."""
   Hkv, Dh, fmt = 8, 128, "mxfp8"

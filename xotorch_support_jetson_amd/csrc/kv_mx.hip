@@ -361,7 +361,7 @@ struct AttnArgs {
   uint16_t* out;
   float *ws_o, *ws_ml;
   int* tickets;
-  int T, width, H, Hkv, ppp, nparts, num_pages, blocks, order;
+  int T, B, width, H, Hkv, ppp, nparts, num_pages, units, per, order;  // units: of a KV head; per: unit_at
   float scale_log2;
 };
 
@@ -387,6 +387,40 @@ __device__ __forceinline__ int sequence_at(const AttnArgs& A, int p) {
     for (int j = 0; j < 8; ++j) rank += (uint32_t)__builtin_amdgcn_readlane((int)key, j0 + j) > key ? 1 : 0;
   const int want = A.order == 1 || p < half ? p : B - 1 - (p - half);
   return __builtin_ctzll(__ballot(lane < B && rank == want));
+}
+
+// Unit u of a launch over new tokens: the sequence and the first of its R rows.  Sequence b's units start at floor(cu_q[b] G / R) + b, so that
+// T G / R + B units hold them all, whatever the lengths, with at most two to spare a sequence: a step of one prompt of 2000 tokens and 511
+// single ones has 6600 units of work where a grid of the longest's for each has a million.  64 sequences a look.  (cu_q that falls somewhere
+// finds some sequence of the launch, or none.)  per: the longest's units for each sequence, where that is no more (prompts about alike: 4 of 64
+// tokens behind 1000 15 us, 20 with a spare unit each, beside which others' CUs get two).
+template <int R>
+__device__ __forceinline__ bool unit_at(const AttnArgs& A, int u, int& b, int& row0, int& q0, int& q1) {
+  const int lane = threadIdx.x & 63, G = A.H / A.Hkv;
+  auto start = [&](int q, int i) { return (int)((uint32_t)(q * G) / R) + i; };
+  if (A.per > 0) {
+    b = u / A.per;
+    row0 = (u - b * A.per) * R;
+    q0 = min(max(A.cu_q[b], 0), A.T);
+    q1 = min(max(A.cu_q[b + 1], 0), A.T);
+    return true;
+  }
+  int k = 0, mine = 0, next = 0;
+  b = 0;
+  for (int n = A.B, step = 64; step > 1;) {
+    step = (n + 63) >> 6;
+    const int at = lane * step, i = b + min(at, n - 1);
+    mine = min(max(A.cu_q[i], 0), A.T);
+    next = min(max(A.cu_q[i + 1], 0), A.T);
+    k = __builtin_popcountll(__ballot(at < n && start(mine, i) <= u)) - 1;
+    if (k < 0) return false;
+    b += k * step;
+    n = min(step, n - k * step);
+  }
+  q0 = __builtin_amdgcn_readlane(mine, k);
+  q1 = __builtin_amdgcn_readlane(next, k);
+  row0 = (u - start(q0, b)) * R;
+  return row0 >= 0;
 }
 
 // What a lane's eight keys hold past the context may be anything, NaN too: it becomes zeros (their probabilities are 0, but 0 NaN is
@@ -608,11 +642,16 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : FP8 || REFILL ||
   constexpr int J = M::J, LD = DH + 4;
   extern __shared__ __attribute__((aligned(16))) float sm[];
   const int kvh = blockIdx.x % A.Hkv, bp = blockIdx.x / A.Hkv, part = bp % A.nparts, bu = bp / A.nparts;
-  const int b = PROMPT ? bu / A.blocks : A.order != 0 ? sequence_at(A, bu) : bu, row0 = PROMPT ? (A.blocks - 1 - (bu - b * A.blocks)) * 16 * NB : 0;
+  int b = bu, row0 = 0, q0 = bu, q1 = bu + 1;
+  if (PROMPT) {
+    if (!unit_at<16 * NB>(A, A.units - 1 - bu, b, row0, q0, q1)) return;  // (the whole workgroup, here and below)
+  } else if (A.order != 0) {
+    q0 = b = sequence_at(A, bu);
+  }
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, G = A.H / A.Hkv;
   const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int q0 = PROMPT ? min(max(A.cu_q[b], 0), A.T) : b, qlen = PROMPT ? min(max(A.cu_q[b + 1], q0), A.T) - q0 : 1, nrows = qlen * G;
-  if (PROMPT && row0 >= nrows) return;  // the whole workgroup, here and below
+  const int qlen = PROMPT ? max(q1 - q0, 0) : 1, nrows = qlen * G;
+  if (PROMPT && row0 >= nrows) return;
   const int RN = PROMPT ? min(16 * NB, nrows - row0) : G, RS = PROMPT ? 16 * NB : G;  // rows, and from unit to unit
   const int ctx = min(max(A.ctx_lens[b], 0), A.width * PAGE), pos0 = ctx - qlen;       // pos0: keys before the new tokens
   const int seen = PROMPT ? max(0, pos0 + (row0 + RN - 1) / G + 1) : ctx;              // keys that the unit's last row sees
@@ -1106,8 +1145,8 @@ std::tuple<at::Tensor, at::Tensor> kv_read_mx(const at::Tensor& k_cache, const a
 // what both forms of the attention check; cu_q: several tokens a sequence
 AttnArgs attn_args(const char* op, bool& fp8, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables,
                    const at::Tensor& ctx_lens, const at::Tensor* cu_q, at::Tensor& out, const c10::optional<at::Tensor>& ws_o,
-                   const c10::optional<at::Tensor>& ws_ml, const c10::optional<at::Tensor>& tickets, int64_t blocks, int64_t block_rows,
-                   int64_t pages_per_part, int64_t nparts, double scale, int order = 0) {
+                   const c10::optional<at::Tensor>& ws_ml, const c10::optional<at::Tensor>& tickets, int64_t units, int64_t unit_rows,
+                   int64_t pages_per_part, int64_t nparts, double scale, int per = 0, int order = 0) {
   const at::Device dev = q.device();
   on_gpu(op, q, at::kBFloat16, "q", dev);
   on_gpu(op, out, at::kBFloat16, "out", dev);
@@ -1128,11 +1167,10 @@ AttnArgs attn_args(const char* op, bool& fp8, const at::Tensor& q, const at::Ten
   XCHECK(T < (int64_t(1) << 31) / std::max<int64_t>(H, 1), op, ": too many tokens");
   XCHECK(out.sizes() == q.sizes(), op, ": out must have q's shape");
   XCHECK((reinterpret_cast<uintptr_t>(q.data_ptr()) | reinterpret_cast<uintptr_t>(out.data_ptr())) % 16 == 0, op, ": q and out must be aligned to 16 bytes");
-  XCHECK(pages_per_part >= 1 && pages_per_part <= (1 << 24) && nparts >= 1 && blocks >= 1, op, ": bad partitioning");
+  XCHECK(pages_per_part >= 1 && pages_per_part <= (1 << 24) && nparts >= 1, op, ": bad partitioning");
   XCHECK(scale > 0 && std::isfinite(scale), op, ": the scale must be positive");
-  XCHECK(blocks < (1 << 24) && nparts < (1 << 24) && B * blocks < (int64_t(1) << 24) && B * blocks * nparts < (int64_t(1) << 24) &&
-             B * blocks * nparts * Hkv < (int64_t(1) << 24),
-         op, ": too many parts for one launch");
+  XCHECK(nparts < (1 << 24) && units < (int64_t(1) << 24) && units * nparts < (int64_t(1) << 24) && units * nparts * Hkv < (int64_t(1) << 24), op,
+         ": too many parts for one launch");
   float *o = nullptr, *ml = nullptr;
   int* tk = nullptr;
   if (nparts > 1) {
@@ -1140,8 +1178,8 @@ AttnArgs attn_args(const char* op, bool& fp8, const at::Tensor& q, const at::Ten
     on_gpu(op, *ws_o, at::kFloat, "ws_o", dev);
     on_gpu(op, *ws_ml, at::kFloat, "ws_ml", dev);
     on_gpu(op, *tickets, at::kInt, "tickets", dev);
-    const int64_t rows = B * blocks * nparts * Hkv * block_rows;
-    XCHECK(tickets->numel() >= B * blocks * Hkv && ws_o->numel() >= rows * Dh && ws_ml->numel() >= rows * 2 &&
+    const int64_t rows = units * nparts * Hkv * unit_rows;
+    XCHECK(tickets->numel() >= units * Hkv && ws_o->numel() >= rows * Dh && ws_ml->numel() >= rows * 2 &&
                (reinterpret_cast<uintptr_t>(ws_o->data_ptr()) | reinterpret_cast<uintptr_t>(ws_ml->data_ptr())) % 16 == 0,
            op, ": workspace small");
     o = ws_o->data_ptr<float>();
@@ -1149,8 +1187,8 @@ AttnArgs attn_args(const char* op, bool& fp8, const at::Tensor& q, const at::Ten
     tk = tickets->data_ptr<int32_t>();
   }
   return {bf(q), k_cache.data_ptr<uint8_t>(), v_cache.data_ptr<uint8_t>(), tables.data_ptr<int32_t>(), ctx_lens.data_ptr<int32_t>(),
-          cu_q == nullptr ? nullptr : cu_q->data_ptr<int32_t>(), bf(out), o, ml, tk, (int)T, (int)tables.size(1), (int)H, (int)Hkv, (int)pages_per_part,
-          (int)nparts, (int)k_cache.size(0), (int)blocks, order, (float)scale * LOG2E};
+          cu_q == nullptr ? nullptr : cu_q->data_ptr<int32_t>(), bf(out), o, ml, tk, (int)T, (int)B, (int)tables.size(1), (int)H, (int)Hkv, (int)pages_per_part,
+          (int)nparts, (int)k_cache.size(0), (int)units, per, order, (float)scale * LOG2E};
 }
 
 at::Tensor attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& tables,
@@ -1162,8 +1200,8 @@ at::Tensor attn_decode_mx(const at::Tensor& q, const at::Tensor& k_cache, const 
   bool fp8 = false;
   at::Tensor out = out_opt.has_value() ? *out_opt : at::empty_like(q);
   const int64_t H = q.size(1), Dh = q.size(2), Hkv = k_cache.dim() == 3 ? k_cache.size(1) : 1;
-  const AttnArgs a = attn_args(op, fp8, q, k_cache, v_cache, tables, ctx_lens, nullptr, out, ws_o, ws_ml, tickets, 1, H / std::max<int64_t>(Hkv, 1),
-                               pages_per_part, nparts, scale, (int)order);
+  const AttnArgs a = attn_args(op, fp8, q, k_cache, v_cache, tables, ctx_lens, nullptr, out, ws_o, ws_ml, tickets, q.size(0), H / std::max<int64_t>(Hkv, 1),
+                               pages_per_part, nparts, scale, 0, (int)order);
   XCHECK(order == 0 || (order >= 1 && order <= 2 && q.size(0) <= 64), op, ": an order of at most 64 sequences");
   XCHECK(waves == 1 || waves == 2 || waves == 4, op, ": 1, 2 or 4 waves");
   if (q.size(0) == 0) return out;
@@ -1194,13 +1232,17 @@ at::Tensor attn_prompt_mx(const at::Tensor& q, const at::Tensor& k_cache, const 
   at::Tensor out = out_opt.has_value() ? *out_opt : at::empty_like(q);
   const int64_t H = q.size(1), Dh = q.size(2), Hkv = k_cache.dim() == 3 ? k_cache.size(1) : 1, B = ctx_lens.numel();
   XCHECK(max_qlen >= 0 && max_qlen < (1 << 24), op, ": max_qlen");
-  constexpr int64_t ROWS = 16 * PROMPT_BLOCKS;
-  const int64_t blocks = std::max<int64_t>(1, (max_qlen * (H / std::max<int64_t>(Hkv, 1)) + ROWS - 1) / ROWS);
-  const AttnArgs a = attn_args(op, fp8, q, k_cache, v_cache, tables, ctx_lens, &cu_q, out, ws_o, ws_ml, tickets, blocks, ROWS, pages_per_part, nparts, scale);
+  constexpr int64_t ROWS = 16 * PROMPT_BLOCKS, TILE = 128;
+  tiles = tiles && Hkv < 65536 && B < 65536;  // (the grid's limits)
+  const int64_t G = H / std::max<int64_t>(Hkv, 1), rows = tiles ? TILE : ROWS, per = (max_qlen * G + rows - 1) / rows;  // units of the longest
+  const bool even = tiles || B * per <= q.size(0) * G / ROWS + B;
+  const int64_t units = even ? B * per : q.size(0) * G / ROWS + B;
+  const AttnArgs a = attn_args(op, fp8, q, k_cache, v_cache, tables, ctx_lens, &cu_q, out, ws_o, ws_ml, tickets, units, ROWS, pages_per_part, nparts, scale,
+                               even ? (int)std::min<int64_t>(per, 1 << 24) : 0);
   if (B == 0 || max_qlen == 0) return out;
-  if (tiles && Hkv < 65536 && B < 65536) {  // (the grid's limits)
+  if (tiles) {
     XCHECK(nparts == 1, op, ": parts are of units");
-    const dim3 grid((unsigned)((blocks * ROWS + 127) / 128), (unsigned)Hkv, (unsigned)B);
+    const dim3 grid((unsigned)per, (unsigned)Hkv, (unsigned)B);
 #define GO(DHV, F)                                                                                                             \
   do {                                                                                                                         \
     using L = PromptLds<DHV, F>;                                                                                               \
@@ -1214,13 +1256,13 @@ at::Tensor attn_prompt_mx(const at::Tensor& q, const at::Tensor& k_cache, const 
     return out;
   }
   const size_t lds = (size_t)PROMPT_WAVES * ROWS * (Dh + 6) * sizeof(float);  // 67 KB at heads of 128
-  const unsigned units = (unsigned)(B * blocks * nparts * Hkv);
+  const unsigned grid = (unsigned)(units * nparts * Hkv);
 #define GO(DHV, F)                                                                                                                         \
   do {                                                                                                                                     \
     auto* f = attn_mx_kernel<DHV, F, PROMPT_WAVES, PROMPT_BLOCKS, true, !(F && DHV == 128)>;                                               \
     static const hipError_t set = hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);              \
     XCHECK(set == hipSuccess, op, ": LDS");                                                                                                \
-    f<<<units, 64 * PROMPT_WAVES, lds, stream()>>>(a);                                                                                     \
+    f<<<grid, 64 * PROMPT_WAVES, lds, stream()>>>(a);                                                                                      \
   } while (0)
   MX_GO(fp8, Dh, GO);
 #undef GO

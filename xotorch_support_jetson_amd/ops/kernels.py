@@ -479,48 +479,52 @@ def attn_decode_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 MX_READ_BYTES = 1 << 30
 
 
-def mx_prompt_units(B: int, max_qlen: int, G: int, Hkv: int) -> int:
-  """Units (32 rows of token and head) of a launch over B sequences of at most max_qlen new tokens; those past a sequence's end are empty."""
-  return max(1, B) * Hkv * max(1, -(-max_qlen * G // 32))
+def mx_prompt_units(T: int, B: int, max_qlen: int, G: int, Hkv: int) -> int:
+  """Units (32 rows of token and head) of a launch over T new tokens of B sequences, of at most max_qlen each (csrc/kv_mx.hip unit_at)."""
+  return Hkv * min(B * -(-max_qlen * G // 32), T * G // 32 + B)
 
 
-def mx_prompt_direct(units: int) -> bool:
-  """Whether attn_prefill_mx reads the pools themselves: not where a long prompt among many sequences would make most of the units empty.
-  us via bf16 pages / from the pools, 32 heads of 128 on 8: 4 sequences of 64 new tokens behind 1000 50 / 15, 12 of 512 82 / 56, one of 4096
-  165 / 150; mxfp8 50 / 17, 82 / 59, 165 / 164."""
-  return units <= 1 << 18
+def mx_prompt_direct(rows: float, W: int, Dh: int, fp8: bool) -> bool:
+  """Whether attn_prefill_mx reads the pools themselves: not for long prompts (rows of token and head, on average) behind tables of W pages
+  in mxfp8 of 128 dims.  us via bf16 pages / from the pools, 32 heads on 8: one prompt of 4096 165 / 164, behind 16384 more 1212 / 1342, one
+  of 8192 583 / 598, of 16384 2198 / 2320; mxfp4 165 / 150, 1189 / 1195, 577 / 535, 2156 / 2075; mxfp8 of 64 dims 120 / 95, 875 / 824, 422 /
+  344, 1588 / 1298; mxfp8, 4 of 64 behind 1000 50 / 17, 12 of 512 82 / 59, one of 500 beside 63 single tokens behind 1000 275 / 42."""
+  return not (fp8 and Dh == 128 and rows >= 16384 and W >= 128)
 
 
-def mx_prompt_tiles(units: int, rows: float, Dh: int) -> bool:
-  """Which kernel (csrc/kv_mx.hip) takes prompts of on average so many rows (token and head): a unit's waves share its pages, where the units
-  are few; or (True) four units lie together in a workgroup, whose pages and bf16 values are in LDS.  us, 32 heads on 8, mxfp4, of 128 dims:
-  256 units (4 sequences of 64 new tokens behind 1000) 15 / 29, 704 (700 behind 700) 29 / 37, 768 (24 of 30 behind 300) 20 / 16, 1000 (one
-  prompt) 27 / 28, 1536 (12 of 128 behind 1000) 51 / 45, 2048 (one; 4 of 512) 63 / 55 and 39 / 26, 6144 (12 of 512) 107 / 56.  Of 64 dims,
-  where few prompts' longest workgroups run alone: 256 10 / 24, 768 12 / 13, 832 (8 of 100) 11 / 8, 1000 17 / 24, 2000 (2 of 1000) 29 / 31,
-  2048 (one; 4 of 512) 39 / 43 and 23 / 19, 6144 58 / 36."""
-  return units >= 768 and (Dh == 128 or rows <= 2048 or units > 2048)
+def mx_prompt_tiles(units: int, rows: float, most: int, others: float, Dh: int) -> bool:
+  """Which kernel (csrc/kv_mx.hip) takes sequences of `rows` rows (new tokens x query heads of a KV head) on average, at most `most`, all but
+  one such of `others`: a unit's waves share its pages, where the units are few or some sequences' rows; or (True) four units lie together in
+  a workgroup, whose pages and bf16 values are in LDS.  us, 32 heads on 8, mxfp4, of 128 dims, units apart / together: 256 units (4 sequences
+  of 64 new tokens behind 1000) 15 / 29, 704 (700 behind 700) 29 / 37, 768 (24 of 30 behind 300) 20 / 16, 800 (100 of 8 behind 500) 26 / 35, 1000
+  (one) 27 / 28, 1536 (12 of 128 behind 1000) 50 / 45, 2048 (one; 4 of 512) 63 / 55 and 39 / 26, 2864 (1500, 700, 6 of 100) 65 / 45,
+  6144 (12 of 512) 107 / 56; beside 63 single tokens behind 1000 one of 500 29 / 114, of 4000 188 / 249; beside 511 one of 2000 195 / 594.  Of
+  64 dims, where few prompts' longest workgroups run alone: 256 10 / 24, 768 11 / 13, 832 (8 of 100) 11 / 8, 1000 17 / 24, 2000 (2 of 1000)
+  29 / 31, 2048 (one; 4 of 512) 39 / 43 and 23 / 19, 6144 58 / 36."""
+  return units >= 768 and others >= 64 and most <= 8 * rows and (Dh == 128 or rows <= 2048 or units > 2048)
 
 
 def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, cu_q: torch.Tensor,
                     ctx_lens: torch.Tensor, max_qlen: int, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
   """attn_prefill over pools in 8 or 4 bits: q [T, H, Dh], the tokens cu_q[b] .. cu_q[b + 1] are the last of sequence b's ctx_lens[b] (at
-  most max_qlen of them), each attends to what lies before it and itself; a token without keys gives zeros.  From the pools themselves
-  (mx_prompt_direct), or their pages are read back into bf16 scratch, a group of sequences at a time, which the bf16 prompt attention
-  reads.  As there, a NaN among a later token's values reaches the earlier ones of its page."""
+  most max_qlen of them), each attends to what lies before it and itself; a token without keys gives zeros.  From the pools themselves, or
+  (mx_prompt_direct) their pages are read back into bf16 scratch, a group of sequences at a time, which the bf16 prompt attention reads.
+  As there, a NaN among a later token's values reaches the earlier ones of its page."""
   T, H, Dh = q.shape
   B, W = block_tables.shape
   Hkv = k_cache.shape[1]
   gpu = _gpu(q)
   G = max(1, H // Hkv)
-  units = mx_prompt_units(B, max_qlen, G, Hkv)
-  if gpu and mx_prompt_direct(units):
-    nparts = max(1, min(W // 16, 512 // units))
+  units, rows = mx_prompt_units(T, B, max_qlen, G, Hkv), T * G / max(1, B)
+  if gpu and mx_prompt_direct(rows, W, Dh, k_cache.shape[2] > PAGE * Dh):
+    nparts = max(1, min(W // 16, 512 // max(1, units)))
+    most, others = max_qlen * G, (T - max_qlen) * G / (B - 1) if B > 1 else rows
     ws = [None] * 3
     if nparts > 1:  # few rows behind long contexts
       ws = [torch.empty(units * nparts * 32 * n, dtype=torch.float32, device=q.device) for n in (Dh, 2)]
       ws.append(torch.zeros(units, dtype=torch.int32, device=q.device))
     return require().attn_prompt_mx(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, out, *ws, int(max_qlen), max(1, -(-W // nparts)), nparts,
-                                    mx_prompt_tiles(units, T * G / max(1, B), Dh), float(scale))
+                                    mx_prompt_tiles(units, rows, most, others, Dh), float(scale))
   out = torch.empty_like(q) if out is None else out
   per = max(1, min(B, MX_READ_BYTES // max(1, W * Hkv * PAGE * Dh * 4))) if gpu else max(1, B)
   k = torch.empty(per * W, Hkv, PAGE, Dh, dtype=torch.bfloat16, device=q.device)
