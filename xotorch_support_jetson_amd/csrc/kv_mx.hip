@@ -857,8 +857,8 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : FP8 || REFILL ||
 // asked for, the values of p + 1 are made, page p is computed.
 // Bound by the vector unit and the waits for each other: 32 rows of a page are 1100 cycles of matrix instructions and 1300 of vector ones
 // (512 of them exponentials'), which overlap in part (46 % and 59 % busy; LDS 44 %).  One prompt, 32 heads on 8: of 128 dims, mxfp4, 4096
-// tokens 150 us (900 TFLOP/s), 8192 535 (1030), mxfp8 164 and 598; of 64 dims 93 and 305, 95 and 344; the bf16 kernel behind kv_read_mx 165
-// and 577, 165 and 583, 121 and 421, 120 and 422.  us of others, 4096 of 128 dims, mxfp4 / mxfp8: units of one wave that make their own values
+// tokens 150 us (900 TFLOP/s), 8192 507 to 535 (1030 and more), mxfp8 164 and 557 to 598; of 64 dims 92 and 288, 94 and 330; the bf16 kernel
+// behind kv_read_mx 165 and 577, 165 and 580, 120 and 421, 120 and 424.  us of others, 4096 of 128 dims, mxfp4 / mxfp8: units of one wave that make their own values
 // 149 / 192 (12 prompts of 512 62 / 68, here 56 / 59), four waves of 32 rows 158 / 164, half of the waves making values behind their products
 // instead of before 156 / 171, six waves of 32 rows 244; mxfp4 of 64 dims eight waves of 16 rows 92, 12 prompts of 512 37 (36).
 template <int DH, bool FP8>

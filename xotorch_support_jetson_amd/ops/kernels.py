@@ -485,11 +485,12 @@ def mx_prompt_units(T: int, B: int, max_qlen: int, G: int, Hkv: int) -> int:
 
 
 def mx_prompt_direct(rows: float, W: int, Dh: int, fp8: bool) -> bool:
-  """Whether attn_prefill_mx reads the pools themselves: not for long prompts (rows of token and head, on average) behind tables of W pages
-  in mxfp8 of 128 dims.  us via bf16 pages / from the pools, 32 heads on 8: one prompt of 4096 165 / 164, behind 16384 more 1212 / 1342, one
-  of 8192 583 / 598, of 16384 2198 / 2320; mxfp4 165 / 150, 1189 / 1195, 577 / 535, 2156 / 2075; mxfp8 of 64 dims 120 / 95, 875 / 824, 422 /
-  344, 1588 / 1298; mxfp8, 4 of 64 behind 1000 50 / 17, 12 of 512 82 / 59, one of 500 beside 63 single tokens behind 1000 275 / 42."""
-  return not (fp8 and Dh == 128 and rows >= 16384 and W >= 128)
+  """Whether attn_prefill_mx reads the pools themselves: not for long portions (rows of token and head, on average) behind tables of W pages
+  in mxfp8 of 128 dims, whose values take the prompt kernel longest.  us via bf16 pages / from the pools, 32 heads on 8: 2048 tokens behind
+  30000 1019 / 1077, 4096 behind 16384 1183 / 1251, 8192 behind 30000 4213 / 4625, 16384 alone 2152 / 2169, 8192 alone 580 / 556, 4096
+  alone 166 / 165; 32 on 32 2048 behind 30000 1133 / 1085, 8192 behind 30000 4407 / 4672; mxfp4 4096 behind 16384 1189 / 1195, 8192 alone
+  578 / 507; of 64 dims 875 / 824 and 425 / 330 (mxfp8); mxfp8, 4 of 64 behind 1000 50 / 17, one of 500 beside 63 single tokens 275 / 41."""
+  return not (fp8 and Dh == 128 and rows >= 8192 and W >= 256)
 
 
 def mx_prompt_tiles(units: int, rows: float, most: int, others: float, Dh: int) -> bool:
