@@ -493,6 +493,13 @@ def mx_prompt_direct(rows: float, W: int, Dh: int, fp8: bool) -> bool:
   return not (fp8 and Dh == 128 and rows >= 8192 and W >= 256)
 
 
+def mx_prompt_parts(units: int, W: int) -> int:
+  """Most parts of a context behind few rows.  A merge costs 3 to 6 us and pays where the units leave CUs without any and contexts are long: us in
+  1 / 2 / 3 / 4 / 8 parts, 32 heads of 128 on 8, mxfp4: 8 units (8 tokens behind 4000) 28 / 25 / 23 / 20 / 18, 64 (60 behind 1500; 8000)
+  17 / 20 / 19 / 19 / 21; 51 / 37 / 30 / 27 / 28, 128 (4 x 30 behind 4000) 30 / 28 / 31 / 28 / 39, 256 (64 heads) 31 / 38 / 47 / 47 / 61."""
+  return max(1, min(W // (8 if units <= 32 else 16), 256 // max(1, units)))
+
+
 def mx_prompt_tiles(units: int, rows: float, most: int, others: float, Dh: int) -> bool:
   """Which kernel (csrc/kv_mx.hip) takes sequences of `rows` rows (new tokens x query heads of a KV head) on average, at most `most`, all but
   one such of `others`: a unit's waves share its pages, where the units are few or some sequences' rows; or (True) four units lie together in
@@ -518,7 +525,7 @@ def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
   G = max(1, H // Hkv)
   units, rows = mx_prompt_units(T, B, max_qlen, G, Hkv), T * G / max(1, B)
   if gpu and mx_prompt_direct(rows, W, Dh, k_cache.shape[2] > PAGE * Dh):
-    nparts = max(1, min(W // 16, 512 // max(1, units)))
+    nparts = mx_prompt_parts(units, W)
     most, others = max_qlen * G, (T - max_qlen) * G / (B - 1) if B > 1 else rows
     ws = [None] * 3
     if nparts > 1:  # few rows behind long contexts
