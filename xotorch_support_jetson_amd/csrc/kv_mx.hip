@@ -623,14 +623,14 @@ struct Rows {
 // One unit: 16 NB rows (tokens of a sequence x query heads of a KV head; single tokens: its G heads) against a part of the pages.
 // NW waves share the part, wave w takes pages w, w + NW, ..., and meet in LDS.  REFILL: a page's registers are loaded anew as soon as
 // they are consumed, keys behind the scores, values behind their products, so that a page's loads fly under the other half's math; without
-// it a page is loaded and then computed, in fewer registers (mxfp4 124, four waves a SIMD; 153, three).  Many pairs have waves enough to
+// it a page is loaded and then computed, in fewer registers (mxfp4 126, four waves a SIMD; 155, three).  Many pairs have waves enough to
 // hide the loads (512 sequences of 525 tokens 56 / 60 us with REFILL, 128 of 30 to 8000 103 / 110), few have not (64 of 30 to 2000 21.0 /
 // 19.9, 8 on 32 KV heads 9.3 / 8.4); mxfp8 pages of 128 dims have no registers left for it.  Two sets of a page's registers, and three,
 // leave two waves a SIMD: 59, 59, 107, 107 us of the first two.
 // A context of several parts (at most nparts, of ppp pages and more) is merged by the workgroup that arrives last (a ticket a (rows, KV
 // head), zero between launches), in the parts' order whoever it is.
 // Bound by memory where the pairs of single tokens fill the chip: 512 sequences of 1500 tokens, 32 heads of 128 on 8, mxfp8 1.66 GB in 257
-// us (6.5 TB/s), mxfp4 856 MB in 138 us (6.2 TB/s); of 525 tokens, 64 heads, mxfp4 56 us (5.2 TB/s of what counts).  A page of mxfp4 is
+// us (6.5 TB/s), mxfp4 856 MB in 138 us (6.2 TB/s); of 525 tokens, 64 heads, mxfp4 54 us (5.7 TB/s of what counts).  A page of mxfp4 is
 // about 330 vector operations a wave, 190 of them making bf16 values; K needs none.  Uncut contexts and no loads ahead: 8 sequences of
 // 32000 tokens 239 us, now 48.
 // Prompts (PROMPT) start with their last rows, which see the most keys; here where they are few (attn_prompt_mx_kernel): 4 sequences of 64 new
@@ -826,9 +826,13 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : FP8 || REFILL ||
       f32x4 po[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const size_t row = row_ws + min(s0 + i, parts - 1) * step + rw;
-        ml[i] = agent_load2(A.ws_ml + row * 2);
-        po[i] = agent_load4(A.ws_o + row * DH + d);
+        ml[i] = {NEG_BIG, 0.f};
+        po[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (!PROMPT || s0 + i < parts) {  // (single tokens read the last again: a branch costs them registers; prompts' rows are many)
+          const size_t row = row_ws + min(s0 + i, parts - 1) * step + rw;
+          ml[i] = agent_load2(A.ws_ml + row * 2);
+          po[i] = agent_load4(A.ws_o + row * DH + d);
+        }
       }
       float mx = mm;
 #pragma unroll

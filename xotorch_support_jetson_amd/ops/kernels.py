@@ -494,9 +494,10 @@ def mx_prompt_direct(rows: float, W: int, Dh: int, fp8: bool) -> bool:
 
 
 def mx_prompt_parts(units: int, W: int) -> int:
-  """Most parts of a context behind few rows.  A merge costs 3 to 6 us and pays where the units leave CUs without any and contexts are long: us in
-  1 / 2 / 3 / 4 / 8 parts, 32 heads of 128 on 8, mxfp4: 8 units (8 tokens behind 4000) 28 / 25 / 23 / 20 / 18, 64 (60 behind 1500; 8000)
-  17 / 20 / 19 / 19 / 21; 51 / 37 / 30 / 27 / 28, 128 (4 x 30 behind 4000) 30 / 28 / 31 / 28 / 39, 256 (64 heads) 31 / 38 / 47 / 47 / 61."""
+  """Most parts of a context behind few rows.  A merge costs 2 to 5 us and pays where the units leave CUs without any and contexts are long: us in
+  1 / 2 / 3 / 4 / 8 parts, 32 heads of 128 on 8, mxfp4: 8 units (8 tokens behind 4000) 28 / 23 / 21 / 19 / 18, 64 (60 behind 1500; 8000)
+  17 / 18 / 17 / 17 / 20; 51 / 35 / 29 / 26 / 28, 128 (4 x 30 behind 4000) 29 / 26 / 29 / 27 / 39, 256 (4 x 60 behind 1500) 18 / 24 / 32 / 36 /
+  51."""
   return max(1, min(W // (8 if units <= 32 else 16), 256 // max(1, units)))
 
 
