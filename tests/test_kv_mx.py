@@ -616,6 +616,60 @@ def test_queries_not_finite_gpu(gpu, fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt,Dh", [("mxfp4", 128), ("mxfp8", 64)])
+def test_outputs_given_gpu(gpu, fmt, Dh):
+  """Results into the caller's tensors, the attentions' into their queries too; pages read back into used ones, with and without the tables'
+  rest."""
+  H, Hkv = 8, 2
+  s = Seqs(fmt, [70, 1200, 5], Hkv, Dh, dev=gpu, width=24)
+  g = torch.Generator().manual_seed(0)
+  x, pos, cs = qkv_of(9, H, Hkv, Dh).to(gpu), torch.arange(9, dtype=torch.int32, device=gpu), build_cos_sin(Dh, 16, 10000.0).to(gpu)
+  none = torch.full((9,), -1, device=gpu)
+  want = K.rope_kv_write_mx(x, pos, cs, none, s.k, s.v, H, Hkv)
+  flat = torch.empty(9, H * Dh, dtype=torch.bfloat16, device=gpu)
+  assert K.rope_kv_write_mx(x, pos, cs, none, s.k, s.v, H, Hkv, q_out=flat).data_ptr() == flat.data_ptr() and torch.equal(flat.view_as(want), want)
+  q = torch.randn(3, H, Dh, generator=g).to(torch.bfloat16).to(gpu)
+  want = K.attn_decode_mx(q, s.k, s.v, s.tables, s.ctx, 0.1)
+  assert torch.equal(K.attn_decode_mx(q, s.k, s.v, s.tables, s.ctx, 0.1, out=q), want) and torch.equal(q, want)
+  cu = torch.tensor([0, 40, 46, 49], dtype=torch.int32, device=gpu)
+  for most in (40, 1500):  # (the second: a bound only)
+    q = torch.randn(49, H, Dh, generator=g).to(torch.bfloat16).to(gpu)
+    want = K.attn_prefill_mx(q, s.k, s.v, s.tables, cu, s.ctx, most, 0.1)
+    assert torch.equal(K.attn_prefill_mx(q, s.k, s.v, s.tables, cu, s.ctx, most, 0.1, out=q), want) and torch.equal(q, want)
+  k, v = K.kv_read_mx(s.k, s.v, s.tables, s.ctx, Dh)
+  for skip in (False, True):
+    ko, vo = torch.full_like(k, 3.0), torch.full_like(v, 3.0)
+    K.kv_read_mx(s.k, s.v, s.tables, s.ctx, Dh, ko, vo, skip)
+    past = (torch.arange(24, device=gpu)[None] * PAGE >= s.ctx[:, None]).flatten()
+    for a, b in ((ko, k), (vo, v)):
+      assert torch.equal(a[~past], b[~past]) and (a[past] == (3.0 if skip else 0.0)).all()
+
+
+@pytest.mark.gpu
+def test_two_streams_gpu(gpu):
+  """Calls in flight on two streams at once, single tokens with a workspace each."""
+  H, Hkv, Dh = 8, 2, 128
+  s = Seqs("mxfp4", [4000, 1200, 900], Hkv, Dh, dev=gpu)
+  cu = torch.tensor([0, 9, 12, 20], dtype=torch.int32, device=gpu)
+  qs = [torch.randn(20, H, Dh, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16).to(gpu) for i in range(2)]
+  ws = [K.MXDecodeWorkspace(3, H, Hkv, Dh, 4096, gpu) for _ in range(2)]
+
+  def both(i):
+    return K.attn_decode_mx(qs[i][:3], s.k, s.v, s.tables, s.ctx, 0.1, ws[i]), K.attn_prefill_mx(qs[i], s.k, s.v, s.tables, cu, s.ctx, 9, 0.1)
+  want = [both(i) for i in range(2)]
+  streams = [torch.cuda.Stream(gpu) for _ in range(2)]
+  torch.cuda.synchronize()
+  got = []
+  for n in range(10):
+    for i, stream in enumerate(streams):
+      with torch.cuda.stream(stream):
+        got.append((i, both(i)))
+  torch.cuda.synchronize()
+  for i, (a, b) in got:
+    assert torch.equal(a, want[i][0]) and torch.equal(b, want[i][1])
+
+
+@pytest.mark.gpu
 def test_nothing_to_do_gpu(gpu):
   s = Seqs("mxfp4", [70, 5], 2, 128, dev=gpu)
   none = lambda *shape, dt=torch.bfloat16: torch.zeros(*shape, dtype=dt, device=gpu)  # noqa: E731
