@@ -715,3 +715,40 @@ def test_refusals_gpu(gpu):
     with pytest.raises((RuntimeError, ValueError)):
       call()
       print("not refused:", i)
+
+
+# ------------------------------------------------------------------ edges
+SCALES_REFUSED = (0.0, -1.0, 1e-50, 1e-38, 1e-310, 2e38, 3e38, 1e300, float("inf"), float("nan"))
+
+
+def check_scales(dev):
+  """A scale that vanishes or overflows as the float that scores are multiplied by; the bounds themselves pass."""
+  s = Seqs("mxfp8", [70, 5], 2, 128, dev=dev)
+  q = torch.zeros(2, 4, 128, dtype=torch.bfloat16, device=dev)
+  cu = torch.tensor([0, 1, 2], dtype=torch.int32, device=dev)
+  for scale in SCALES_REFUSED:
+    with pytest.raises(RuntimeError, match="scale"):
+      K.attn_decode_mx(q, s.k, s.v, s.tables, s.ctx, scale)
+    with pytest.raises(RuntimeError, match="scale"):
+      K.attn_prefill_mx(q, s.k, s.v, s.tables, cu, s.ctx, 1, scale)
+  for scale in (2.0 ** -125, 2.0 ** 126):  # (queries of zeros: every key weighs alike)
+    for out in (K.attn_decode_mx(q, s.k, s.v, s.tables, s.ctx, scale), K.attn_prefill_mx(q, s.k, s.v, s.tables, cu, s.ctx, 1, scale)):
+      for b, n in enumerate(s.lens):
+        close(out[b:b + 1], *attend64(q[b:b + 1], *s.kv[b], 1.0, n - 1))
+
+
+def test_scales():
+  check_scales("cpu")
+
+
+@pytest.mark.gpu
+def test_scales_gpu(gpu, monkeypatch):
+  for direct in (True, False):
+    monkeypatch.setattr(K, "mx_prompt_direct", lambda *a: direct)
+    check_scales(gpu)
+  s = Seqs("mxfp4", [70, 5], 2, 128, dev=gpu)
+  q = torch.zeros(2, 4, 128, dtype=torch.bfloat16, device=gpu)
+  monkeypatch.setattr(K, "_mx_scale", lambda scale: None)  # (the binding by itself)
+  for scale in SCALES_REFUSED:
+    with pytest.raises(RuntimeError, match="scale"):
+      K.attn_decode_mx(q, s.k, s.v, s.tables, s.ctx, scale)

@@ -16,7 +16,6 @@
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 #include <algorithm>
-#include <cmath>
 #include "handover.h"
 
 namespace xot {
@@ -1174,7 +1173,8 @@ AttnArgs attn_args(const char* op, bool& fp8, const at::Tensor& q, const at::Ten
   XCHECK(out.sizes() == q.sizes(), op, ": out must have q's shape");
   XCHECK((reinterpret_cast<uintptr_t>(q.data_ptr()) | reinterpret_cast<uintptr_t>(out.data_ptr())) % 16 == 0, op, ": q and out must be aligned to 16 bytes");
   XCHECK(pages_per_part >= 1 && pages_per_part <= (1 << 24) && nparts >= 1, op, ": bad partitioning");
-  XCHECK(scale > 0 && std::isfinite(scale), op, ": the scale must be positive");
+  // (what the kernels multiply by, the scale times log2 e as a float, stays a positive normal number: masked scores are -inf)
+  XCHECK(scale >= 0x1p-125 && scale <= 0x1p126, op, ": the scale must be positive, 2^-125 to 2^126");
   XCHECK(nparts < (1 << 24) && units < (int64_t(1) << 24) && units * nparts < (int64_t(1) << 24) && units * nparts * Hkv < (int64_t(1) << 24), op,
          ": too many parts for one launch");
   float *o = nullptr, *ml = nullptr;

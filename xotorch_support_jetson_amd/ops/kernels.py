@@ -358,6 +358,12 @@ mx_page_bytes = ref.mx_page_bytes
 mx_format = ref.mx_format
 
 
+def _mx_scale(scale: float) -> None:
+  """Refuses what the kernels cannot multiply scores by (csrc/kv_mx.hip attn_args), on the CPU too."""
+  if not 2.0 ** -125 <= scale <= 2.0 ** 126:
+    raise RuntimeError(f"the scale must be positive, 2^-125 to 2^126, not {scale}")
+
+
 def rope_kv_write_mx(qkv: torch.Tensor, pos: torch.Tensor, cos_sin: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
                      v_cache: torch.Tensor, H: int, Hkv: int, q_out: torch.Tensor | None = None) -> torch.Tensor:
   """qkv [T, (H+2Hkv)*Dh] -> rotated q [T, H, Dh]; rotated k (quantised from fp32) and v into the pools at `slots` (distinct; one
@@ -459,6 +465,7 @@ def attn_decode_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
                    scale: float, ws: MXDecodeWorkspace | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
   """attn_decode over pools in 8 or 4 bits: q [B, H, Dh], one token a sequence, attends to its first ctx_lens keys; a sequence without
   any gives zeros."""
+  _mx_scale(scale)
   if not _gpu(q):
     y = ref.attn_decode_mx(q, k_cache, v_cache, block_tables, ctx_lens, scale)
     if out is not None:
@@ -519,6 +526,7 @@ def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
   most max_qlen of them), each attends to what lies before it and itself; a token without keys gives zeros.  From the pools themselves, or
   (mx_prompt_direct) their pages are read back into bf16 scratch, a group of sequences at a time, which the bf16 prompt attention reads.
   As there, a NaN among a later token's values reaches the earlier ones of its page."""
+  _mx_scale(scale)
   T, H, Dh = q.shape
   B, W = block_tables.shape
   Hkv = k_cache.shape[1]
