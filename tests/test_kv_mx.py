@@ -752,3 +752,46 @@ def test_scales_gpu(gpu, monkeypatch):
   for scale in SCALES_REFUSED:
     with pytest.raises(RuntimeError, match="scale"):
       K.attn_decode_mx(q, s.k, s.v, s.tables, s.ctx, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("far", [1e31, -1e31, 1e37, -1e37, 1e12, -1e12, 3e7])
+@pytest.mark.parametrize("fmt,Dh", [("mxfp4", 128), ("mxfp8", 128), ("mxfp4", 64), ("mxfp8", 64)])
+def test_far_scores_gpu(gpu, fmt, Dh, far, monkeypatch):
+  """Scores of any finite size (of either sign, past the precision of their products): equal ones weigh alike, a largest one takes all.
+  Every product is a power of two times 207 / 128 and 1, 1.5 or 0, so scores are exact and weights 1 or 0: the result is off by its rounding
+  and its sum's, n <= 200 terms of 2^-24 each."""
+  H, Hkv = 4, 2
+  s = Seqs(fmt, [200, 130, 70], Hkv, Dh, dev=gpu)
+  a = round(math.log2(abs(far) / Dh) / 2)
+  c = torch.randint(0, 2, (Dh,), generator=torch.Generator().manual_seed(0)) * 2.0 - 1
+  levels = [torch.ones(200), torch.where(torch.arange(130) % 7 == 3, 1.5, 1.0), torch.where(torch.arange(70) % 5 == 2, 0.0, 1.0)]
+  s.kv = []
+  for b, m in enumerate(s.lens):
+    v = torch.randn(m, Hkv, Dh, generator=torch.Generator().manual_seed(b))
+    k = (levels[b][:, None, None] * c * 2.0 ** a).expand(m, Hkv, Dh)
+    at = s.tables[b].cpu().long()[torch.arange(m) // PAGE] * PAGE + torch.arange(m) % PAGE
+    kc, vc = s.k.cpu(), s.v.cpu()
+    ref.mx_write(k, v, at, kc, vc)
+    s.k, s.v = kc.to(gpu), vc.to(gpu)
+    s.kv.append((held(k, fmt), held(v, fmt)))
+    assert torch.equal(s.kv[b][0], k.double())
+  q = (c * 2.0 ** a * math.copysign(207 / 128, far)).expand(400, H, Dh).to(torch.bfloat16).contiguous()
+
+  def check(out, rows, b, past):
+    want, weight, _ = attend64(q[:rows], *s.kv[b], 0.9, past)
+    assert ((out.double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -16 * weight).all()
+  for waves in ((1, False), (2, False), (4, True)):
+    for least in (1, 4):
+      with monkeypatch.context() as m:
+        m.setattr(K, "mx_decode_waves", lambda *a: waves)
+        m.setattr(K.MXDecodeWorkspace, "parts", staticmethod(lambda b, h, pages: (least, -(-pages // least))))
+        out = K.attn_decode_mx(q[:3].contiguous().to(gpu), s.k, s.v, s.tables, s.ctx, 0.9)
+      for b, n in enumerate(s.lens):
+        check(out[b:b + 1], 1, b, n - 1)
+  cu = [0, 200, 330, 400]
+  for tiles in (True, False):
+    monkeypatch.setattr(K, "mx_prompt_tiles", lambda *a: tiles)
+    out = K.attn_prefill_mx(q.to(gpu), s.k, s.v, s.tables, torch.tensor(cu, dtype=torch.int32, device=gpu), s.ctx, 200, 0.9)
+    for b, n in enumerate(s.lens):
+      check(out[cu[b]:cu[b + 1]], n, b, 0)

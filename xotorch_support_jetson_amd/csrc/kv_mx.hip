@@ -22,7 +22,8 @@ namespace xot {
 namespace {
 
 constexpr int PAGE = 64;
-constexpr float NEG_BIG = -1e30f;
+constexpr float NEG_BIG = -3.402823466e38f;  // a maximum of no scores: no finite score is below it
+constexpr float FAR = 16777216.f;            // (Rows::weights)
 constexpr float LOG2E = 1.4426950408889634f;
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -543,7 +544,9 @@ struct Rows {
       for (int r = 0; r < 4; ++r) st[t][r] = 32 * (t >> 1) + 4 * (t & 1) + r < left ? st[t][r] : -INFINITY;
   }
   // The page's weights in bf16, B operands of the products with its values; what the rows have so far is brought to the new maxima.
-  __device__ __forceinline__ void weights(const f32x4 (&st)[NB][4], float scale_log2, s16x8 (&pf)[NB][2]) {
+  // Weights are 2^fma(score, scale, -m): the product unrounded, m the largest one rounded.  Past 2^24 the two differ by more than 1, soon by
+  // hundreds, and all weights of a row would overflow or vanish: the scores there are scaled, with m's rounding, before m is taken from them.
+  __device__ __forceinline__ void weights(f32x4 (&st)[NB][4], float scale_log2, s16x8 (&pf)[NB][2]) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       float mx = -INFINITY;
@@ -564,13 +567,19 @@ struct Rows {
           o[nb][j][1] *= alpha;
         }
       }
+      float scale = scale_log2;
+      if (__ballot(fabsf(m[nb]) > FAR)) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) st[nb][t] *= scale_log2;
+        scale = 1.f;
+      }
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         u32x4 pw;
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(st[nb][2 * kk + (e >> 2)][e & 3], scale_log2, -m[nb]));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(st[nb][2 * kk + (e >> 2)][(e & 3) + 1], scale_log2, -m[nb]));
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(st[nb][2 * kk + (e >> 2)][e & 3], scale, -m[nb]));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(st[nb][2 * kk + (e >> 2)][(e & 3) + 1], scale, -m[nb]));
           if constexpr (!ONES) l[nb] += p0 + p1;
           pw[e >> 1] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{p0, p1}), bf16x2_t));
         }
@@ -582,7 +591,7 @@ struct Rows {
   }
   // The page's weights and their products with its values; vv(kk, v, vs): eight keys' units and scales.
   template <class V>
-  __device__ __forceinline__ void weigh(V vv, const f32x4 (&st)[NB][4], float scale_log2) {
+  __device__ __forceinline__ void weigh(V vv, f32x4 (&st)[NB][4], float scale_log2) {
     s16x8 pf[NB][2];
     weights(st, scale_log2, pf);
 #pragma unroll
