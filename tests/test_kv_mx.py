@@ -795,3 +795,22 @@ def test_far_scores_gpu(gpu, fmt, Dh, far, monkeypatch):
     out = K.attn_prefill_mx(q.to(gpu), s.k, s.v, s.tables, torch.tensor(cu, dtype=torch.int32, device=gpu), s.ctx, 200, 0.9)
     for b, n in enumerate(s.lens):
       check(out[cu[b]:cu[b + 1]], n, b, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,Dh", [("mxfp4", 128), ("mxfp8", 128), ("mxfp4", 64), ("mxfp8", 64)])
+def test_rows_without_keys_gpu(gpu, fmt, Dh, monkeypatch):
+  """Tokens before the first key give zeros whatever the cache holds, NaN too; the others see it."""
+  H, Hkv = 4, 2
+  s = Seqs(fmt, [3, 70], Hkv, Dh, dev=gpu)
+  k, v = s.k.cpu(), s.v.cpu()
+  bad = torch.full((1, Hkv, Dh), float("nan"))
+  for b in range(2):
+    ref.mx_write(bad, bad, s.tables[b, :1].cpu().long() * PAGE, k, v)
+  q = torch.randn(87, H, Dh, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).to(gpu)
+  cu = torch.tensor([0, 7, 87], dtype=torch.int32, device=gpu)
+  for tiles in (True, False):
+    monkeypatch.setattr(K, "mx_prompt_tiles", lambda *a: tiles)
+    out = K.attn_prefill_mx(q, k.to(gpu), v.to(gpu), s.tables, cu, s.ctx, 80, 0.1)
+    assert (out[:4] == 0).all() and (out[7:17] == 0).all()
+    assert torch.isnan(out[4:7]).all() and torch.isnan(out[17:]).all()

@@ -1027,12 +1027,17 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 4) void attn_prompt_mx_kerne
   for (int nb = 0; nb < NB; ++nb) {
     const int row = wrow0 + 16 * nb + c, ti = row / G;
     if (row >= nrows) continue;
-    const float inv = pos0 + ti >= 0 ? 1.f / rows.l[nb] : 0.f;  // a row without keys: zeros (its sums are)
+    const bool keys = pos0 + ti >= 0;  // without any: zeros (its sums are, or NaN where values of the page are)
+    const float inv = 1.f / rows.l[nb];
     uint16_t* p = A.out + ((size_t)(q0 + ti) * A.H + kvh * G + row - ti * G) * DH + 8 * g;
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) st_results(p + 32 * j + 4 * half, rows.dims(nb, j, half), inv);
+      for (int half = 0; half < 2; ++half) {
+        uint16_t* to = p + 32 * j + 4 * half;
+        if (keys) st_results(to, rows.dims(nb, j, half), inv);
+        else *reinterpret_cast<s16x4*>(to) = s16x4{0, 0, 0, 0};
+      }
   }
 }
 
