@@ -814,3 +814,27 @@ def test_rows_without_keys_gpu(gpu, fmt, Dh, monkeypatch):
     out = K.attn_prefill_mx(q, k.to(gpu), v.to(gpu), s.tables, cu, s.ctx, 80, 0.1)
     assert (out[:4] == 0).all() and (out[7:17] == 0).all()
     assert torch.isnan(out[4:7]).all() and torch.isnan(out[17:]).all()
+
+
+@pytest.mark.parametrize("fmt,Dh", [("mxfp4", 128), ("mxfp8", 64)])
+def test_prompt_rows_cpu(fmt, Dh):
+  """On the CPU as on the GPU: tokens before the first key give zeros, rows of no sequence stay, contexts end with their table, a NaN
+  reaches the tokens that see it."""
+  s = Seqs(fmt, [3, 0, 100, 70], 2, Dh)
+  q = torch.randn(33, 4, Dh, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+  cu = torch.tensor([0, 5, 7, 7, 30], dtype=torch.int32)
+  out = K.attn_prefill_mx(q, s.k, s.v, s.tables, cu, s.ctx, 23, 0.1, out=torch.full_like(q, 7.0))
+  assert (out[:2] == 0).all() and (out[5:7] == 0).all() and (out[30:] == 7).all()
+  close(out[2:5], *attend64(q[2:5], *s.kv[0], 0.1, 0))
+  close(out[7:30], *attend64(q[7:30], *s.kv[3], 0.1, 47))
+  n = s.tables.shape[1] * PAGE
+  past = K.attn_prefill_mx(q[:1], s.k, s.v, s.tables[2:3], torch.tensor([0, 1], dtype=torch.int32), torch.tensor([n + 60], dtype=torch.int32), 1, 0.1)
+  whole = K.attn_prefill_mx(q[:1], s.k, s.v, s.tables[2:3], torch.tensor([0, 1], dtype=torch.int32), torch.tensor([n], dtype=torch.int32), 1, 0.1)
+  assert torch.equal(past, whole)
+  bad = torch.ones(1, 2, Dh)
+  bad[0, 1, 40] = float("nan")
+  ref.mx_write(torch.ones(1, 2, Dh), bad, s.tables[3, 0:1].long() * PAGE + 50, s.k, s.v)
+  got = K.attn_prefill_mx(q, s.k, s.v, s.tables, cu, s.ctx, 23, 0.1)[7:30]
+  want = torch.zeros(23, 4, Dh, dtype=torch.bool)
+  want[3:, 2:, 32:64] = True
+  assert torch.equal(torch.isnan(got), want)

@@ -7,7 +7,6 @@ raises (see `ops._ext.require`).
 """
 from __future__ import annotations
 
-import contextlib
 import os
 
 import torch
@@ -525,7 +524,7 @@ def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
   """attn_prefill over pools in 8 or 4 bits: q [T, H, Dh], the tokens cu_q[b] .. cu_q[b + 1] are the last of sequence b's ctx_lens[b] (at
   most max_qlen of them), each attends to what lies before it and itself; a token without keys gives zeros.  From the pools themselves, or
   (mx_prompt_direct) their pages are read back into bf16 scratch, a group of sequences at a time, which the bf16 prompt attention reads.
-  As there, a NaN among a later token's values reaches the earlier ones of its page."""
+  As there, a NaN among a later token's values reaches the earlier ones of its page (not on the CPU)."""
   _mx_scale(scale)
   T, H, Dh = q.shape
   B, W = block_tables.shape
@@ -543,18 +542,18 @@ def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     return require().attn_prompt_mx(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, out, *ws, int(max_qlen), max(1, -(-W // nparts)), nparts,
                                     mx_prompt_tiles(units, rows, most, others, Dh), float(scale))
   out = torch.empty_like(q) if out is None else out
-  per = max(1, min(B, MX_READ_BYTES // max(1, W * Hkv * PAGE * Dh * 4))) if gpu else max(1, B)
+  if not gpu:
+    ref.attn_prefill_mx(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, scale, out)
+    return out
+  per = max(1, min(B, MX_READ_BYTES // max(1, W * Hkv * PAGE * Dh * 4)))
   k = torch.empty(per * W, Hkv, PAGE, Dh, dtype=torch.bfloat16, device=q.device)
   v = torch.empty(per * W, Hkv, Dh, PAGE, dtype=torch.bfloat16, device=q.device)
-  own = torch.empty(per, W, dtype=torch.int32, device=q.device) if gpu else torch.arange(per * W, dtype=torch.int32).view(per, W)
+  own = torch.empty(per, W, dtype=torch.int32, device=q.device)
   for b in range(0, B, per):
     n = min(per, B - b)
     tables, ctx, cu = block_tables[b:b + n], ctx_lens[b:b + n], cu_q[b:b + n + 1]
-    if gpu:
-      require().kv_read_mx(k_cache, v_cache, tables, ctx, Dh, k[:n * W], v[:n * W], True, own[:n])
-    else:
-      ref.kv_read_mx(k_cache, v_cache, tables, ctx, k, v)
-    with torch.cuda.device(q.device) if gpu else contextlib.nullcontext():
+    require().kv_read_mx(k_cache, v_cache, tables, ctx, Dh, k[:n * W], v[:n * W], True, own[:n])
+    with torch.cuda.device(q.device):
       attn_prefill(q, k, v, own[:n], cu, ctx, max_qlen, scale, out=out)
   return out
 

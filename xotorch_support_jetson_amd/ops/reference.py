@@ -275,6 +275,24 @@ def attn_decode_mx(q, k_cache, v_cache, block_tables, ctx_lens, scale):
   return out
 
 
+def attn_prefill_mx(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, scale, out):
+  """q [T, H, Dh] -> out over pools in 8 or 4 bits: causal at the end of each context, zeros for tokens without keys; rows of no sequence stay"""
+  width = 64 * block_tables.shape[1]
+  for b in range(ctx_lens.numel()):
+    q0, q1 = (min(max(int(cu_q[b + i]), 0), q.shape[0]) for i in range(2))
+    n = min(int(ctx_lens[b]), width)
+    live = q0 + max(0, q1 - q0 - max(n, 0))  # the first row that sees a key
+    if live >= q1:
+      out[q0:max(q0, q1)] = 0
+      continue
+    k, v = mx_gather(k_cache, v_cache, block_tables[b], n, q.shape[-1])
+    past = n - (q1 - live)
+    y = _attend(q[live:q1], k, v.nan_to_num(0.0), scale, past)
+    seen = (torch.isnan(v).cumsum(0) > 0)[past:].repeat_interleave(q.shape[1] // v.shape[1], 1)  # (a NaN reaches the rows that see its key)
+    out[q0:live] = 0
+    out[live:q1] = torch.where(seen, float("nan"), y).to(q.dtype)
+
+
 def sample_greedy(logits: torch.Tensor) -> torch.Tensor:
   return logits.float().argmax(dim=-1).to(torch.int32)
 
