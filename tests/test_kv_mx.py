@@ -838,3 +838,16 @@ def test_prompt_rows_cpu(fmt, Dh):
   want = torch.zeros(23, 4, Dh, dtype=torch.bool)
   want[3:, 2:, 32:64] = True
   assert torch.equal(torch.isnan(got), want)
+
+
+@pytest.mark.parametrize("fmt,Dh", [("mxfp4", 128), ("mxfp8", 64)])
+def test_read_skips_cpu(fmt, Dh):
+  """Pages read back into used ones: those wholly past a context become zeros, or (skip) stay, on the CPU too."""
+  s = Seqs(fmt, [70, 0, 130], 2, Dh, width=4)
+  k, v = K.kv_read_mx(s.k, s.v, s.tables, s.ctx, Dh)
+  past = (torch.arange(4)[None] * PAGE >= s.ctx[:, None]).flatten()
+  for skip in (False, True):
+    ko, vo = torch.full_like(k, 3.0), torch.full_like(v, 3.0)
+    K.kv_read_mx(s.k, s.v, s.tables, s.ctx, Dh, ko, vo, skip)
+    for a, b in ((ko, k), (vo, v)):
+      assert torch.equal(a[~past], b[~past]) and (a[past] == (3.0 if skip else 0.0)).all()

@@ -389,7 +389,7 @@ def kv_read_mx(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch
     k_out = torch.empty(n, Hkv, PAGE, Dh, dtype=torch.bfloat16, device=k_cache.device)
   if v_out is None:
     v_out = torch.empty(n, Hkv, Dh, PAGE, dtype=torch.bfloat16, device=k_cache.device)
-  ref.kv_read_mx(k_cache, v_cache, block_tables, ctx_lens, k_out, v_out)
+  ref.kv_read_mx(k_cache, v_cache, block_tables, ctx_lens, k_out, v_out, skip)
   return k_out, v_out
 
 

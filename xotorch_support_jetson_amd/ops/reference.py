@@ -255,13 +255,15 @@ def mx_gather(k_cache, v_cache, table, n: int, Dh: int):
   return tuple(t.transpose(1, 2).flatten(0, 1)[:n] for t in (k, v))
 
 
-def kv_read_mx(k_cache, v_cache, block_tables, ctx_lens, k_out, v_out) -> None:
-  """The tables' pages as bf16 pages [entries, Hkv, 64, Dh] and (storage chunk-major) [entries, Hkv, Dh, 64]; zeros past the contexts."""
+def kv_read_mx(k_cache, v_cache, block_tables, ctx_lens, k_out, v_out, skip: bool = False) -> None:
+  """The tables' pages as bf16 pages [entries, Hkv, 64, Dh] and (storage chunk-major) [entries, Hkv, Dh, 64]; zeros past the contexts, skip:
+  pages wholly past them stay."""
   B, W = block_tables.shape
   k, v = mx_read(k_cache, v_cache, block_tables.flatten(), k_out.shape[-1])
   live = (torch.arange(W * 64, device=k.device)[None] < ctx_lens[:, None]).view(B * W, 1, 64, 1)
-  k_out.copy_(torch.where(live, k, 0.0))
-  v_chunks(v_out).copy_(torch.where(live, v, 0.0).unflatten(2, (8, 8)).transpose(3, 4))
+  at = live[:, 0, 0, 0] if skip else torch.ones(B * W, dtype=torch.bool, device=k.device)
+  k_out[at] = torch.where(live, k, 0.0)[at].to(k_out.dtype)
+  v_chunks(v_out)[at] = torch.where(live, v, 0.0).unflatten(2, (8, 8)).transpose(3, 4)[at].to(v_out.dtype)
 
 
 def attn_decode_mx(q, k_cache, v_cache, block_tables, ctx_lens, scale):
