@@ -851,3 +851,28 @@ def test_read_skips_cpu(fmt, Dh):
     K.kv_read_mx(s.k, s.v, s.tables, s.ctx, Dh, ko, vo, skip)
     for a, b in ((ko, k), (vo, v)):
       assert torch.equal(a[~past], b[~past]) and (a[past] == (3.0 if skip else 0.0)).all()
+
+
+def test_prompt_form_by_contexts(monkeypatch):
+  """Long portions of mxfp8 go over bf16 pages where their contexts are long, not where only the table is wide."""
+  asked = []
+  monkeypatch.setattr(K, "_gpu", lambda t: True)
+  monkeypatch.setattr(K, "mx_prompt_direct", lambda rows, pages, *a, rule=K.mx_prompt_direct: asked.append((pages, rule(rows, pages, *a))) or True)
+
+  class Bindings:
+    def attn_prompt_mx(self, *a):
+      asked.append(a[-4:-1])
+  monkeypatch.setattr(K, "require", Bindings)
+  k, v = pools("mxfp8", 2, 8, 128)
+  q = torch.zeros(2048, 32, 128, dtype=torch.bfloat16)
+  cu, tables = torch.tensor([0, 2048], dtype=torch.int32), torch.zeros(1, 2048, dtype=torch.int32)
+
+  def ask(max_ctx, q=q):
+    asked.clear()
+    K.attn_prefill_mx(q, k, v, tables, cu, cu[1:], q.shape[0], 1.0, max_ctx=max_ctx)
+    return asked[0]
+  assert ask(2048) == (32, True) and ask(2049) == (33, True) and ask(16384) == (256, False) and ask(0) == (2048, False)
+  assert ask(1 << 20) == (2048, False)  # (a bound past the table says no more than the table)
+  ask(4000, q[:8])  # few rows: parts of such a context, not of the table
+  pages_of_part, parts, _ = asked[1]
+  assert parts == K.mx_prompt_parts(8, 63) > 1 and parts * pages_of_part >= 63

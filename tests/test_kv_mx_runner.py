@@ -146,3 +146,16 @@ def test_routed_model_gpu(gpu):
   got, want = (play(runner("tiny-mixtral", gpu, d), "tiny-mixtral") for d in ("mxfp8", "bf16"))
   for a, b in zip(got, want):
     assert torch.corrcoef(torch.stack([a.flatten(), b.flatten()]))[0, 1] > 0.9
+
+
+@pytest.mark.parametrize("fmt", ("mxfp8", "bf16"))
+def test_steps_know_their_longest_context(fmt, monkeypatch):
+  seen = []
+  attention = transformer.ShardModel._attention
+
+  def looked(self, q, li, inp, *a, **kw):
+    seen.append((inp.max_ctx, int(inp.ctx_lens.max()), inp.block_tables.shape[1]))
+    return attention(self, q, li, inp, *a, **kw)
+  monkeypatch.setattr(transformer.ShardModel, "_attention", looked)
+  play(runner("tiny-llama-d64", "cpu", fmt, max_ctx=4096), "tiny-llama-d64")
+  assert len(seen) == 8 * preset("tiny-llama-d64").num_layers and all(a == b < 200 and w == 64 for a, b, w in seen)

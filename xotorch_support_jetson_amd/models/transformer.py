@@ -87,6 +87,7 @@ class StepInputs:
   # models with recurrent layers: [B] int32 state slot of each sequence (-1: padding row, nothing is read or written)
   state_slots: Optional[torch.Tensor] = None
   all_rows: bool = False  # last_idx is 0 .. T - 1 (a decode step): the rows need no gather
+  max_ctx: int = 0  # the longest of ctx_lens where the host knows it (0: whatever the tables hold)
 
   @property
   def num_tokens(self) -> int:
@@ -301,7 +302,8 @@ class ShardModel:
     if self.kv.kv_dtype != "bf16":
       if inp.decode:
         return K.attn_decode_mx(q, kc, vc, inp.block_tables, inp.ctx_lens, self.scale, ws or self.ws)
-      return K.attn_prefill_mx(q, kc, vc, inp.block_tables, inp.cu_q, inp.ctx_lens, inp.max_qlen, self.scale)
+      return K.attn_prefill_mx(q, kc, vc, inp.block_tables, inp.cu_q, inp.ctx_lens, inp.max_qlen, self.scale,
+                               max_ctx=inp.max_ctx)
     if inp.decode:
       return K.attn_decode(q, kc, vc, inp.block_tables, inp.ctx_lens, self.scale, ws or self.ws,
                            defer_merge=defer_merge, plan=plan)

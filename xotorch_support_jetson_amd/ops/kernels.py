@@ -490,21 +490,21 @@ def mx_prompt_units(T: int, B: int, max_qlen: int, G: int, Hkv: int) -> int:
   return Hkv * min(B * -(-max_qlen * G // 32), T * G // 32 + B)
 
 
-def mx_prompt_direct(rows: float, W: int, Dh: int, fp8: bool) -> bool:
-  """Whether attn_prefill_mx reads the pools themselves: not for long portions (rows of token and head, on average) behind tables of W pages
+def mx_prompt_direct(rows: float, pages: int, Dh: int, fp8: bool) -> bool:
+  """Whether attn_prefill_mx reads the pools themselves: not for long portions (rows of token and head, on average) of contexts of many pages
   in mxfp8 of 128 dims, whose values take the prompt kernel longest.  us via bf16 pages / from the pools, 32 heads on 8: 2048 tokens behind
   30000 1019 / 1077, 4096 behind 16384 1183 / 1251, 8192 behind 30000 4213 / 4625, 16384 alone 2152 / 2169, 8192 alone 580 / 556, 4096
   alone 166 / 165; 32 on 32 2048 behind 30000 1133 / 1085, 8192 behind 30000 4407 / 4672; mxfp4 4096 behind 16384 1189 / 1195, 8192 alone
   578 / 507; of 64 dims 875 / 824 and 425 / 330 (mxfp8); mxfp8, 4 of 64 behind 1000 50 / 17, one of 500 beside 63 single tokens 275 / 41."""
-  return not (fp8 and Dh == 128 and rows >= 8192 and W >= 256)
+  return not (fp8 and Dh == 128 and rows >= 8192 and pages >= 256)
 
 
-def mx_prompt_parts(units: int, W: int) -> int:
-  """Most parts of a context behind few rows.  A merge costs 2 to 5 us and pays where the units leave CUs without any and contexts are long: us in
-  1 / 2 / 3 / 4 / 8 parts, 32 heads of 128 on 8, mxfp4: 8 units (8 tokens behind 4000) 28 / 23 / 21 / 19 / 18, 64 (60 behind 1500; 8000)
-  17 / 18 / 17 / 17 / 20; 51 / 35 / 29 / 26 / 28, 128 (4 x 30 behind 4000) 29 / 26 / 29 / 27 / 39, 256 (4 x 60 behind 1500) 18 / 24 / 32 / 36 /
-  51."""
-  return max(1, min(W // (8 if units <= 32 else 16), 256 // max(1, units)))
+def mx_prompt_parts(units: int, pages: int) -> int:
+  """Most parts of a context of that many pages behind few rows.  A merge costs 2 to 5 us and pays where the units leave CUs without any and
+  contexts are long: us in 1 / 2 / 3 / 4 / 8 parts, 32 heads of 128 on 8, mxfp4: 8 units (8 tokens behind 4000) 28 / 23 / 21 / 19 / 18, 64 (60
+  behind 1500; 8000) 17 / 18 / 17 / 17 / 20; 51 / 35 / 29 / 26 / 28, 128 (4 x 30 behind 4000) 29 / 26 / 29 / 27 / 39, 256 (4 x 60 behind 1500)
+  18 / 24 / 32 / 36 / 51."""
+  return max(1, min(pages // (8 if units <= 32 else 16), 256 // max(1, units)))
 
 
 def mx_prompt_tiles(units: int, rows: float, most: int, others: float, Dh: int) -> bool:
@@ -520,11 +520,13 @@ def mx_prompt_tiles(units: int, rows: float, most: int, others: float, Dh: int) 
 
 
 def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, cu_q: torch.Tensor,
-                    ctx_lens: torch.Tensor, max_qlen: int, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
+                    ctx_lens: torch.Tensor, max_qlen: int, scale: float, out: torch.Tensor | None = None, max_ctx: int = 0) -> torch.Tensor:
   """attn_prefill over pools in 8 or 4 bits: q [T, H, Dh], the tokens cu_q[b] .. cu_q[b + 1] are the last of sequence b's ctx_lens[b] (at
   most max_qlen of them), each attends to what lies before it and itself; a token without keys gives zeros.  From the pools themselves, or
   (mx_prompt_direct) their pages are read back into bf16 scratch, a group of sequences at a time, which the bf16 prompt attention reads.
-  As there, a NaN among a later token's values reaches the earlier ones of its page (not on the CPU)."""
+  As there, a NaN among a later token's values reaches the earlier ones of its page (not on the CPU).
+  max_ctx: a bound of ctx_lens where the caller knows one (0: what the tables hold); it only chooses the form, which a wide table of short
+  contexts would mislead."""
   _mx_scale(scale)
   T, H, Dh = q.shape
   B, W = block_tables.shape
@@ -532,14 +534,15 @@ def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
   gpu = _gpu(q)
   G = max(1, H // Hkv)
   units, rows = mx_prompt_units(T, B, max_qlen, G, Hkv), T * G / max(1, B)
-  if gpu and mx_prompt_direct(rows, W, Dh, k_cache.shape[2] > PAGE * Dh):
-    nparts = mx_prompt_parts(units, W)
+  pages = min(W, -(-max_ctx // PAGE)) if max_ctx > 0 else W  # of the longest context
+  if gpu and mx_prompt_direct(rows, pages, Dh, k_cache.shape[2] > PAGE * Dh):
+    nparts = mx_prompt_parts(units, pages)
     most, others = max_qlen * G, (T - max_qlen) * G / (B - 1) if B > 1 else rows
     ws = [None] * 3
     if nparts > 1:  # few rows behind long contexts
       ws = [torch.empty(units * nparts * 32 * n, dtype=torch.float32, device=q.device) for n in (Dh, 2)]
       ws.append(torch.zeros(units, dtype=torch.int32, device=q.device))
-    return require().attn_prompt_mx(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, out, *ws, int(max_qlen), max(1, -(-W // nparts)), nparts,
+    return require().attn_prompt_mx(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, out, *ws, int(max_qlen), max(1, -(-pages // nparts)), nparts,
                                     mx_prompt_tiles(units, rows, most, others, Dh), float(scale))
   out = torch.empty_like(q) if out is None else out
   if not gpu:

@@ -265,12 +265,13 @@ class ShardRunner:
     self._reuse_staging()
     pos: List[int] = []
     slots: List[int] = []
-    cu = [0]
+    cu, most = [0], 0
     sslots = self._state_slots(rids) if self.sm is not None else None
     for rid, n in zip(rids, qlens):
       start = self.num_tokens(rid)
       if start + n > self.max_ctx:
         raise ValueError(f"request {rid}: context {start + n} exceeds max_ctx {self.max_ctx}")
+      most = max(most, start + n)
       slots += self.bm.append(rid, n)
       pos += self.model.rope_pos(start, n)
       cu.append(cu[-1] + n)
@@ -292,6 +293,7 @@ class ShardRunner:
       decode=all(q == 1 for q in qlens),
       state_slots=None if sslots is None else torch.tensor(sslots, dtype=torch.int32).to(dev, non_blocking=nb),
       all_rows=logit_rows is None and all(q == 1 for q in qlens),
+      max_ctx=most,
     )
     self._mark_staged()
     return inp
