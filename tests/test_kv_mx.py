@@ -876,3 +876,36 @@ def test_prompt_form_by_contexts(monkeypatch):
   ask(4000, q[:8])  # few rows: parts of such a context, not of the table
   pages_of_part, parts, _ = asked[1]
   assert parts == K.mx_prompt_parts(8, 63) > 1 and parts * pages_of_part >= 63
+
+
+def test_decode_form_by_contexts(monkeypatch):
+  """Parts, waves and order of single tokens by their longest context where it is known, in a table of any width."""
+  asked = []
+
+  class Bindings:
+    def attn_decode_mx(self, *a):
+      asked.append(a[9:14])
+  monkeypatch.setattr(K, "_gpu", lambda t: True)
+  monkeypatch.setattr(K, "require", Bindings)
+  k, v = pools("mxfp8", 2, 8, 128)
+  for B, n in ((1, 700), (4, 3000), (64, 5000), (512, 520), (300, 9000)):
+    q, ctx = torch.zeros(B, 32, 128, dtype=torch.bfloat16), torch.full((B,), n, dtype=torch.int32)
+    ws = K.MXDecodeWorkspace(B, 32, 8, 128, 2048 * PAGE, "meta")
+    for width, bound in ((-(-n // PAGE), 0), (2048, n), (-(-n // PAGE), 1 << 20)):
+      K.attn_decode_mx(q, k, v, torch.zeros(B, width, dtype=torch.int32), ctx, 1.0, ws, max_ctx=bound)
+    assert asked[-3] == asked[-2] == asked[-1], asked[-3:]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_contexts_past_their_bound_gpu(gpu, fmt, monkeypatch):
+  """A bound chooses the form and nothing else: results are right where contexts pass it too."""
+  s = Seqs(fmt, [1500, 33, 0, 700], 2, 128, dev=gpu, width=40)
+  for bound in (1, 64, 700, 1500, 1 << 20):
+    check_decode(s, 8, 128 ** -0.5, max_ctx=bound)
+    check_decode(s, 8, 128 ** -0.5, max_ctx=bound, ws=K.MXDecodeWorkspace(4, 8, 2, 128, 40 * PAGE, gpu))
+  new = [5, 3, 0, 9]
+  prefill = K.attn_prefill_mx
+  for bound in (1, 700, 1500):
+    monkeypatch.setattr(K, "attn_prefill_mx", lambda *a, **kw: prefill(*a, **kw, max_ctx=bound))
+    check_prompt(s, new, 8, 128 ** -0.5)

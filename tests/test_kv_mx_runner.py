@@ -159,3 +159,11 @@ def test_steps_know_their_longest_context(fmt, monkeypatch):
   monkeypatch.setattr(transformer.ShardModel, "_attention", looked)
   play(runner("tiny-llama-d64", "cpu", fmt, max_ctx=4096), "tiny-llama-d64")
   assert len(seen) == 8 * preset("tiny-llama-d64").num_layers and all(a == b < 200 and w == 64 for a, b, w in seen)
+
+
+def test_table_widths_of_graphs():
+  """Classes of block tables that decode graphs are captured with: on to the longest context where no plan cuts contexts by their lengths."""
+  assert runner("tiny-llama", "cpu", "mxfp8", max_ctx=9000, num_pages=64)._widths == [8, 16, 32, 64, 128, 141]
+  assert runner("tiny-llama", "cpu", "mxfp4", max_ctx=512, num_pages=64)._widths == [8]
+  assert runner("tiny-llama", "cpu", "bf16", max_ctx=9000, num_pages=64)._widths == [8, 16, 32, 141]
+  assert runner("tiny-llama", "cpu", "bf16", max_ctx=1024, num_pages=64)._widths == [8, 16]

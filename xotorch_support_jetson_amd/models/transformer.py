@@ -301,7 +301,7 @@ class ShardModel:
     kc, vc = self.kv.k[li], self.kv.v[li]
     if self.kv.kv_dtype != "bf16":
       if inp.decode:
-        return K.attn_decode_mx(q, kc, vc, inp.block_tables, inp.ctx_lens, self.scale, ws or self.ws)
+        return K.attn_decode_mx(q, kc, vc, inp.block_tables, inp.ctx_lens, self.scale, ws or self.ws, max_ctx=inp.max_ctx)
       return K.attn_prefill_mx(q, kc, vc, inp.block_tables, inp.cu_q, inp.ctx_lens, inp.max_qlen, self.scale,
                                max_ctx=inp.max_ctx)
     if inp.decode:

@@ -393,6 +393,13 @@ def kv_read_mx(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch
   return k_out, v_out
 
 
+def mx_pages(width: int, max_ctx: int) -> int:
+  """Pages of the longest context of tables that wide: by its bound where there is one.  What is chosen from them is right for any context,
+  and fast for those.  us by the table / by the bound, 32 heads of 128 on 8, mxfp8, 2048 pages: 64 single tokens of 1000 to 5000 207 / 69, 8 of
+  3000 68 / 18, 512 of 520 (64 heads) 315 / 104 (empty parts of a launch, none of the contexts cut, no order); a prompt of 2048 85 / 60."""
+  return min(width, -(-max_ctx // PAGE)) if max_ctx > 0 else width
+
+
 class MXDecodeWorkspace:
   """Scratch of attn_decode_mx for every batch up to max_batch at this context bound (wider tables: parts as long as the scratch allows).
   Calls that share one run one after the other: on one stream, or ordered by events."""
@@ -461,9 +468,9 @@ def mx_decode_order(batch: int, Hkv: int, parts: int) -> int:
 
 
 def attn_decode_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
-                   scale: float, ws: MXDecodeWorkspace | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                   scale: float, ws: MXDecodeWorkspace | None = None, out: torch.Tensor | None = None, max_ctx: int = 0) -> torch.Tensor:
   """attn_decode over pools in 8 or 4 bits: q [B, H, Dh], one token a sequence, attends to its first ctx_lens keys; a sequence without
-  any gives zeros."""
+  any gives zeros.  max_ctx: a bound of ctx_lens where the caller knows one (0: what the tables hold); it chooses parts, waves and order."""
   _mx_scale(scale)
   if not _gpu(q):
     y = ref.attn_decode_mx(q, k_cache, v_cache, block_tables, ctx_lens, scale)
@@ -472,13 +479,13 @@ def attn_decode_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
       return out
     return y
   B, H, Dh = q.shape
-  width = block_tables.shape[1]
+  pages = mx_pages(block_tables.shape[1], max_ctx)
   if ws is None:
-    ws = MXDecodeWorkspace(B, H, k_cache.shape[1], Dh, width * PAGE, q.device)
+    ws = MXDecodeWorkspace(B, H, k_cache.shape[1], Dh, pages * PAGE, q.device)
   elif ws.Hkv != k_cache.shape[1]:
     raise RuntimeError(f"decode workspace for {ws.Hkv} KV heads, not {k_cache.shape[1]}")
   return require().attn_decode_mx(q, k_cache, v_cache, block_tables, ctx_lens, out, ws.o, ws.ml, ws.tickets,
-                                  *ws.choose(B, width, k_cache.shape[2] > PAGE * Dh), float(scale))
+                                  *ws.choose(B, pages, k_cache.shape[2] > PAGE * Dh), float(scale))
 
 
 # scratch of attn_prefill_mx's bf16 pages: at most this much, or one sequence's
@@ -534,7 +541,7 @@ def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
   gpu = _gpu(q)
   G = max(1, H // Hkv)
   units, rows = mx_prompt_units(T, B, max_qlen, G, Hkv), T * G / max(1, B)
-  pages = min(W, -(-max_ctx // PAGE)) if max_ctx > 0 else W  # of the longest context
+  pages = mx_pages(W, max_ctx)
   if gpu and mx_prompt_direct(rows, pages, Dh, k_cache.shape[2] > PAGE * Dh):
     nparts = mx_prompt_parts(units, pages)
     most, others = max_qlen * G, (T - max_qlen) * G / (B - 1) if B > 1 else rows
