@@ -909,3 +909,46 @@ def test_contexts_past_their_bound_gpu(gpu, fmt, monkeypatch):
   for bound in (1, 700, 1500):
     monkeypatch.setattr(K, "attn_prefill_mx", lambda *a, **kw: prefill(*a, **kw, max_ctx=bound))
     check_prompt(s, new, 8, 128 ** -0.5)
+
+
+def test_prompt_pages_in_bounds(monkeypatch):
+  """Starts out of range reach the bf16 kernel, which takes them as they are, within the tokens; entries too few or too many are refused
+  whatever the form."""
+  import contextlib
+  starts = []
+
+  class Bindings:
+    def kv_read_mx(self, *a):
+      pass
+
+    def attn_prefill(self, q, k, v, tables, cu, ctx, *a):
+      starts.append((cu.tolist(), ctx.tolist(), cu.dtype, ctx.dtype))
+  monkeypatch.setattr(K, "_gpu", lambda t: True)
+  monkeypatch.setattr(K, "require", Bindings)
+  monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+  monkeypatch.setattr(K, "mx_prompt_direct", lambda *a: False)
+  k, v = pools("mxfp8", 2, 2, 128)
+  q, tables = torch.zeros(40, 4, 128, dtype=torch.bfloat16), torch.zeros(3, 2, dtype=torch.int32)
+  ctx = torch.tensor([70, -3, 130], dtype=torch.int32)
+  for cu in ([0, 30, 20, 40], [5, 5, 900, 3], [-7, 2, 3, 1 << 30]):
+    K.attn_prefill_mx(q, k, v, tables, torch.tensor(cu, dtype=torch.int32), ctx, 40, 1.0)
+    got, lens, *types = starts.pop()
+    assert got == [min(max(c, 0), 40) for c in cu] and lens == [70, 0, 130] and types == [torch.int32] * 2
+  for direct in (True, False):
+    monkeypatch.setattr(K, "mx_prompt_direct", lambda *a: direct)
+    for n, m, most in ((4, 4, 40), (3, 3, 40), (5, 3, 40), (4, 2, 40), (4, 3, 1 << 24), (4, 3, -1)):
+      with pytest.raises(RuntimeError, match="attn_prefill_mx"):
+        K.attn_prefill_mx(q, k, v, tables, torch.zeros(n, dtype=torch.int32), torch.ones(m, dtype=torch.int32), most, 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cu", [[0, 30, 20, 40], [5, 5, 900, 3], [-7, 2, 3, 1 << 30], [40, 30, 20, 10]])
+def test_starts_that_fall_pages_gpu(gpu, cu, monkeypatch):
+  """As test_starts_that_fall_gpu, over bf16 pages."""
+  monkeypatch.setattr(K, "mx_prompt_direct", lambda *a: False)
+  s = Seqs("mxfp8", [70, 33, 130], 2, 128, dev=gpu)
+  q = torch.randn(40, 4, 128, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).to(gpu)
+  whole = torch.full((80, 4, 128), 7.0, dtype=torch.bfloat16, device=gpu)
+  for most in (40, 400):
+    K.attn_prefill_mx(q, s.k, s.v, s.tables, torch.tensor(cu, dtype=torch.int32, device=gpu), s.ctx, most, 0.125, out=whole[20:60])
+    assert (whole[:20] == 7).all() and (whole[60:] == 7).all()

@@ -539,6 +539,8 @@ def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
   B, W = block_tables.shape
   Hkv = k_cache.shape[1]
   gpu = _gpu(q)
+  if ctx_lens.numel() != B or cu_q.numel() != B + 1 or not 0 <= max_qlen < 1 << 24:
+    raise RuntimeError(f"attn_prefill_mx: {B} rows of block_tables, {ctx_lens.numel()} ctx_lens, {cu_q.numel()} cu_q, max_qlen {max_qlen}")
   G = max(1, H // Hkv)
   units, rows = mx_prompt_units(T, B, max_qlen, G, Hkv), T * G / max(1, B)
   pages = mx_pages(W, max_ctx)
@@ -559,6 +561,7 @@ def attn_prefill_mx(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
   k = torch.empty(per * W, Hkv, PAGE, Dh, dtype=torch.bfloat16, device=q.device)
   v = torch.empty(per * W, Hkv, Dh, PAGE, dtype=torch.bfloat16, device=q.device)
   own = torch.empty(per, W, dtype=torch.int32, device=q.device)
+  cu_q, ctx_lens = cu_q.clamp(0, T), ctx_lens.clamp(min=0)  # (the bf16 kernel takes them as they are)
   for b in range(0, B, per):
     n = min(per, B - b)
     tables, ctx, cu = block_tables[b:b + n], ctx_lens[b:b + n], cu_q[b:b + n + 1]
