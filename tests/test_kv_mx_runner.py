@@ -167,3 +167,22 @@ def test_table_widths_of_graphs():
   assert runner("tiny-llama", "cpu", "mxfp4", max_ctx=512, num_pages=64)._widths == [8]
   assert runner("tiny-llama", "cpu", "bf16", max_ctx=9000, num_pages=64)._widths == [8, 16, 32, 141]
   assert runner("tiny-llama", "cpu", "bf16", max_ctx=1024, num_pages=64)._widths == [8, 16]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["tiny-mixtral", "tiny-llama"])
+def test_routed_projections_keep_their_order_gpu(gpu, name, monkeypatch):
+  """From 17 rows on a routed model's query, key and value projection never takes the GEMM whose sums run in another order, as
+  linear_rope_kv(wide=False) (a token whose experts are almost tied turns on the last bits); other models' may."""
+  from xotorch_support_jetson_amd.ops import linear as linear_mod
+  choose, asked = linear_mod.policy.shuffled_cfg, []
+  r = runner(name, gpu, "mxfp8", use_graphs=False)
+
+  def looked(x, w, *a, **kw):
+    if any(w is t.qkv_w for t in r.weights.layers.values()):
+      asked.append((x.shape[0], kw.get("wave", "")))
+    return choose(x, w, *a, **kw)
+  monkeypatch.setattr(linear_mod.policy, "shuffled_cfg", looked)
+  r.forward(["a", "b"], [4, 5], tokens(name, 9))
+  r.forward(["c"], [40], tokens(name, 40))
+  assert set(asked) == {(9, "y"), (40, "" if preset(name).num_experts else "y")}

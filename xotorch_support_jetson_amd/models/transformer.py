@@ -1197,8 +1197,8 @@ class ShardModel:
       else:
         # QKV projection + RoPE + paged KV write (split-K slabs reduced inside the RoPE kernel)
         if mx:  # (quantised as they are written: csrc/kv_mx.hip)
-          q = K.rope_kv_write_mx(linear(xn, lw.qkv_w, bias=lw.qkv_b), inp.positions, self.cos_sin, inp.slots, self.kv.k[j], self.kv.v[j],
-                                 c.num_heads, c.num_kv_heads)
+          q = K.rope_kv_write_mx(linear(xn, lw.qkv_w, bias=lw.qkv_b, wide=not c.num_experts), inp.positions, self.cos_sin, inp.slots,
+                                 self.kv.k[j], self.kv.v[j], c.num_heads, c.num_kv_heads)
         else:
           q = linear_rope_kv(xn, lw.qkv_w, lw.qkv_b, inp.positions, self.cos_sin, inp.slots, self.kv.k[j],
                              self.kv.v[j], c.num_heads, c.num_kv_heads, wide=not c.num_experts)

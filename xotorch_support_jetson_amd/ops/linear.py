@@ -782,9 +782,9 @@ def _pending_cfg(p: PendingNorm, w: torch.Tensor, bias, epi: str, wave: str = "y
 
 def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
            epi: str = "none", out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
-           epi_arg: float = 0.0) -> torch.Tensor:
+           epi_arg: float = 0.0, wide: bool = True) -> torch.Tensor:
   """epi "clamp_glu" (limit: epi_arg), "gelu_glu" (from BIG_MIN_M rows) and "relu2" run on pre-shuffled GPU weights with bf16
-  output only."""
+  output only.  wide=False: as linear_rope_kv's."""
   if isinstance(x, PendingNorm):
     cfg = None if (residual is not None or (out_dtype not in (None, torch.bfloat16))
                    or (out is not None and out.dtype != torch.bfloat16)) else _pending_cfg(x, w, bias, epi)
@@ -809,7 +809,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, r
     out = torch.empty(M, N // 2 if epi in K.GLU_EPI else N, dtype=dt, device=x.device)
   if x.stride(1) != 1 or x.stride(0) % 8:
     x = x.contiguous()
-  cfg = policy.shuffled_cfg(x, w, bias, residual, epi, dt, wave="y")
+  cfg = policy.shuffled_cfg(x, w, bias, residual, epi, dt, wave="y" if wide or M <= WAVE_MAX_M else "")
   _shuffled_call(x, w, bias, residual, epi, out, cfg, epi_arg)
   return out
 
