@@ -952,3 +952,27 @@ def test_starts_that_fall_pages_gpu(gpu, cu, monkeypatch):
   for most in (40, 400):
     K.attn_prefill_mx(q, s.k, s.v, s.tables, torch.tensor(cu, dtype=torch.int32, device=gpu), s.ctx, most, 0.125, out=whole[20:60])
     assert (whole[:20] == 7).all() and (whole[60:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,Dh", [("mxfp4", 128), ("mxfp8", 128), ("mxfp4", 64), ("mxfp8", 64)])
+def test_long_contexts_gpu(gpu, fmt, Dh):
+  """Contexts past 128 pages as the rule itself cuts them, beside short ones; a workspace made for shorter ones; a few new tokens behind them."""
+  s = Seqs(fmt, [32000, 33, 0, 8256], 1, Dh, dev=gpu)
+  assert K.MXDecodeWorkspace.parts(4, 1, 500)[1] > 4
+  for max_ctx in (32000, 4096, 64):
+    check_decode(s, 4, Dh ** -0.5, ws=K.MXDecodeWorkspace(4, 4, 1, Dh, max_ctx, gpu))
+  check_decode(s, 4, Dh ** -0.5)
+  check_prompt(s, [3, 5, 0, 9], 4, Dh ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_long_context_among_many_gpu(gpu, fmt):
+  """Pairs enough to fill the chip uncut: a context past 128 pages is cut all the same, the others stay whole."""
+  lens = [5 + 7 * (b % 9) for b in range(64)]
+  lens[40] = 9000
+  s = Seqs(fmt, lens, 8, 64, dev=gpu)
+  assert K.MXDecodeWorkspace.parts(64, 8, 141) == (71, 2)
+  check_decode(s, 16, 0.125)
+  check_decode(s, 16, 0.125, ws=K.MXDecodeWorkspace(64, 16, 8, 64, 4096, gpu))
