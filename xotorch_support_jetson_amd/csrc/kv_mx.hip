@@ -545,7 +545,10 @@ struct Rows {
   }
   // The page's weights in bf16, B operands of the products with its values; what the rows have so far is brought to the new maxima.
   // Weights are 2^fma(score, scale, -m): the product unrounded, m the largest one rounded.  Past 2^24 the two differ by more than 1, soon by
-  // hundreds, and all weights of a row would overflow or vanish: the scores there are scaled, with m's rounding, before m is taken from them.
+  // hundreds, and all weights of a row overflow or vanish: the scores of far rows are scaled, with m's rounding, before m is taken from them.
+  // Single tokens branch (no slower); prompts, from whose registers a branch takes too many (one prompt of 4096 in mxfp8 of 64 dims 94 / 119 us),
+  // leave far rows to a second pass over the unit with FARS (95 us; 8 prompts of 100 to 900 2 % slower).
+  template <bool FARS>
   __device__ __forceinline__ void weights(f32x4 (&st)[NB][4], float scale_log2, s16x8 (&pf)[NB][2]) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -568,7 +571,12 @@ struct Rows {
         }
       }
       float scale = scale_log2;
-      if (__ballot(fabsf(m[nb]) > FAR)) {
+      if constexpr (FARS) {
+#pragma clang fp contract(off)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) st[nb][t] *= scale_log2;
+        scale = 1.f;
+      } else if (!ONES && __ballot(fabsf(m[nb]) > FAR)) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) st[nb][t] *= scale_log2;
         scale = 1.f;
@@ -590,10 +598,10 @@ struct Rows {
     }
   }
   // The page's weights and their products with its values; vv(kk, v, vs): eight keys' units and scales.
-  template <class V>
+  template <bool FARS, class V>
   __device__ __forceinline__ void weigh(V vv, f32x4 (&st)[NB][4], float scale_log2) {
     s16x8 pf[NB][2];
-    weights(st, scale_log2, pf);
+    weights<FARS>(st, scale_log2, pf);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       u32x4 v[R::VU], vs[R::VS];
@@ -620,6 +628,13 @@ struct Rows {
         l[nb] = xor_sum<32>(l[nb]);
       }
     }
+  }
+  // Whether some row of the wave is far, or was and overflowed before a larger score came (behind finish; sums of others stay below 2^9 a key)
+  __device__ __forceinline__ bool far() const {
+    bool bad = false;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) bad |= m[nb] > NEG_BIG && (fabsf(m[nb]) > FAR || !(l[nb] < 0x1p40f));
+    return __ballot(bad) != 0;
   }
   // four neighbouring dims of block nb's row c: 32 j + 8 g + 4 half ..
   __device__ __forceinline__ f32x4 dims(int nb, int j, int half) const {
@@ -658,7 +673,8 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : FP8 || REFILL ||
   } else if (A.order != 0) {
     q0 = b = sequence_at(A, bu);
   }
-  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, G = A.H / A.Hkv;
+  int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int G = A.H / A.Hkv;
   const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int qlen = PROMPT ? max(q1 - q0, 0) : 1, nrows = qlen * G;
   if (PROMPT && row0 >= nrows) return;
@@ -673,15 +689,19 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : FP8 || REFILL ||
 
   Rows<DH, FP8, NB, PROMPT> rows;
   int sees[NB];  // the last key of the lane's row
+
+  // the queries, and what follows from the lane
+  auto lanes = [&] {
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int row = row0 + 16 * nb + c, ti = PROMPT ? min(row, nrows - 1) / G : 0, hq = PROMPT ? min(row, nrows - 1) - ti * G : min(c, G - 1);
-    sees[nb] = pos0 + ti;
-    rows.query(nb, A.q + ((size_t)(q0 + ti) * A.H + kvh * G + hq) * DH + 16 * g, row < nrows, g);
-  }
+    for (int nb = 0; nb < NB; ++nb) {
+      const int row = row0 + 16 * nb + c, ti = PROMPT ? min(row, nrows - 1) / G : 0, hq = PROMPT ? min(row, nrows - 1) - ti * G : min(c, G - 1);
+      sees[nb] = pos0 + ti;
+      rows.query(nb, A.q + ((size_t)(q0 + ti) * A.H + kvh * G + hq) * DH + 16 * g, row < nrows, g);
+    }
+  };
+  lanes();
 
   const int32_t* bt = A.tables + (size_t)b * A.width;
-  const int krow = 8 * (c >> 2) + (c & 3);
   auto page_of = [&](int p) -> long { return min(max(bt[min(p, last - 1)], 0), A.num_pages - 1); };  // (last > first)
   // (read once a launch: non-temporal, as fast as plain loads for small caches and up to 11 % faster for large ones)
   auto ld = [](const uint8_t* p) -> u32x4 {
@@ -691,7 +711,7 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : FP8 || REFILL ||
   // (512 contexts of 525 tokens end 13 tokens into a page)
   auto load_k = [&](int p, long page, R& x) {
     const uint8_t* kp = A.kc + ((size_t)page * A.Hkv + kvh) * M::BYTES;
-    const int end = min(ctx - 1 - p * PAGE, PAGE - 1);
+    const int end = min(ctx - 1 - p * PAGE, PAGE - 1), krow = 8 * (c >> 2) + (c & 3);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -718,7 +738,7 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : FP8 || REFILL ||
       for (int i = 0; i < R::KV; ++i) k[i] = x.k[t][i];
     }, x.ks, st);
   };
-  auto weigh = [&](int p, f32x4 (&st)[NB][4]) {
+  auto weigh = [&](auto far, int p, f32x4 (&st)[NB][4]) {
     const int left = ctx - p * PAGE - 8 * g;  // keys of the context from the lane's first on
     // keys that some row does not see: past the context (the last page), or past a new token
     if ((PROMPT ? pos0 + row0 / G + 1 : ctx) - p * PAGE < PAGE) {
@@ -727,7 +747,7 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : FP8 || REFILL ||
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) cut_values<DH, FP8>(x.v[kk], x.vs[kk], left - 32 * kk);
     }
-    rows.weigh([&](int kk, u32x4 (&v)[R::VU], u32x4 (&vs)[R::VS]) {
+    rows.template weigh<decltype(far)::value>([&](int kk, u32x4 (&v)[R::VU], u32x4 (&vs)[R::VS]) {
 #pragma unroll
       for (int u = 0; u < R::VU; ++u) v[u] = x.v[kk][u];
 #pragma unroll
@@ -742,12 +762,13 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : FP8 || REFILL ||
     nxt = page_of(first + wave + NW);
   }
   for (int p = first + wave; p < last; p += NW) {
+    const std::false_type near;
     f32x4 st[NB][4];
     if constexpr (REFILL) {
       const bool more = p + NW < last;
       scores(st);
       if (more) load_k(p + NW, nxt, x);
-      weigh(p, st);
+      weigh(near, p, st);
       if (more) load_v(p + NW, nxt, x);
       nxt = page_of(p + 2 * NW);
     } else {
@@ -755,10 +776,26 @@ __global__ __launch_bounds__(64 * NW, NB > 1 && DH == 128 ? 2 : FP8 || REFILL ||
       load_v(p, nxt, x);
       nxt = page_of(p + NW);
       scores(st);
-      weigh(p, st);
+      weigh(near, p, st);
     }
   }
   rows.finish();
+  if constexpr (PROMPT)
+    if (__builtin_expect(rows.far(), 0)) {
+      asm volatile("" : "+v"(lane));  // (what follows from the lane is found anew: none of it is kept through the first pass)
+      g = lane >> 4;
+      c = lane & 15;
+      lanes();
+      for (int p = first + wave; p < last; p += NW) {
+        f32x4 st[NB][4];
+        const long at = page_of(p);
+        load_k(p, at, x);
+        load_v(p, at, x);
+        scores(st);
+        weigh(std::true_type{}, p, st);
+      }
+      rows.finish();
+    }
 
   const size_t row_ws = ((size_t)bu * A.nparts * A.Hkv + kvh) * RS, step = (size_t)A.Hkv * RS;  // partial results: part 0's first row, from part to part
   auto result = [&](int rw, int d, const f32x4& O, float inv) {
@@ -883,7 +920,7 @@ struct PromptLds {
   static constexpr int N = (2 * NCH + NW - 1) / NW;                // loads a wave and page
   static constexpr int RAW = NCH * 1024;
   static constexpr int VBUF = PAGE * DH * 2;                 // values in bf16: [half of the keys][group][even / odd][eight keys][16 dims][8]
-  static constexpr int K0 = 0, V0 = (AHEAD + 2) * RAW, B0 = V0 + (AHEAD + 1) * RAW, TOTAL = B0 + 2 * VBUF;
+  static constexpr int K0 = 0, V0 = (AHEAD + 2) * RAW, B0 = V0 + (AHEAD + 1) * RAW, FLAGS = B0 + 2 * VBUF, TOTAL = FLAGS + 64;
 };
 // which pieces of row r change places: x of its piece r (row / 16) + i becomes that number ^ x
 template <int DH, bool FP8>
@@ -902,7 +939,8 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 4) void attn_prompt_mx_kerne
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const PromptWork work = prompt_work(A.ctx_lens);
   const int b = __builtin_amdgcn_readfirstlane(work.seq), kvh = work.head, row0 = work.tile * 128;
-  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, G = A.H / A.Hkv;
+  int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int G = A.H / A.Hkv;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q0 = min(max(A.cu_q[b], 0), A.T), qlen = min(max(A.cu_q[b + 1], q0), A.T) - q0, nrows = qlen * G;
   if (row0 >= nrows) return;  // the whole workgroup
@@ -913,13 +951,15 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 4) void attn_prompt_mx_kerne
 
   // this lane's pieces of a page: load i of the wave brings chunk ch of the keys' or (from NCH on) the values' bytes
   int from[L::N], chunk[L::N];
+  auto pieces = [&] {
 #pragma unroll
-  for (int i = 0; i < L::N; ++i) {
-    chunk[i] = min(L::N * wave + i, 2 * L::NCH - 1);  // (one too many: the last again)
-    const bool v = chunk[i] >= L::NCH;
-    const int at = min(64 * (v ? chunk[i] - L::NCH : chunk[i]) + lane, L::KG - 1);  // (past the page: its last piece again)
-    from[i] = 16 * (v || at >= M::ELEMS / 16 ? at : at ^ mx_swizzle<DH, FP8>(at / RG));
-  }
+    for (int i = 0; i < L::N; ++i) {
+      chunk[i] = min(L::N * wave + i, 2 * L::NCH - 1);  // (one too many: the last again)
+      const bool v = chunk[i] >= L::NCH;
+      const int at = min(64 * (v ? chunk[i] - L::NCH : chunk[i]) + lane, L::KG - 1);  // (past the page: its last piece again)
+      from[i] = 16 * (v || at >= M::ELEMS / 16 ? at : at ^ mx_swizzle<DH, FP8>(at / RG));
+    }
+  };
   // the table's entries as scalar loads, one page ahead of the loads that need them (a vector load there would be waited for behind the
   // pages in flight)
   typedef const __attribute__((address_space(4))) int32_t* table_t;
@@ -933,7 +973,9 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 4) void attn_prompt_mx_kerne
 #pragma unroll
     for (int i = 0; i < L::N; ++i) {
       const bool v = chunk[i] >= L::NCH;
-      __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)((v ? vp : kp) + (uint32_t)from[i]),
+      uint32_t at = from[i];
+      if constexpr (DH == 64) asm volatile("" : "+v"(at));  // (else it becomes a 64-bit constant of the loop, and a register too many is spilled)
+      __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)((v ? vp : kp) + at),
                                        (__attribute__((address_space(3))) void*)((v ? vd - L::NCH * 1024 : kd) + chunk[i] * 1024), 16, 0, 0);
     }
   };
@@ -969,75 +1011,95 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 4) void attn_prompt_mx_kerne
     asm volatile("" ::: "memory");
   };
 
-#pragma unroll
-  for (int p = 0; p <= AHEAD; ++p)
-    if (p < pages) issue(p, page_of(p));
   Rows<DH, FP8, NB, true> rows;
   int sees[NB];
+  auto run = [&](auto far) {
+    if constexpr (decltype(far)::value) {  // (what follows from the lane is found anew: none of it is kept through the first pass)
+      asm volatile("" : "+v"(lane));
+      g = lane >> 4;
+      c = lane & 15;
+    }
+    pieces();
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int row = min(wrow0 + 16 * nb + c, nrows - 1), ti = row / G;
-    sees[nb] = pos0 + ti;
-    rows.query(nb, A.q + ((size_t)(q0 + ti) * A.H + kvh * G + row - ti * G) * DH + 16 * g, wrow0 + 16 * nb + c < nrows, g);
-  }
-  int nxt = pages > AHEAD + 1 ? page_of(AHEAD + 1) : 0;
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the queries came behind the first pages)
-  meet();
-  if (pages > 0) make_values(0);
-  for (int p = 0; p < pages; ++p) {
-    if (AHEAD > 1 && p + AHEAD < pages)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * L::N) : "memory");  // this wave's share of page p + 1 has landed
-    else
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    for (int p = 0; p <= AHEAD; ++p)
+      if (p < pages) issue(p, page_of(p));
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int row = min(wrow0 + 16 * nb + c, nrows - 1), ti = row / G;
+      sees[nb] = pos0 + ti;
+      rows.query(nb, A.q + ((size_t)(q0 + ti) * A.H + kvh * G + row - ti * G) * DH + 16 * g, wrow0 + 16 * nb + c < nrows, g);
+    }
+    int nxt = pages > AHEAD + 1 ? page_of(AHEAD + 1) : 0;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the queries came behind the first pages)
     meet();
-    if (p + 1 + AHEAD < pages) {
-      issue(p + 1 + AHEAD, nxt);
-      nxt = page_of(p + 2 + AHEAD);
+    if (pages > 0) make_values(0);
+    for (int p = 0; p < pages; ++p) {
+      if (AHEAD > 1 && p + AHEAD < pages)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * L::N) : "memory");  // this wave's share of page p + 1 has landed
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      meet();
+      if (p + 1 + AHEAD < pages) {
+        issue(p + 1 + AHEAD, nxt);
+        nxt = page_of(p + 2 + AHEAD);
+      }
+      if (p + 1 < pages) make_values(p + 1);
+      if (p * PAGE > wmax) continue;  // every row of this wave is before the page
+      const uint8_t* kr = lds + L::K0 + p % (AHEAD + 2) * L::RAW;
+      const uint8_t* vb = lds + L::B0 + (p & 1) * L::VBUF;
+      f32x4 st[NB][4];
+      rows.scores([&](int t, u32x4 (&k)[R::KV]) {
+        const int r = 32 * (t >> 1) + 4 * (t & 1) + 8 * (c >> 2) + (c & 3);
+#pragma unroll
+        for (int i = 0; i < R::KV; ++i)
+          k[i] = *reinterpret_cast<const u32x4*>(kr + 16 * ((r * RG + (DH == 64 && !FP8 ? g & 1 : g) + 4 * i) ^ mx_swizzle<DH, FP8>(r)));
+      }, *reinterpret_cast<const uint32_t*>(kr + M::ELEMS + 64 * (g & (J - 1)) + 4 * c), st);
+      if (wmin + 1 - p * PAGE < PAGE) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) rows.mask(st[nb], sees[nb] + 1 - p * PAGE - 8 * g);
+      }
+      s16x8 pf[NB][2];
+      rows.template weights<decltype(far)::value>(st, A.scale_log2, pf);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const s16x8 v = ld16(vb + ((kk * J + j) * 2 + e) * 1024 + g * 256 + 16 * c);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) rows.o[nb][j][e] = mfma16(v, pf[nb][kk], rows.o[nb][j][e]);
+          }
     }
-    if (p + 1 < pages) make_values(p + 1);
-    if (p * PAGE > wmax) continue;  // every row of this wave is before the page
-    const uint8_t* kr = lds + L::K0 + p % (AHEAD + 2) * L::RAW;
-    const uint8_t* vb = lds + L::B0 + (p & 1) * L::VBUF;
-    f32x4 st[NB][4];
-    rows.scores([&](int t, u32x4 (&k)[R::KV]) {
-      const int r = 32 * (t >> 1) + 4 * (t & 1) + 8 * (c >> 2) + (c & 3);
+    rows.finish();
+  };
+  run(std::false_type{});
+  const bool again = rows.far();
+  uint32_t* flags = reinterpret_cast<uint32_t*>(lds + L::FLAGS);
+  if (lane == 0) flags[wave] = again;
+  meet();  // (every page has landed and is read)
+  uint32_t any = 0;
 #pragma unroll
-      for (int i = 0; i < R::KV; ++i)
-        k[i] = *reinterpret_cast<const u32x4*>(kr + 16 * ((r * RG + (DH == 64 && !FP8 ? g & 1 : g) + 4 * i) ^ mx_swizzle<DH, FP8>(r)));
-    }, *reinterpret_cast<const uint32_t*>(kr + M::ELEMS + 64 * (g & (J - 1)) + 4 * c), st);
-    if (wmin + 1 - p * PAGE < PAGE) {
+  for (int w = 0; w < L::NW; ++w) any |= flags[w];
+  if (__builtin_expect(__builtin_amdgcn_readfirstlane(any) != 0, 0)) run(std::true_type{});
+  if (wmin < 0) {  // rows without keys: what they weighed with 0 may have been NaN
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) rows.mask(st[nb], sees[nb] + 1 - p * PAGE - 8 * g);
-    }
-    s16x8 pf[NB][2];
-    rows.weights(st, A.scale_log2, pf);
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int j = 0; j < J; ++j)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const s16x8 v = ld16(vb + ((kk * J + j) * 2 + e) * 1024 + g * 256 + 16 * c);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) rows.o[nb][j][e] = mfma16(v, pf[nb][kk], rows.o[nb][j][e]);
-        }
+        for (int e = 0; e < 2; ++e) rows.o[nb][j][e] = sees[nb] >= 0 ? rows.o[nb][j][e] : f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  rows.finish();
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const int row = wrow0 + 16 * nb + c, ti = row / G;
     if (row >= nrows) continue;
-    const bool keys = pos0 + ti >= 0;  // without any: zeros (its sums are, or NaN where values of the page are)
-    const float inv = 1.f / rows.l[nb];
+    const float inv = pos0 + ti >= 0 ? 1.f / rows.l[nb] : 0.f;  // a row without keys: zeros (its sums are)
     uint16_t* p = A.out + ((size_t)(q0 + ti) * A.H + kvh * G + row - ti * G) * DH + 8 * g;
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint16_t* to = p + 32 * j + 4 * half;
-        if (keys) st_results(to, rows.dims(nb, j, half), inv);
-        else *reinterpret_cast<s16x4*>(to) = s16x4{0, 0, 0, 0};
-      }
+      for (int half = 0; half < 2; ++half) st_results(p + 32 * j + 4 * half, rows.dims(nb, j, half), inv);
   }
 }
 
