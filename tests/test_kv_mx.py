@@ -976,3 +976,32 @@ def test_long_context_among_many_gpu(gpu, fmt):
   assert K.MXDecodeWorkspace.parts(64, 8, 141) == (71, 2)
   check_decode(s, 16, 0.125)
   check_decode(s, 16, 0.125, ws=K.MXDecodeWorkspace(64, 16, 8, 64, 4096, gpu))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,Dh", [("mxfp4", 128), ("mxfp8", 128), ("mxfp4", 64), ("mxfp8", 64)])
+def test_far_rows_among_others_gpu(gpu, fmt, Dh, monkeypatch):
+  """Far rows in some waves of a unit only, results where their queries were: the same as far rows and others by themselves."""
+  H, Hkv = 4, 2
+  s = Seqs(fmt, [300, 90], Hkv, Dh, dev=gpu)
+  q = torch.randn(390, H, Dh, generator=torch.Generator().manual_seed(5))
+  q[17], q[40:60], q[389, 1] = q[17] * 2.0 ** 90, q[40:60] * 2.0 ** 40, q[389, 1] * 2.0 ** 30
+  q = q.to(torch.bfloat16)
+  cu = torch.tensor([0, 300, 390], dtype=torch.int32, device=gpu)
+  for tiles in (True, False):
+    monkeypatch.setattr(K, "mx_prompt_tiles", lambda *a: tiles)
+    whole = K.attn_prefill_mx(q.to(gpu), s.k, s.v, s.tables, cu, s.ctx, 300, 0.1)
+    own = q.to(gpu)
+    assert torch.equal(K.attn_prefill_mx(own, s.k, s.v, s.tables, cu, s.ctx, 300, 0.1, out=own), whole)
+    assert torch.isfinite(whole).all()
+    for rows, b, past in ((slice(0, 17), 0, 0), (slice(18, 40), 0, 18), (slice(60, 300), 0, 60), (slice(300, 389), 1, 0)):
+      n = rows.stop - rows.start
+      kv = [t[:past + n] for t in s.kv[b]]
+      close(whole[rows], *attend64(q[rows], *kv, 0.1, past))
+    for t, h in ((17, 0), (45, 3), (389, 1)):  # a far row takes its largest score's value: scores apart by far more than their error
+      b, past = (0, t) if t < 300 else (1, t - 300)
+      k, v = (x[:past + 1, h // (H // Hkv)] for x in s.kv[b])
+      score = k @ q[t, h].double()
+      first, second = score.topk(2).values
+      if first - second > 2.0 ** -12 * (k.abs() @ q[t, h].double().abs()).max():
+        assert torch.allclose(whole[t, h].double().cpu(), v[score.argmax()], rtol=2.0 ** -8, atol=0)

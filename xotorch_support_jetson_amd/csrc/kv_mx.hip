@@ -547,7 +547,7 @@ struct Rows {
   // Weights are 2^fma(score, scale, -m): the product unrounded, m the largest one rounded.  Past 2^24 the two differ by more than 1, soon by
   // hundreds, and all weights of a row overflow or vanish: the scores of far rows are scaled, with m's rounding, before m is taken from them.
   // Single tokens branch (no slower); prompts, from whose registers a branch takes too many (one prompt of 4096 in mxfp8 of 64 dims 94 / 119 us),
-  // leave far rows to a second pass over the unit with FARS (95 us; 8 prompts of 100 to 900 2 % slower).
+  // leave far rows to a second pass over the unit with FARS (95 us; others within 1.5 %).
   template <bool FARS>
   __device__ __forceinline__ void weights(f32x4 (&st)[NB][4], float scale_log2, s16x8 (&pf)[NB][2]) {
 #pragma unroll
@@ -1073,33 +1073,39 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 4) void attn_prompt_mx_kerne
     }
     rows.finish();
   };
+  auto store = [&] {
+    if (wmin < 0) {  // rows without keys: what they weighed with 0 may have been NaN
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) rows.o[nb][j][e] = sees[nb] >= 0 ? rows.o[nb][j][e] : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int row = wrow0 + 16 * nb + c, ti = row / G;
+      if (row >= nrows) continue;
+      const float inv = pos0 + ti >= 0 ? 1.f / rows.l[nb] : 0.f;  // a row without keys: zeros (its sums are)
+      uint16_t* p = A.out + ((size_t)(q0 + ti) * A.H + kvh * G + row - ti * G) * DH + 8 * g;
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) st_results(p + 32 * j + 4 * half, rows.dims(nb, j, half), inv);
+    }
+  };
   run(std::false_type{});
   const bool again = rows.far();
   uint32_t* flags = reinterpret_cast<uint32_t*>(lds + L::FLAGS);
   if (lane == 0) flags[wave] = again;
+  if (!again) store();  // (once: a result may lie where its row's queries were)
   meet();  // (every page has landed and is read)
   uint32_t any = 0;
 #pragma unroll
   for (int w = 0; w < L::NW; ++w) any |= flags[w];
-  if (__builtin_expect(__builtin_amdgcn_readfirstlane(any) != 0, 0)) run(std::true_type{});
-  if (wmin < 0) {  // rows without keys: what they weighed with 0 may have been NaN
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) rows.o[nb][j][e] = sees[nb] >= 0 ? rows.o[nb][j][e] : f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int row = wrow0 + 16 * nb + c, ti = row / G;
-    if (row >= nrows) continue;
-    const float inv = pos0 + ti >= 0 ? 1.f / rows.l[nb] : 0.f;  // a row without keys: zeros (its sums are)
-    uint16_t* p = A.out + ((size_t)(q0 + ti) * A.H + kvh * G + row - ti * G) * DH + 8 * g;
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) st_results(p + 32 * j + 4 * half, rows.dims(nb, j, half), inv);
+  if (__builtin_expect(__builtin_amdgcn_readfirstlane(any) != 0, 0)) {
+    run(std::true_type{});
+    if (again) store();
   }
 }
 
