@@ -1,4 +1,4 @@
-// A paged KV cache in 8 or 4 bits: written as keys are rotated, read back, and read by the attention of single tokens.
+// A paged KV cache in 8 or 4 bits: written as keys are rotated, read back, and read by the attention of single tokens and of prompts.
 //
 // Format.  A head's row of DH dims in groups of 32.  Each group has one power of two as its scale (a byte: exponent + 127; 255: the
 // group held a NaN or an infinity and reads back as NaN) and elements of e2m1 (0 .5 1 1.5 2 3 4 6) or e4m3.  The exponent is the
@@ -325,8 +325,8 @@ __global__ __launch_bounds__(256) void kv_read_mx_kernel(const uint8_t* __restri
 // & 1) + r, so that a lane's scores of tiles 2 kk and 2 kk + 1 are the eight keys 32 kk + 8 g .. that it holds in the B operand of
 // O^T = V^T . P^T: probabilities stay in their registers.
 // Values: two e2m1 / e4m3 of a key become two bf16 (exact, scaled on the way), and two keys' pairs change halves: tile (j, e) of O^T
-// has dims 32 j + 2 row + e.  P is rounded to bf16, the values' own
-// type; sums, maxima and the output are fp32.
+// has dims 32 j + 2 row + e.  P is rounded to bf16 (2^-8 of a weight at most): the values' own type, the widest that the unit multiplies at
+// this rate, and what attention over a bf16 cache does; sums, maxima and the output before its rounding are fp32.
 template <int DH, bool FP8>
 struct PageRegs {
   using M = Mx<DH, FP8>;
@@ -949,12 +949,14 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 4) void attn_prompt_mx_kerne
   const int wrow0 = row0 + 16 * NB * wave, wend = min(wrow0 + 16 * NB, nrows);
   const int wmin = pos0 + wrow0 / G, wmax = wend > wrow0 ? pos0 + (wend - 1) / G : -1;  // last keys of the wave's first and last rows
 
-  // this lane's pieces of a page: load i of the wave brings chunk ch of the keys' or (from NCH on) the values' bytes
+  // this lane's pieces of a page: load i of the wave brings chunk ch of the keys' or (from NCH on) the values' bytes.  Every wave has N loads in
+  // flight, which the waits count, so the waves' loads are more than the chunks: of 128 dims 16 for 10 (mxfp4) and 24 for 18, of 64 8 for 6 and
+  // 12 for 10; the surplus brings the last chunk's bytes once more
   int from[L::N], chunk[L::N];
   auto pieces = [&] {
 #pragma unroll
     for (int i = 0; i < L::N; ++i) {
-      chunk[i] = min(L::N * wave + i, 2 * L::NCH - 1);  // (one too many: the last again)
+      chunk[i] = min(L::N * wave + i, 2 * L::NCH - 1);  // (past the last chunk: that again)
       const bool v = chunk[i] >= L::NCH;
       const int at = min(64 * (v ? chunk[i] - L::NCH : chunk[i]) + lane, L::KG - 1);  // (past the page: its last piece again)
       from[i] = 16 * (v || at >= M::ELEMS / 16 ? at : at ^ mx_swizzle<DH, FP8>(at / RG));

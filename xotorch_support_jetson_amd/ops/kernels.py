@@ -518,11 +518,13 @@ def mx_prompt_tiles(units: int, rows: float, most: int, others: float, Dh: int) 
   """Which kernel (csrc/kv_mx.hip) takes sequences of `rows` rows (new tokens x query heads of a KV head) on average, at most `most`, all but
   one such of `others`: a unit's waves share its pages, where the units are few or some sequences' rows; or (True) four units lie together in
   a workgroup, whose pages and bf16 values are in LDS.  us, 32 heads on 8, mxfp4, of 128 dims, units apart / together: 256 units (4 sequences
-  of 64 new tokens behind 1000) 15 / 29, 704 (700 behind 700) 29 / 37, 768 (24 of 30 behind 300) 20 / 16, 800 (100 of 8 behind 500) 26 / 35, 1000
-  (one) 27 / 28, 1536 (12 of 128 behind 1000) 50 / 45, 2048 (one; 4 of 512) 63 / 55 and 39 / 26, 2864 (1500, 700, 6 of 100) 65 / 45,
-  6144 (12 of 512) 107 / 56; beside 63 single tokens behind 1000 one of 500 29 / 114, of 4000 188 / 249; beside 511 one of 2000 195 / 594.  Of
-  64 dims, where few prompts' longest workgroups run alone: 256 10 / 24, 768 11 / 13, 832 (8 of 100) 11 / 8, 1000 17 / 24, 2000 (2 of 1000)
-  29 / 31, 2048 (one; 4 of 512) 39 / 43 and 23 / 19, 6144 58 / 36."""
+  of 64 new tokens behind 1000) 15 / 30, 704 (700 behind 700) 28 / 36, 768 (24 of 30 behind 300) 19 / 16, 800 (100 of 8 behind 500) 25 / 35, 832
+  (8 of 100) 18 / 10, 1536 (12 of 128 behind 1000) 50 / 46, 2000 (2 of 1000) 44 / 41, 2048 (one; 4 of 512) 60 / 55 and 38 / 27, 2864 (1500, 700,
+  6 of 100) 62 / 45, 6144 (12 of 512 behind 1000) 193 / 149; beside 63 single tokens behind 1000 one of 500 26 / 119, of 4000 192 / 255; beside
+  511 one of 2000 193 / 597.  Of 64 dims, where few prompts' longest workgroups run alone: 256 10 / 25, 832 11 / 9, 1000 (one) 17 / 24, 2000 27 /
+  31, 2048 38 / 43 and 23 / 19, 2864 37 / 35, 6144 115 / 92.  It is wrong for one prompt of 1000 (26 / 29; mxfp8 28 / 30), for one query head a KV
+  head and lone prompts up to 2048 (32 on 32: 1000 26 / 29, 2048 61 / 71; of 64 dims 17 / 24, 37 / 54), and in 64 dims by 10 to 30 % for 24 of
+  30 behind 300, 12 of 128 behind 1000 and (64 heads on 8, mxfp8) 100 of 8 behind 500."""
   return units >= 768 and others >= 64 and most <= 8 * rows and (Dh == 128 or rows <= 2048 or units > 2048)
 
 
