@@ -186,3 +186,35 @@ def test_routed_projections_keep_their_order_gpu(gpu, name, monkeypatch):
   r.forward(["a", "b"], [4, 5], tokens(name, 9))
   r.forward(["c"], [40], tokens(name, 40))
   assert set(asked) == {(9, "y"), (40, "" if preset(name).num_experts else "y")}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_graphs_of_wider_tables_gpu(gpu, fmt):
+  """Replayed steps across the classes past 32 pages against eager ones whose forms are chosen for the same class (so that sums run in the same
+  order: what quantising makes of another order's rounding is in test_same_values_gpu)."""
+  name = "tiny-llama"
+  g, e = (runner(name, gpu, fmt, max_ctx=9000, max_batch=2, num_pages=200, use_graphs=u) for u in (None, False))
+  prepare = e._prepare
+
+  def by_class(*a):
+    inp = prepare(*a)
+    if inp.decode:
+      inp.max_ctx = 64 * next(w for w in g._widths if 64 * w >= inp.max_ctx)
+    return inp
+  e._prepare = by_class
+  ids = tokens(name, 4090)
+  for r in (g, e):
+    r.forward(["a"], [2045], ids[:2045])
+    r.forward(["b"], [70], ids[:70])
+
+  def step(x):
+    a, b = g.forward(["a", "b"], [1, 1], x).clone(), e.forward(["a", "b"], [1, 1], x)
+    assert torch.isfinite(a).all() and torch.allclose(a, b, atol=2e-2, rtol=2e-2)
+  for i in range(6):  # 2046 to 2051 tokens: 32 pages, then 33
+    step(ids[i:i + 2])
+  assert [w for _, w in g._graphs] == [32, 64]
+  for r in (g, e):
+    r.forward(["a"], [2050], ids[2000:4050])
+  step(ids[9:11])
+  assert [w for _, w in g._graphs] == [32, 64, 128]

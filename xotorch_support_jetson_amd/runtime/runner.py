@@ -174,7 +174,8 @@ class ShardRunner:
     # plus a merge pass
     # (16 pages: the widest table the 8-wave single-partition attention takes at small batch, ops/kernels.py)
     # A cache in 8 or 4 bits has no plan by the contexts (ops/kernels.py plan_pays) that would make a wide table cheap: the classes go on,
-    # each twice the last (8 sequences of 3000 tokens, 32 heads of 128 on 8, mxfp8: 18 us in 47 pages, 23 in 128, 30 in 256, 68 in 2048)
+    # each twice the last (8 sequences of 3000 tokens, 32 heads of 128 on 8, mxfp8: 18 us in 47 pages, 23 in 128, 30 in 256, 68 in 2048;
+    # Llama-3-8B's step of 8 at 2900 tokens and max_ctx 131072 3.5 ms, 5.2 without them, bf16 3.6).  A class costs a capture: 12 ms and 58 MB there
     most = self.width if self.kv_dtype != "bf16" else 33
     self._widths = sorted({w for w in (8 << i for i in range(32)) if w < min(self.width, most)} | {self.width})
     # host staging of the step inputs, double-buffered: a step's async copies read one set while the host
